@@ -42,6 +42,7 @@ SOURCES = [
     "batch.cpp",
     "ingest.cu",
     "rows.cu",
+    "paged_attention.cu",
     "runner.cpp",
     "trace.cpp",
 ]

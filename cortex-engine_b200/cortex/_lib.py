@@ -90,6 +90,21 @@ class Model(ctypes.Structure):
     ]
 
 
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", _int),
+        ("B", _i32), ("H", _i32), ("Hkv", _i32), ("Dh", _i32),
+        ("q", _vp), ("q_ld_b", _i64), ("q_ld_h", _i64),
+        ("pool", _vp), ("num_pages", _i64), ("page_ld", _i64), ("row_ld", _i64),
+        ("page_size", _i32), ("page_table_width", _i32),
+        ("page_table", _vp), ("page_table_ld", _i64),
+        ("lengths", _vp),
+        ("o", _vp), ("o_ld_b", _i64), ("o_ld_h", _i64),
+        ("w_in", _vp), ("w_out", _vp), ("w_in_ld", _i64), ("w_out_ld", _i64), ("w_width", _i64),
+        ("scale", _f32),
+    ]
+
+
 class TraceRecord(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 96), ("stream", _vp), ("ms", _f32)]
 
@@ -145,6 +160,8 @@ _SIGS = {
     "ck_copy_rows": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp]),
     "ck_collate_bins_workspace_bytes": (_sz, [_i32, _i32]),
     "ck_collate_bins": (_int, [_vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _sz, _vp, _vp]),
+    "ck_paged_attention_workspace_bytes": (_sz, [ctypes.POINTER(PagedAttentionArgs)]),
+    "ck_paged_attention": (_int, [ctypes.POINTER(PagedAttentionArgs), _vp, _sz, _vp]),
 }
 
 CK_BATCH_HEADER_WORDS = 4
@@ -247,6 +264,24 @@ def stream_of(device: torch.device) -> int:
         idx = device.index
         return _raw_stream(torch.cuda.current_device() if idx is None else idx)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one (a no-op where it already is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(device)
 
 
 def require_cuda(*tensors: torch.Tensor, what: str) -> torch.device:

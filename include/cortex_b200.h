@@ -390,6 +390,44 @@ int ck_collate_bins(const ck_bin_window* windows, int32_t B, int32_t window_bins
                     int32_t n_buckets, int32_t max_neurons, int32_t* batch, int64_t capacity,
                     void* workspace, size_t workspace_bytes, int32_t* n_total, void* stream);
 
+/* ── serving operators over paged rows ────────────────────────────────────
+ * Attention of one new token per sequence over a paged K|V pool. No reference
+ * counterpart: the reference's StreamingKVCache (cortex/cache/streaming.py:79-236)
+ * hands its pages to nothing.
+ *   o[b, h] = sum_{j < lengths[b]} p_hj v_j,  p_h = softmax_j(scale q[b, h] . k_j)
+ * Position j of sequence b is row j % page_size of page page_table[b, j / page_size];
+ * a row holds K of every K|V head, then V of every head (2 * Hkv * Dh elements).
+ * Query head h reads K|V head h / (H / Hkv). A sequence of length 0 gives 0.
+ * With w_out: w_out[b, j] = w_in[b, j] + sum_h p_hj for j < lengths[b], and w_in
+ * for the rest of the w_width >= page_table_width * page_size columns; w_out may
+ * be w_in (in place: the rest is not touched). Strides in elements. A page
+ * outside the pool records CK_ERR_INDEX and its rows count as absent; a length
+ * outside [0, page_table_width * page_size] records CK_ERR_INDEX and is clamped.
+ * Dh <= 256, fp32 or bf16, fp32 statistics. The workspace (size from the query
+ * with the same arguments) is this call's alone until its kernels are done. */
+typedef struct ck_paged_attention_args {
+  int dtype;
+  int32_t B, H, Hkv, Dh;
+  const void* q; /* (B, H, Dh), Dh contiguous */
+  int64_t q_ld_b, q_ld_h;
+  const void* pool; /* (num_pages, page_size, 2 * Hkv * Dh), rows contiguous */
+  int64_t num_pages, page_ld, row_ld;
+  int32_t page_size;
+  int32_t page_table_width;
+  const int32_t* page_table; /* (B, page_table_width) */
+  int64_t page_table_ld;
+  const int32_t* lengths; /* (B,) */
+  void* o;                /* (B, H, Dh), Dh contiguous */
+  int64_t o_ld_b, o_ld_h;
+  const float* w_in; /* (B, w_width) or NULL */
+  float* w_out;
+  int64_t w_in_ld, w_out_ld, w_width;
+  float scale;
+} ck_paged_attention_args;
+size_t ck_paged_attention_workspace_bytes(const ck_paged_attention_args* args);
+int ck_paged_attention(const ck_paged_attention_args* args, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
