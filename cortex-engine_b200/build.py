@@ -43,6 +43,7 @@ SOURCES = [
     "ingest.cu",
     "rows.cu",
     "paged_attention.cu",
+    "evict.cu",
     "runner.cpp",
     "trace.cpp",
 ]

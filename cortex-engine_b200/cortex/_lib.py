@@ -105,6 +105,20 @@ class PagedAttentionArgs(ctypes.Structure):
     ]
 
 
+class EvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("elem_bytes", _int), ("B", _i32),
+        ("pool", _vp), ("num_pages", _i64), ("page_ld", _i64), ("row_ld", _i64),
+        ("page_size", _i32), ("width", _i32),
+        ("page_table", _vp), ("page_table_ld", _i64), ("page_table_width", _i32),
+        ("budget", _i32), ("recent", _i32), ("fill", _i32),
+        ("lengths", _vp), ("lengths_out", _vp),
+        ("w_in", _vp), ("w_out", _vp), ("pos_in", _vp), ("pos_out", _vp),
+        ("w_in_ld", _i64), ("w_out_ld", _i64), ("pos_in_ld", _i64), ("pos_out_ld", _i64),
+        ("in_width", _i32), ("out_width", _i32),
+    ]
+
+
 class TraceRecord(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 96), ("stream", _vp), ("ms", _f32)]
 
@@ -161,6 +175,8 @@ _SIGS = {
     "ck_collate_bins_workspace_bytes": (_sz, [_i32, _i32]),
     "ck_collate_bins": (_int, [_vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _sz, _vp, _vp]),
     "ck_paged_attention_workspace_bytes": (_sz, [ctypes.POINTER(PagedAttentionArgs)]),
+    "ck_evict_workspace_bytes": (_sz, [ctypes.POINTER(EvictArgs)]),
+    "ck_evict_by_weight": (_int, [ctypes.POINTER(EvictArgs), _vp, _sz, _vp]),
     "ck_paged_attention": (_int, [ctypes.POINTER(PagedAttentionArgs), _vp, _sz, _vp]),
 }
 

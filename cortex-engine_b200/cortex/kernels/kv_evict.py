@@ -1,0 +1,113 @@
+"""Eviction from a paged row pool by accumulated attention weight.
+
+``paged_attention`` adds up how much attention each position of a sequence has
+received; ``evict_by_weight`` keeps every sequence inside a budget of rows by
+dropping those that received least, the newest excepted. It has no counterpart
+in the reference, whose cache drops whole entries only
+(cortex/cache/streaming.py:186-195). CUDA tensors only. Launches on the current
+stream of the tensors' device, never synchronises, and allocates its workspace
+per call.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from cortex import _lib as L
+from cortex.kernels.paged_attention import check_pages
+
+
+def _table(what: str, t: torch.Tensor, dtype: torch.dtype, B: int, width: int) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"evict_by_weight: {what} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2 or t.shape[0] != B or t.shape[1] < width:
+        raise ValueError(f"evict_by_weight: {what} must be ({B}, >= {width}), got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"evict_by_weight: {what} rows must be contiguous")
+
+
+def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                    weights: torch.Tensor, positions: torch.Tensor, *, budget: int,
+                    recent: int = 0, out: tuple | None = None):
+    """Drop the rows with the least weight of every sequence over its budget.
+
+    Args:
+        pool: (num_pages, page_size, width) rows, changed in place (float32 or
+            bfloat16).
+        page_table: (B, pages) int32; slot j of sequence b is row j % page_size of
+            page ``page_table[b, j // page_size]``. A sequence's pages must be its
+            own: with a page in two places of the table, the rows in it are
+            unspecified afterwards.
+        lengths: (B,) int32 rows per sequence.
+        weights: (B, W) float32, W >= pages * page_size: the weight of each slot.
+        positions: (B, W) int32: the position of the row in each slot. Rows move, so
+            slots are not positions once a sequence has been through an eviction.
+        budget: rows a sequence may keep (>= 1).
+        recent: rows whose position is among the newest ``recent`` (position >
+            newest - recent) are kept before all others; 0 <= recent <= budget.
+        out: optional (lengths, weights, positions) to write to, each of which may be
+            the input itself (in place; otherwise they must not overlap); slots
+            behind the new lengths are left as they were. Without it new tensors:
+            weights and positions (B, budget), 0 and -1 behind the new lengths.
+
+    Of a sequence of n > budget rows the ``budget`` best stay: the newest, then by
+    weight, largest first (NaN last), equal ones by lower slot. The kept rows in
+    slots from ``budget`` on move into the freed slots before it, both in
+    ascending order, with their weight and position. Returns (lengths, weights,
+    positions); pages behind ``budget`` are free afterwards.
+
+    A length outside [0, pages * page_size] (its sequence is left alone) or a page
+    outside the pool (its rows are not copied) is recorded in the device status.
+    """
+    dev = L.require_cuda(pool, page_table, lengths, weights, positions, *(out or ()),
+                         what="evict_by_weight")
+    B = check_pages("evict_by_weight", pool, page_table, lengths)
+    if pool.dtype not in (torch.float32, torch.bfloat16):
+        raise NotImplementedError(f"evict_by_weight: rows of {pool.dtype}")
+    if pool.shape[2] < 1:
+        raise ValueError("evict_by_weight: rows must hold at least one element")
+    if not 1 <= budget < 2 ** 31 or not 0 <= recent <= budget:
+        raise ValueError(f"evict_by_weight: needs 1 <= budget and 0 <= recent <= budget, "
+                         f"got {budget} and {recent}")
+    cap = page_table.shape[1] * pool.shape[1]
+    _table("weights", weights, torch.float32, B, cap)
+    _table("positions", positions, torch.int32, B, cap)
+    fill = out is None
+    if fill:
+        out = (torch.empty(B, dtype=torch.int32, device=dev),
+               torch.empty(B, budget, dtype=torch.float32, device=dev),
+               torch.empty(B, budget, dtype=torch.int32, device=dev))
+    new_len, new_w, new_pos = out
+    if not fill:
+        if new_len.dtype != torch.int32 or new_len.shape != lengths.shape:
+            raise ValueError("evict_by_weight: out lengths must be like lengths")
+        if B > 1 and (new_len.stride(0) != 1 or lengths.stride(0) != 1):
+            raise ValueError("evict_by_weight: lengths must be contiguous")
+        _table("out weights", new_w, torch.float32, B, min(budget, cap))
+        _table("out positions", new_pos, torch.int32, B, min(budget, cap))
+    elif B > 1 and lengths.stride(0) != 1:
+        lengths = lengths.contiguous()
+    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+        page_table = page_table.contiguous()
+    a = L.EvictArgs(
+        pool.element_size(), B, pool.data_ptr(), pool.shape[0], pool.stride(0), pool.stride(1),
+        pool.shape[1], pool.shape[2], page_table.data_ptr(), page_table.stride(0),
+        page_table.shape[1], budget, recent, fill, lengths.data_ptr(), new_len.data_ptr(),
+        weights.data_ptr(), new_w.data_ptr(), positions.data_ptr(), new_pos.data_ptr(),
+        weights.stride(0), new_w.stride(0), positions.stride(0), new_pos.stride(0),
+        min(weights.shape[1], positions.shape[1]), min(new_w.shape[1], new_pos.shape[1]))
+    lib = L.load()
+    ref = ctypes.byref(a)
+    with L.on_device(dev):
+        n = lib.ck_evict_workspace_bytes(ref)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        rc = lib.ck_evict_by_weight(ref, None if ws is None else ws.data_ptr(), n,
+                                    L.stream_of(dev))
+    if rc != L.CK_OK:
+        L.check(rc, "ck_evict_by_weight")
+    return new_len, new_w, new_pos
+
+
+__all__ = ["evict_by_weight"]

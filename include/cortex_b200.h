@@ -428,6 +428,45 @@ size_t ck_paged_attention_workspace_bytes(const ck_paged_attention_args* args);
 int ck_paged_attention(const ck_paged_attention_args* args, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* Eviction from the paged pool by accumulated weight (no reference counterpart;
+ * the reference evicts whole entries, cortex/cache/streaming.py:186-195). A
+ * sequence of n = lengths[b] > budget rows keeps `budget` of them: first those
+ * with pos_in > max(pos_in[0..n)) - recent, then by w_in, largest first (NaN
+ * last, -0 equal to 0), equal ones by lower slot. The kept rows in slots >=
+ * budget move into the slots < budget of evicted rows, both in ascending
+ * order; their pool rows (width elements of elem_bytes 2 or 4), weights and
+ * positions move together. lengths_out[b] = min(n, budget). Sequences within
+ * their budget keep everything. w_out / pos_out / lengths_out may be w_in /
+ * pos_in / lengths (in place); columns from lengths_out[b] on are left as they
+ * were, or set to 0 / -1 up to out_width with fill != 0 (outputs then must
+ * not be the inputs). Pages of a sequence must be its own. A length outside
+ * [0, page_table_width * page_size] records CK_ERR_INDEX and is passed
+ * through, nothing of that sequence moves; a page outside the pool records
+ * CK_ERR_INDEX and its rows are not copied. in_width >= page_table_width *
+ * page_size, out_width >= min(budget, that), 0 <= recent <= budget, budget >= 1. */
+typedef struct ck_evict_args {
+  int elem_bytes;
+  int32_t B;
+  void* pool; /* (num_pages, page_size, width), rows contiguous */
+  int64_t num_pages, page_ld, row_ld;
+  int32_t page_size, width;
+  const int32_t* page_table; /* (B, page_table_width) */
+  int64_t page_table_ld;
+  int32_t page_table_width;
+  int32_t budget, recent, fill;
+  const int32_t* lengths; /* (B,) */
+  int32_t* lengths_out;
+  const float* w_in; /* (B, in_width) */
+  float* w_out;      /* (B, out_width) */
+  const int32_t* pos_in;
+  int32_t* pos_out;
+  int64_t w_in_ld, w_out_ld, pos_in_ld, pos_out_ld;
+  int32_t in_width, out_width;
+} ck_evict_args;
+size_t ck_evict_workspace_bytes(const ck_evict_args* args);
+int ck_evict_by_weight(const ck_evict_args* args, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif
