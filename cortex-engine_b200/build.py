@@ -44,6 +44,7 @@ SOURCES = [
     "rows.cu",
     "paged_attention.cu",
     "evict.cu",
+    "lora.cu",
     "runner.cpp",
     "trace.cpp",
 ]

@@ -119,6 +119,15 @@ class EvictArgs(ctypes.Structure):
     ]
 
 
+class LoraArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", _int), ("n_adapters", _i32), ("rank", _i32),
+        ("M", _i64), ("K", _i64), ("N", _i64),
+        ("x", _vp), ("ldx", _i64), ("w", _vp), ("ldw", _i64), ("a", _vp), ("b", _vp),
+        ("ids", _vp), ("scaling", _vp), ("bias", _vp), ("y", _vp), ("ldy", _i64),
+    ]
+
+
 class TraceRecord(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 96), ("stream", _vp), ("ms", _f32)]
 
@@ -177,6 +186,8 @@ _SIGS = {
     "ck_paged_attention_workspace_bytes": (_sz, [ctypes.POINTER(PagedAttentionArgs)]),
     "ck_evict_workspace_bytes": (_sz, [ctypes.POINTER(EvictArgs)]),
     "ck_evict_by_weight": (_int, [ctypes.POINTER(EvictArgs), _vp, _sz, _vp]),
+    "ck_lora_workspace_bytes": (_sz, [ctypes.POINTER(LoraArgs)]),
+    "ck_lora_linear": (_int, [ctypes.POINTER(LoraArgs), _vp, _sz, _vp]),
     "ck_paged_attention": (_int, [ctypes.POINTER(PagedAttentionArgs), _vp, _sz, _vp]),
 }
 

@@ -467,6 +467,33 @@ size_t ck_evict_workspace_bytes(const ck_evict_args* args);
 int ck_evict_by_weight(const ck_evict_args* args, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* A projection shared by many requests beside each one's low-rank adapter (no
+ * reference counterpart; the shared part is nn.Linear's):
+ *   y[m] = W x[m] + scaling[i] B_i (A_i x[m]) + bias,  i = ids[m], none for ids[m] < 0
+ * x (M, K), w (N, K), a (n_adapters, rank, K) and b (n_adapters, N, rank) without
+ * gaps, y (M, N); fp32 or bf16, scaling fp32 or NULL (1), bias (N,) of dtype or
+ * NULL. Sums in fp32, one rounding. An id >= n_adapters records CK_ERR_INDEX and
+ * counts as none. rank <= 256. y may not overlap an input. */
+typedef struct ck_lora_args {
+  int dtype;
+  int32_t n_adapters, rank;
+  int64_t M, K, N;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const void* a;
+  const void* b;
+  const int32_t* ids; /* (M,) */
+  const float* scaling;
+  const void* bias;
+  void* y;
+  int64_t ldy;
+} ck_lora_args;
+size_t ck_lora_workspace_bytes(const ck_lora_args* args);
+int ck_lora_linear(const ck_lora_args* args, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,256 @@
+"""lora_linear on the GPU against its definition in 64 bits.
+
+Tolerance, with u = 2^-24: every sum is fp32 over K, rank or both in some
+order, so its error is at most (K + rank + 4) u times the sum of the terms'
+magnitudes P = |W||x| + |s||B||A||x| + |bias|; the result is rounded once (2^-8
+|y| for bf16, u |y| for fp32). bf16 calls whose rows go through the tensor-core
+tiles round h = s A x to bf16 for the second product: 2^-8 |B||h|, and s A x
+itself is within (K + 1) u |s||A||x| (inside the first term).
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cortex import _lib as L
+from cortex.kernels.lora import lora_linear
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+
+
+def make(M, K, N, rank, n, dtype, seed=0, pattern="random"):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(M, K, generator=g)
+    w = torch.randn(N, K, generator=g) * K ** -0.5
+    a = torch.randn(n, rank, K, generator=g) * K ** -0.5
+    b = torch.randn(n, N, rank, generator=g) * rank ** -0.5
+    ids = {"random": lambda: torch.randint(-1, n, (M,), generator=g),
+           "runs": lambda: torch.arange(M) // 37 % (n + 1) - 1,
+           "one": lambda: torch.full((M,), n - 1),
+           "none": lambda: torch.full((M,), -3)}[pattern]()
+    scaling = torch.randn(n, generator=g)
+    bias = torch.randn(N, generator=g)
+    return ([t.to(dtype).to(DEV) for t in (x, w, a, b)] + [ids.int().to(DEV), scaling.to(DEV),
+                                                           bias.to(dtype).to(DEV)])
+
+
+def want(x, w, a, b, ids, scaling, bias):
+    x, w, a, b = (t.double().cpu() for t in (x, w, a, b))
+    ids = ids.cpu().long()
+    M, K = x.shape
+    s = torch.ones(len(a)).double() if scaling is None else scaling.double().cpu()
+    y = x @ w.t()
+    P = x.abs() @ w.abs().t()
+    H = torch.zeros_like(y)
+    for i in range(len(a)):
+        r = (ids == i).nonzero().flatten()
+        if len(r):
+            h = s[i] * (x[r] @ a[i].t())
+            y[r] += h @ b[i].t()
+            P[r] += s[i].abs() * (x[r].abs() @ a[i].abs().t()) @ b[i].abs().t()
+            H[r] = h.abs() @ b[i].abs().t()
+    if bias is not None:
+        y += bias.double().cpu()
+        P += bias.double().cpu().abs()
+    tol = (K + a.shape[1] + 4) * U * P
+    return y, tol, H
+
+
+def check(got, state, scaling=True, bias=True):
+    x, w, a, b, ids, s, bi = state
+    y, tol, H = want(x, w, a, b, ids, s if scaling else None, bi if bias else None)
+    half = 2.0 ** -8 if x.dtype == torch.bfloat16 else U
+    tol = tol + half * y.abs() + (2.0 ** -8 * H if x.dtype == torch.bfloat16 else 0)
+    err = (got.double().cpu() - y).abs()
+    assert bool((err <= tol).all()), float((err / tol.clamp(min=1e-30)).max())
+
+
+BF, F = torch.bfloat16, torch.float32
+CASES = [
+    # M, K, N, rank, adapters, dtype, pattern
+    (1, 512, 1536, 16, 4, BF, "one"),
+    (1, 64, 8, 1, 1, BF, "one"),
+    (2, 256, 100, 8, 3, BF, "random"),
+    (7, 512, 512, 16, 5, BF, "random"),
+    (8, 4096, 256, 16, 8, BF, "random"),
+    (17, 520, 264, 24, 9, BF, "random"),
+    (48, 768, 2304, 64, 64, BF, "random"),
+    (63, 1000, 77, 12, 5, BF, "random"),
+    (64, 256, 768, 4, 2, BF, "runs"),
+    (65, 256, 768, 32, 70, BF, "random"),
+    (128, 512, 256, 16, 3, BF, "none"),
+    (129, 512, 1536, 16, 8, BF, "runs"),
+    (300, 256, 768, 16, 200, BF, "random"),
+    (777, 768, 1000, 48, 24, BF, "runs"),
+    (1025, 512, 2048, 128, 7, BF, "runs"),
+    (513, 264, 520, 200, 3, BF, "random"),
+    (2000, 512, 1536, 16, 8, BF, "one"),
+    (400, 72, 77, 5, 6, BF, "runs"),
+    (33, 70, 97, 3, 4, BF, "random"),
+    (200, 70, 97, 16, 4, BF, "runs"),
+    (1, 256, 768, 8, 5, F, "one"),
+    (301, 256, 768, 8, 5, F, "runs"),
+    (130, 70, 97, 3, 4, F, "random"),
+    (1500, 512, 264, 64, 9, F, "random"),
+    (40, 1024, 64, 256, 2, F, "random"),
+]
+
+
+@pytest.mark.parametrize("M,K,N,rank,n,dtype,pattern", CASES)
+def test_against_definition(M, K, N, rank, n, dtype, pattern):
+    state = make(M, K, N, rank, n, dtype, pattern=pattern)
+    x, w, a, b, ids, s, bias = state
+    check(lora_linear(x, w, a, b, ids, scaling=s, bias=bias), state)
+    check(lora_linear(x, w, a, b, ids), state, scaling=False, bias=False)
+    assert L.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("M", [1, 20, 100, 700])
+def test_same_inputs_same_bits(M):
+    x, w, a, b, ids, s, bias = make(M, 512, 768, 16, 6, BF)
+    y = lora_linear(x, w, a, b, ids, scaling=s, bias=bias)
+    for _ in range(5):
+        assert torch.equal(y, lora_linear(x, w, a, b, ids, scaling=s, bias=bias))
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("M", [3, 40, 200, 600])
+def test_strides_and_leading_shape(M, dtype):
+    state = make(M, 512, 256, 16, 5, dtype)
+    x, w, a, b, ids, s, bias = state
+    wide = torch.full((M, 520), float("nan"), dtype=dtype, device=DEV)
+    wide[:, :512] = x
+    ww = torch.full((256, 528), float("nan"), dtype=dtype, device=DEV)
+    ww[:, 8:520] = w
+    out = torch.full((M, 300), 7.0, dtype=dtype, device=DEV)
+    got = lora_linear(wide[:, :512], ww[:, 8:520], a, b, ids, scaling=s, bias=bias,
+                      out=out[:, 8:264])
+    check(got, state)
+    assert bool((out[:, :8] == 7).all()) and bool((out[:, 264:] == 7).all())
+    odd = torch.full((M, 513), float("nan"), dtype=dtype, device=DEV)
+    odd[:, 1:] = x
+    oo = torch.full((M, 257), 7.0, dtype=dtype, device=DEV)
+    check(lora_linear(odd[:, 1:], w, a, b, ids, scaling=s, bias=bias, out=oo[:, 1:]), state)
+    assert bool((oo[:, 0] == 7).all())
+    if M % 4 == 0:
+        y = lora_linear(x.view(4, M // 4, 512), w, a, b, ids.view(4, -1), scaling=s, bias=bias)
+        assert y.shape == (4, M // 4, 256)
+        check(y.reshape(M, 256), state)
+    # adapters that are slices of a larger store, transposed weight
+    store = torch.full((5, 20, 512), float("nan"), dtype=dtype, device=DEV)
+    store[:, :16] = a
+    check(lora_linear(x, w.t().contiguous().t(), store[:, :16], b, ids, scaling=s, bias=bias), state)
+
+
+@pytest.mark.parametrize("M", [5, 64, 300, 2000])
+def test_rows_do_not_mix(M):
+    """NaN and infinities in one row, or in an adapter that no row names, stay there."""
+    x, w, a, b, ids, s, bias = state = make(M, 512, 256, 16, 5, BF)
+    ids[ids == 2] = -1
+    y = lora_linear(x, w, a, b, ids, scaling=s, bias=bias)
+    a2, b2, s2 = a.clone(), b.clone(), s.clone()
+    a2[2], b2[2], s2[2] = float("nan"), float("inf"), float("nan")
+    assert torch.equal(y, lora_linear(x, w, a2, b2, ids, scaling=s2, bias=bias))
+    x2 = x.clone()
+    x2[M // 2, 3] = float("inf")
+    y2 = lora_linear(x2, w, a, b, ids, scaling=s, bias=bias)
+    rest = torch.arange(M, device=DEV) != M // 2
+    assert torch.equal(y[rest], y2[rest])
+    assert not bool(torch.isfinite(y2[M // 2]).any())
+    # an adapter with NaN reaches its own rows only
+    a3 = a.clone()
+    a3[1, 0, 0] = float("nan")
+    y3 = lora_linear(x, w, a3, b, ids, scaling=s, bias=bias)
+    mine = ids == 1
+    assert torch.equal(y[~mine], y3[~mine]) and bool(torch.isnan(y3[mine]).all())
+
+
+@pytest.mark.parametrize("M", [5, 300])
+def test_bad_ids_are_recorded(M):
+    x, w, a, b, ids, s, bias = make(M, 512, 256, 16, 5, BF)
+    ids[::2] = 0
+    bad = ids.clone()
+    bad[1] = 5
+    bad[3] = 2 ** 31 - 1
+    none = ids.clone()
+    none[1] = none[3] = -1
+    got = lora_linear(x, w, a, b, bad, scaling=s, bias=bias)
+    with pytest.raises(IndexError):
+        L.check_device_status("lora_linear")
+    assert torch.equal(got, lora_linear(x, w, a, b, none, scaling=s, bias=bias))
+    none[:] = -2 ** 31
+    y = lora_linear(x, w, a[:0], b[:0], none, bias=bias)
+    assert torch.equal(y, lora_linear(x, w, a, b, none, scaling=s, bias=bias))
+    assert L.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("M", [4, 300, 1100])
+def test_capture_replay_and_streams(M):
+    x, w, a, b, ids, s, bias = state = make(M, 512, 768, 16, 6, BF)
+    lora_linear(x, w, a, b, ids, scaling=s, bias=bias)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(st):
+        with torch.cuda.graph(graph, stream=st):
+            y = lora_linear(x, w, a, b, ids, scaling=s, bias=bias)
+    for i in range(2):
+        x.normal_()
+        ids.copy_(torch.randint(-1, 6, (M,)))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(y, state)
+    other = make(M, 512, 768, 16, 6, BF, seed=9)
+    ox, ow, oa, ob, oids, os_, obias = other
+    s2 = torch.cuda.Stream()
+    s2.wait_stream(torch.cuda.current_stream())
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        one = [lora_linear(x, w, a, b, ids, scaling=s, bias=bias) for _ in range(20)]
+    with torch.cuda.stream(s2):
+        two = [lora_linear(ox, ow, oa, ob, oids, scaling=os_, bias=obias) for _ in range(20)]
+    torch.cuda.synchronize()
+    for p, q in zip(one, two):
+        check(p, state)
+        check(q, other)
+    assert L.device_status()[0] == 0
+
+
+def test_empty():
+    x, w, a, b, ids, s, bias = make(4, 64, 32, 8, 3, BF)
+    assert lora_linear(x[:0], w, a, b, ids[:0], scaling=s).shape == (0, 32)
+    assert lora_linear(x, w[:0], a, b[:, :0], ids).shape == (4, 0)
+
+
+def test_refusals():
+    x, w, a, b, ids, s, bias = make(4, 64, 32, 8, 3, BF)
+    with pytest.raises(ValueError):
+        lora_linear(x, w[:, :60], a, b, ids)
+    with pytest.raises(ValueError):
+        lora_linear(x, w, a[:, :, :60], b, ids)
+    with pytest.raises(ValueError):
+        lora_linear(x, w, a, b[:2], ids)
+    with pytest.raises(ValueError):
+        lora_linear(x, w, a, b[:, :, :4], ids)
+    with pytest.raises(ValueError):
+        lora_linear(x, w, a, b, ids[:3])
+    with pytest.raises(TypeError):
+        lora_linear(x, w, a, b, ids.long())
+    with pytest.raises(TypeError):
+        lora_linear(x.float(), w, a, b, ids)
+    with pytest.raises(ValueError):
+        lora_linear(x, w, a, b, ids, scaling=s.double())
+    with pytest.raises(ValueError):
+        lora_linear(x, w, a, b, ids, bias=bias[:3])
+    with pytest.raises(ValueError):
+        lora_linear(x, w, a, b, ids, out=torch.empty(4, 31, dtype=BF, device=DEV))
+    with pytest.raises(RuntimeError):
+        lora_linear(x.cpu(), w, a, b, ids)
+    with pytest.raises(NotImplementedError):
+        lora_linear(x.half(), w.half(), a.half(), b.half(), ids)
+    with pytest.raises(NotImplementedError):
+        lora_linear(x, w, torch.zeros(3, 300, 64, dtype=BF, device=DEV),
+                    torch.zeros(3, 32, 300, dtype=BF, device=DEV), ids)
