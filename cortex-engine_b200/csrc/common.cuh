@@ -599,6 +599,20 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
+// tc_mma_ss that leaves the accumulator lanes whose bit is set in `off` (128
+// bits, lane i = bit i % 32 of word i / 32) as they are.
+__device__ __forceinline__ void tc_mma_ss_masked(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                 uint32_t idesc, uint32_t accumulate, uint4 off) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(off.x), "r"(off.y), "r"(off.z),
+      "r"(off.w)
+      : "memory");
+}
+
 // 2-SM MMA (cta_group::2), issued by the even CTA of the pair: M rows split over
 // the two CTAs (A and D), B's N rows split likewise, operands at the same
 // shared-memory offsets in both CTAs.

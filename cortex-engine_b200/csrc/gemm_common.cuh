@@ -34,9 +34,16 @@ struct GemmArgs {
   // A tile by rms_gamma in shared memory and sum x^2 per row; the epilogue
   // multiplies each row by 1 / sqrt(sum / K + norm_eps).
   const __nv_bfloat16* rms_gamma;
+  // Low-rank adapters (FUSE_LORA): after its K blocks a row tile takes one
+  // block per 64 ranks of every adapter its rows name: A operand h (tmY2), B
+  // operand the adapter's (N, rank) matrix (tmR), the other rows' accumulator
+  // lanes masked off. lora_cnt[row tile] slots of lora_slots[row tile * lora_max].
+  const int* lora_cnt;
+  const uint4* lora_slots;  // two uint4 a slot: (adapter, 0, 0, 0), masked-off lanes
+  int lora_max, lora_blocks;
 };
 
-enum Fuse { FUSE_NONE = 0, FUSE_LN = 3, FUSE_RMS = 4 };
+enum Fuse { FUSE_NONE = 0, FUSE_LN = 3, FUSE_RMS = 4, FUSE_LORA = 5 };
 
 __device__ __forceinline__ int64_t residual_row(const GemmArgs& p, int m) {
   return p.aux_row_mod > 0 ? (m % p.aux_row_mod) : m;

@@ -75,6 +75,7 @@ struct GemmCfg {
   // (and always in int8 mode, whose converter warps need the registers)
   static constexpr bool LN = FUSE == 3;   // gemm::FUSE_LN
   static constexpr bool RMS = FUSE == 4;  // gemm::FUSE_RMS: a norm warpgroup scales the A tiles
+  static constexpr bool LORA = FUSE == 5;  // gemm::FUSE_LORA: adapter blocks after the K blocks
   static constexpr int EPI_WARPS =
       (WMODE != W_I8_NK && (EPI == CK_EPI_GELU || LN)) ? 16 : 8;
   static constexpr int EPI_GROUPS = EPI_WARPS / 4;  // column slices of a tile
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
                    const __grid_constant__ CUtensorMap tmR, const GemmArgs p) {
   using C = GemmCfg<BN, WMODE, FUSE, EPI, PAIR>;
   static_assert(!PAIR || (WMODE == W_BF16_NK && FUSE == 0), "PAIR: bf16 (N, K) weights, no fusion");
+  static_assert(!C::LORA || WMODE == W_BF16_NK, "FUSE_LORA: bf16 (N, K) weights");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -189,6 +191,10 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
     prefetch_tmap(&tmY);
+    if (C::LORA) {
+      prefetch_tmap(&tmY2);
+      prefetch_tmap(&tmR);
+    }
     if (C::LN) {
       prefetch_tmap(&tmY2);
       if (p.res_tma) prefetch_tmap(&tmR);
@@ -257,7 +263,10 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
       }
     }
   }
-  grid_dep_wait();
+  // FUSE_LORA: the launch before this one (lora.cu's adapter rows) lets it start
+  // only once all earlier work is done, and writes none of A, B and Y; the two
+  // threads that read its results wait for it where they first need them.
+  if (!C::LORA) grid_dep_wait();
   // Dependent grids may launch at once; FUSE_LN signals them only when its
   // epilogue is done (measured on B200: the early signal made the Cortex
   // forward 1.5-2 % slower with the fused LayerNorm, 1 % faster without it).
@@ -312,6 +321,24 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
             phase ^= 1;
           }
         }
+        if constexpr (C::LORA) {
+          grid_dep_wait();
+          const int blocks = p.lora_cnt[mt] * p.lora_blocks;
+          for (int i = 0; i < blocks; ++i) {
+            const int slot = i / p.lora_blocks, rb = i - slot * p.lora_blocks;
+            const int id = (int)p.lora_slots[2 * ((int64_t)mt * p.lora_max + slot)].x;
+            if (!mbar_wait_park(&empty[stage], phase ^ 1, abort_flag, 1)) break;
+            mbar_arrive_expect_tx(&full[stage], C::TX_BYTES);
+            tma_load_2d(sA + stage * C::A_BYTES, &tmY2, &full[stage], rb * BK, mt * BM);
+            // (rows past the adapter's N are columns that the store drops)
+            tma_load_2d(sB + stage * C::B_BYTES, &tmR, &full[stage], rb * BK, id * p.N + nt * BN);
+            ++issued;
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
       }
       // Drain: make sure every issued copy has landed before the CTA can exit
       // (PAIR: the even CTA's barriers count both CTAs' copies; the odd CTA is
@@ -363,6 +390,30 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
           if (++stage == C::STAGES) {
             stage = 0;
             phase ^= 1;
+          }
+        }
+        if constexpr (C::LORA) {
+          if (ok) grid_dep_wait();
+          const int blocks = ok ? p.lora_cnt[mt_] * p.lora_blocks : 0;
+          for (int i = 0; i < blocks; ++i) {
+            const uint4 off =
+                p.lora_slots[2 * ((int64_t)mt_ * p.lora_max + i / p.lora_blocks) + 1];
+            if (!mbar_wait(&full[stage], phase, abort_flag, 3)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(sA + stage * C::A_BYTES);
+            const uint32_t b_addr = smem_u32(sB + stage * C::B_BYTES);
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+              tc_mma_ss_masked(d_tmem, sw128_desc(a_addr + k * 32, 16, 1024),
+                               sw128_desc(b_addr + k * 32, 16, 1024), idesc, 1u, off);
+            tc_commit(&empty[stage]);
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
         }
         if (!ok) break;
@@ -535,7 +586,23 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
 #pragma unroll
             for (int i = 0; i < 32; ++i) cur[i] *= row_rstd;
           }
-          epilogue_math<EPI>(p, m, n0, cur,
+          if constexpr (C::LORA && EPI == CK_EPI_BIAS) {
+            // one rounding: the bias joins the fp32 sum
+            if (n0 + 32 <= p.N && (reinterpret_cast<uintptr_t>(p.aux) & 15u) == 0) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                float f[8];
+                unpack8(__ldg(reinterpret_cast<const uint4*>(p.aux + n0) + q), f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) cur[8 * q + i] += f[i];
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (n0 + i < p.N) cur[i] += bf2f(p.aux[n0 + i]);
+            }
+          }
+          epilogue_math<C::LORA ? CK_EPI_STORE : EPI>(p, m, n0, cur,
                              ((kPrefetch || res_box) && n0 + 32 <= p.N) ? rcur : nullptr, packed);
           if (C::LN) tmem_st16w(tbase + (uint32_t)(c * 32), packed);  // Y, for the norm pass
           if (C::LN) {
@@ -895,6 +962,13 @@ int dispatch_epi(int epi, int fuse, const CUtensorMap& ta, const CUtensorMap& tb
     if (epi == CK_EPI_BIAS) return launch_gemm<BN, WMODE, CK_EPI_BIAS, FUSE_RMS>(ta, tb, ty0, ty2, tr, a, st);
     return CK_ERR_UNSUPPORTED;
   }
+  if (fuse == gemm::FUSE_LORA) {
+    if constexpr (WMODE == W_BF16_NK) {
+      if (epi == CK_EPI_STORE) return launch_gemm<BN, WMODE, CK_EPI_STORE, gemm::FUSE_LORA>(ta, tb, ty0, ty2, tr, a, st);
+      if (epi == CK_EPI_BIAS) return launch_gemm<BN, WMODE, CK_EPI_BIAS, gemm::FUSE_LORA>(ta, tb, ty0, ty2, tr, a, st);
+    }
+    return CK_ERR_UNSUPPORTED;
+  }
   if (fuse == FUSE_LN) {
     if constexpr (BN == 256) {
       if (epi == CK_EPI_RESID) return launch_gemm<BN, WMODE, CK_EPI_RESID, FUSE_LN>(ta, tb, ty0, ty2, tr, a, st);
@@ -958,7 +1032,10 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
             int w_layout, int64_t N, int64_t ldw, const float* w_scale, int epi, const void* aux,
             int64_t ld_aux, int64_t aux_row_mod, void* Y, int64_t ldy, cudaStream_t st,
             const GemmFusion* fz) {
-  const int BN = gemm_tc_block_n(N);
+  const bool lora = fz != nullptr && fz->lora_h != nullptr;
+  int BN = gemm_tc_block_n(N);
+  // adapters: 128-wide tiles while 256-wide ones would not give every SM one
+  if (lora && ((M + BM - 1) / BM) * ((N + 255) / 256) < num_sms()) BN = 128;
   GemmArgs a;
   a.M = (int)M;
   a.N = (int)N;
@@ -980,8 +1057,19 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
   a.ln_beta = nullptr;
   a.res_tma = 0;
   a.pre_b = (fz != nullptr && fz->w_static) ? 1 : 0;
+  a.lora_cnt = nullptr;
+  a.lora_slots = nullptr;
+  a.lora_max = a.lora_blocks = 0;
   int fuse = gemm::FUSE_NONE;
-  if (fz != nullptr && fz->ln_out != nullptr) {
+  if (lora) {
+    if (w_dtype != CK_BF16 || w_layout != CK_W_NK || (epi != CK_EPI_STORE && epi != CK_EPI_BIAS))
+      return CK_ERR_UNSUPPORTED;
+    a.lora_cnt = fz->lora_cnt;
+    a.lora_slots = reinterpret_cast<const uint4*>(fz->lora_slots);
+    a.lora_max = fz->lora_max;
+    a.lora_blocks = (fz->lora_rank + BK - 1) / BK;
+    fuse = gemm::FUSE_LORA;
+  } else if (fz != nullptr && fz->ln_out != nullptr) {
     // LayerNorm of the residual output as a second output: whole rows of
     // N = 2 * 256 columns, one row block per cluster of two CTAs
     auto al16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
@@ -1040,6 +1128,10 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
     if (!make_tmap_2d(&ty2, fz->ln_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, N, M, fz->ln_ld, 64,
                       32, 128))
       return CK_ERR_INVALID_ARG;
+  } else if (lora) {
+    if (!make_tmap_2d(&ty2, fz->lora_h, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.lora_blocks * BK, M,
+                      a.lora_blocks * BK, BK, BM, 128))
+      return CK_ERR_INVALID_ARG;
   } else {
     ty2 = ty;
   }
@@ -1049,6 +1141,10 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
   if (a.res_tma) {
     if (!make_tmap_2d(&tr, aux, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, N,
                       aux_row_mod > 0 ? (uint64_t)aux_row_mod : (uint64_t)M, ld_aux, 64, 32, 128))
+      return CK_ERR_INVALID_ARG;
+  } else if (lora) {
+    if (!make_tmap_2d(&tr, fz->lora_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, fz->lora_rank,
+                      (uint64_t)fz->lora_n * N, fz->lora_b_ld, BK, BN, 128))
       return CK_ERR_INVALID_ARG;
   } else {
     tr = ty;

@@ -79,6 +79,17 @@ struct GemmFusion {
   // RMSNorm of A fused into the GEMM (bf16 A, K a multiple of 8, gamma 16-byte
   // aligned, store or bias epilogue): y = epi((x * gamma) W^T / sqrt(mean_k(x^2) + eps))
   const void* rms_gamma = nullptr;
+  // Low-rank adapters (lora.cu): y += B_i h for the adapter i of each row. h
+  // (M, 64 * ceil(rank / 64)) bf16, zero behind rank; lora_b (n * N, rank) with
+  // row stride lora_b_ld (a multiple of 8); per 128-row tile lora_cnt slots of
+  // two uint4 (adapter; rows that are not its own). Store or bias epilogue, one
+  // rounding.
+  const void* lora_h = nullptr;
+  const void* lora_b = nullptr;
+  int64_t lora_b_ld = 0;
+  int32_t lora_n = 0, lora_rank = 0, lora_max = 0;
+  const int32_t* lora_cnt = nullptr;
+  const void* lora_slots = nullptr;
 };
 // Tensor-core GEMM when supported, else the CUDA-core one (capi.cu).
 // w_static: the weight is not written by the kernel launched just before on

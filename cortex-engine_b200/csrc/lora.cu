@@ -7,8 +7,18 @@
 // rounding at the end. 2 M N K + 2 M rank (K + N) flop over each operand once:
 // a few rows are bound by reading W, many rows by the product with it.
 //
-// shrink_kernel computes h[m] = s_i A_i x[m] (fp32, rank values a row); the
-// product with W then adds B_i h[m] to its accumulator before it rounds.
+// Two launches: the first computes h[m] = s_i A_i x[m] (rank values a row), the
+// second the product with W, to whose fp32 accumulator it adds B_i h[m]:
+//   * few rows (bf16): lora_rows_kernel, W as the 128-row operand of tcgen05
+//     MMAs and the rows of x as its narrow one, K split over a cluster;
+//   * many rows (bf16): gemm_tc.cu's tiles with the adapters as further K
+//     blocks (h rounded to bf16, rows of other adapters masked off);
+//   * fp32, and layouts that TMA does not take: lora_simt_kernel.
+// Order of the launches: a kernel of the first kind waits for all earlier work
+// before it lets its successor start, and writes h and the slot lists alone.
+// The second may therefore read x and W, and write y, before its own wait for
+// the first: only the adapters' part comes after it, so the first launch runs
+// beside the product.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -19,6 +29,17 @@ namespace {
 struct LoraParams {
   ck_lora_args a;
   float* h;  // [M][rank]
+};
+
+// tensor-core path: h as bf16 rows and the adapters of every 128-row tile
+struct TileParams {
+  ck_lora_args a;
+  __nv_bfloat16* h;  // [M][ld_h], zero behind rank
+  int32_t ld_h;
+  int32_t max_slots;  // per tile
+  int32_t groups;     // 16-row groups: blocks [0, groups); then a block per tile
+  int32_t* cnt;       // [tiles]
+  uint4* slots;       // [tiles][max_slots][2]
 };
 
 __device__ __forceinline__ float tofl(float v) { return v; }
@@ -198,12 +219,336 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
   }
 }
 
+// h = s_i A_i x as bf16 for 16 rows a block, its four warps each a quarter of K
+// (matrix instructions fed from registers as in paged_attention.cu: any order of
+// the K sum will do, so every lane takes 16 bytes of a row of x and of A). One
+// pass over K per adapter that the 16 rows name, one for rows of one request.
+// Blocks behind the groups list the adapters of a 128-row tile, in the order of
+// their first row, with the rows that are not theirs.
+__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ void list_tile(const TileParams& p, int tile, int* s_id, uint32_t* s_first) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t m = (int64_t)tile * 128 + tid;
+  const int id = m < p.a.M ? adapter_of(p.a, m, true) : -1;
+  s_id[tid] = id;
+  __syncthreads();
+  const uint32_t peers = __match_any_sync(0xffffffffu, id);
+  bool first = id >= 0 && (peers & ((1u << lane) - 1u)) == 0u;
+  for (int j = 0; j < warp * 32; ++j) first = first && s_id[j] != id;
+  const uint32_t fm = __ballot_sync(0xffffffffu, first);
+  if (lane == 0) s_first[warp] = fm;
+  __syncthreads();
+  int before = __popc(fm & ((1u << lane) - 1u)), total = 0;
+  for (int w = 0; w < 4; ++w) {
+    if (w < warp) before += __popc(s_first[w]);
+    total += __popc(s_first[w]);
+  }
+  if (tid == 0) p.cnt[tile] = total;
+  if (first) {
+    uint32_t off[4];
+    for (int w = 0; w < 4; ++w) {
+      off[w] = 0u;
+      for (int j = 0; j < 32; ++j) off[w] |= (uint32_t)(s_id[w * 32 + j] != id) << j;
+    }
+    uint4* dst = p.slots + 2 * ((int64_t)tile * p.max_slots + before);
+    dst[0] = make_uint4((uint32_t)id, 0u, 0u, 0u);
+    dst[1] = make_uint4(off[0], off[1], off[2], off[3]);
+  }
+}
+
+template <int NT>
+__global__ void __launch_bounds__(128) lora_tiles_kernel(const TileParams p) {
+  __shared__ float s_part[4][16][8 * NT + 1];
+  __shared__ int s_id[128];
+  __shared__ uint32_t s_first[4];
+  grid_dep_wait();
+  grid_dep_launch();
+  if ((int)blockIdx.x >= p.groups) {
+    list_tile(p, blockIdx.x - p.groups, s_id, s_first);
+    return;
+  }
+  const ck_lora_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int64_t m0 = (int64_t)blockIdx.x * 16;
+  if (tid < 16) s_id[tid] = m0 + tid < a.M ? adapter_of(a, m0 + tid, false) : -1;
+  __syncthreads();
+  const int64_t kq = (a.K + 127) / 128 * 32;  // K per warp
+  const int64_t k_begin = warp * kq, k_end = min(a.K, k_begin + kq);
+  const bool r0 = m0 + g < a.M, r1 = m0 + g + 8 < a.M;
+  const __nv_bfloat16* x0 =
+      reinterpret_cast<const __nv_bfloat16*>(a.x) + (r0 ? m0 + g : m0) * a.ldx + 8 * t;
+  const __nv_bfloat16* x1 =
+      reinterpret_cast<const __nv_bfloat16*>(a.x) + (r1 ? m0 + g + 8 : m0) * a.ldx + 8 * t;
+  const int rows = (int)min((int64_t)16, a.M - m0);
+  for (int j0 = 0; j0 < p.ld_h; j0 += 8 * NT) {
+    // rows without an adapter, and the columns behind the rank, are zero
+    for (int i = tid; i < rows * 8 * NT; i += 128) {
+      const int r = i / (8 * NT), j = j0 + i - r * (8 * NT);
+      if (j < p.ld_h && (s_id[r] < 0 || j >= a.rank)) p.h[(m0 + r) * p.ld_h + j] = f2bf(0.f);
+    }
+    if (j0 >= a.rank) continue;
+    for (int i = 0; i < 16; ++i) {
+      const int id = s_id[i];
+      bool first = id >= 0;
+      for (int q = 0; q < i; ++q) first = first && s_id[q] != id;
+      if (!first) continue;  // (the same for every thread)
+      float acc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
+      const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) +
+                               ((int64_t)id * a.rank + j0 + g) * a.K + 8 * t;
+#pragma unroll 2
+      for (int64_t k = k_begin; k < k_end; k += 32) {
+        const bool in = k + 8 * t < a.K;  // (K is a multiple of 8)
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        const uint4 u0 = in && r0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : z;
+        const uint4 u1 = in && r1 ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : z;
+        uint4 v[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          v[nt] = in && j0 + 8 * nt + g < a.rank
+                      ? __ldg(reinterpret_cast<const uint4*>(A + (int64_t)8 * nt * a.K + k))
+                      : z;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_bf16(acc[nt], u0.x, u1.x, u0.y, u1.y, v[nt].x, v[nt].y);
+          mma_bf16(acc[nt], u0.z, u1.z, u0.w, u1.w, v[nt].z, v[nt].w);
+        }
+      }
+      __syncthreads();  // the last adapter's sums have been read
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        s_part[warp][g][8 * nt + 2 * t] = acc[nt][0];
+        s_part[warp][g][8 * nt + 2 * t + 1] = acc[nt][1];
+        s_part[warp][g + 8][8 * nt + 2 * t] = acc[nt][2];
+        s_part[warp][g + 8][8 * nt + 2 * t + 1] = acc[nt][3];
+      }
+      __syncthreads();
+      const float s = a.scaling != nullptr ? __ldg(a.scaling + id) : 1.f;
+      for (int q = tid; q < 16 * 8 * NT; q += 128) {
+        const int r = q / (8 * NT), j = q - r * (8 * NT);
+        if (s_id[r] == id && j0 + j < a.rank)
+          p.h[(m0 + r) * p.ld_h + j0 + j] =
+              f2bf(s * (s_part[0][r][j] + s_part[1][r][j] + s_part[2][r][j] + s_part[3][r][j]));
+      }
+    }
+  }
+}
+
+// Row copies with a change of stride: B rows padded to 16-byte rows (rank not
+// a multiple of 8), and y out of the padded staging rows (N or ldy not one).
+__global__ void __launch_bounds__(256) lora_copy_kernel(const __nv_bfloat16* src, int64_t ld_src,
+                                                        __nv_bfloat16* dst, int64_t ld_dst,
+                                                        int64_t rows, int64_t cols) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int64_t total = rows * cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / cols, c = i - r * cols;
+    dst[r * ld_dst + c] = src[r * ld_src + c];
+  }
+}
+
+// ── few rows ─────────────────────────────────────────────────────────────────
+//
+// W is read once and bounds the call, so it is the operand that streams: a CTA
+// takes 128 rows of W and NTOK rows of x, D[128 x NTOK] = W_tile x^T in TMEM,
+// both operands by TMA into a ring of 64-wide K blocks. The SK CTAs of a
+// cluster share a tile, each an SK-th of K, so that a small W still fills the
+// SMs; they exchange their fp32 partials through distributed shared memory,
+// each finishing NTOK / SK of the rows: sum over the ranks in order, adapter
+// and bias added, one rounding, a warp storing 32 neighbouring columns.
+
+template <int NTOK, int SK>
+struct RowsCfg {
+  static constexpr int W_BYTES = 128 * 128;
+  static constexpr int X_BYTES = NTOK * 128;
+  static constexpr int STAGE = W_BYTES + X_BYTES;
+  static constexpr int STAGES = 5;
+  static constexpr int PART = 128 * NTOK * 4;  // partials, over the ring once it is drained
+  static constexpr int RING = STAGES * STAGE > PART ? STAGES * STAGE : PART;
+  static constexpr int SMEM = 1024 + RING + 256;
+  static constexpr uint32_t COLS = NTOK < 32 ? 32 : NTOK;
+};
+
+template <int NTOK, int SK>
+__global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ CUtensorMap tmW,
+                                                        const __grid_constant__ CUtensorMap tmX,
+                                                        const LoraParams p, int n_tiles) {
+  using C = RowsCfg<NTOK, SK>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint8_t* sW = smem;
+  uint8_t* sX = smem + C::STAGES * C::W_BYTES;
+  float* part = reinterpret_cast<float*>(smem);  // [NTOK][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::RING);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* done = empty + C::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const ck_lora_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = SK > 1 ? (int)cl_rank() : 0;
+  const int unit = blockIdx.x / SK;
+  const int n0 = (unit % n_tiles) * 128;
+  const int64_t m0 = (int64_t)(unit / n_tiles) * NTOK;
+  const int kb_all = (int)((a.K + 63) / 64);
+  const int kb_per = (kb_all + SK - 1) / SK;
+  const int kb0 = min(kb_all, rank * kb_per), kb1 = min(kb_all, kb0 + kb_per);
+
+  if (tid == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    prefetch_tmap(&tmW);
+    prefetch_tmap(&tmX);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  bool ok = true;
+  if (warp == 0 && lane == 0) {
+    int issued = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++issued) {
+      const int s = issued % C::STAGES;
+      if (!mbar_wait(&empty[s], ((issued / C::STAGES) & 1) ^ 1, abort_flag, 20)) break;
+      mbar_arrive_expect_tx(&full[s], C::STAGE);
+      tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], kb * 64, n0);
+      tma_load_2d(sX + s * C::X_BYTES, &tmX, &full[s], kb * 64, (int)m0);
+    }
+    // every copy lands before this CTA can exit or reuse the ring
+    for (int s = 0; s < C::STAGES && s < issued; ++s) {
+      const int last = issued - 1 - ((issued - 1 - s) % C::STAGES);
+      mbar_wait(&full[s], (uint32_t)((last / C::STAGES) & 1), nullptr, 21);
+    }
+  } else if (warp == 1 && lane == 0) {
+    constexpr uint32_t idesc = idesc_bf16(128, NTOK, 0u);
+    int i = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++i) {
+      const int s = i % C::STAGES;
+      if (!mbar_wait(&full[s], (uint32_t)((i / C::STAGES) & 1), abort_flag, 22)) break;
+      tc_fence_after();
+      const uint32_t wa = smem_u32(sW + s * C::W_BYTES), xa = smem_u32(sX + s * C::X_BYTES);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        tc_mma_ss(tmem, sw128_desc(wa + k * 32, 16, 1024), sw128_desc(xa + k * 32, 16, 1024), idesc,
+                  (i | k) != 0 ? 1u : 0u);
+      tc_commit(&empty[s]);
+    }
+    tc_commit(done);
+    mbar_wait(done, 0, nullptr, 23);
+  }
+  __syncthreads();  // (the two threads above come back once the ring is drained)
+  tc_fence_after();
+  ok = *abort_flag == 0;
+
+  // partials: lane n of the accumulator, column by column
+  {
+    const uint32_t base = tmem + ((uint32_t)(warp * 32) << 16);
+#pragma unroll
+    for (int c = 0; c < NTOK; c += 16) {
+      uint32_t v[16];
+      if (kb1 > kb0) {
+        tmem_ld16w(base + c, v);
+        tc_wait_ld();
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        part[(c + i) * 128 + tid] = kb1 > kb0 ? __uint_as_float(v[i]) : 0.f;
+    }
+  }
+  tc_fence_before();
+  grid_dep_wait();  // h is there
+  grid_dep_launch();
+  if (SK > 1) cl_sync(); else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::COLS);
+  }
+  const int n = n0 + tid;
+  if (ok && n < a.N) {
+    constexpr int PER = (NTOK + SK - 1) / SK;
+    uint32_t src[SK];
+#pragma unroll
+    for (int r = 0; r < SK; ++r) src[r] = SK > 1 ? cl_map(part + tid, r) : smem_u32(part + tid);
+    const float bias = a.bias != nullptr ? bf2f(reinterpret_cast<const __nv_bfloat16*>(a.bias)[n]) : 0.f;
+    const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b);
+    const bool vec = a.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(B) & 15u) == 0;
+    for (int i = 0; i < PER; ++i) {
+      const int c = rank * PER + i;
+      const int64_t m = m0 + c;
+      if (c >= NTOK || m >= a.M) break;
+      float v = 0.f;
+#pragma unroll
+      for (int r = 0; r < SK; ++r) {
+        float f;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(src[r] + c * 512) : "memory");
+        v += f;
+      }
+      const int id = adapter_of(a, m, false);
+      if (id >= 0) {
+        const __nv_bfloat16* br = B + ((int64_t)id * a.N + n) * a.rank;
+        const float* h = p.h + m * a.rank;
+        float d = 0.f;
+        if (vec) {
+          for (int j = 0; j < a.rank; j += 8) {
+            float f[8];
+            load16(br + j, f);
+            const float4 h0 = *reinterpret_cast<const float4*>(h + j);
+            const float4 h1 = *reinterpret_cast<const float4*>(h + j + 4);
+            d = fmaf(f[0], h0.x, d); d = fmaf(f[1], h0.y, d);
+            d = fmaf(f[2], h0.z, d); d = fmaf(f[3], h0.w, d);
+            d = fmaf(f[4], h1.x, d); d = fmaf(f[5], h1.y, d);
+            d = fmaf(f[6], h1.z, d); d = fmaf(f[7], h1.w, d);
+          }
+        } else {
+          for (int j = 0; j < a.rank; ++j) d = fmaf(bf2f(br[j]), h[j], d);
+        }
+        v += d;
+      }
+      reinterpret_cast<__nv_bfloat16*>(a.y)[m * a.ldy + n] = f2bf(v + bias);
+    }
+  }
+  if (SK > 1) cl_sync();  // no CTA leaves while another reads its partials
+}
+
+enum Path { PATH_ROWS, PATH_TILES, PATH_SIMT };
+
 struct LoraPlan {
   LoraParams p;
+  Path path;
+  int ld_h, max_slots, tiles;     // PATH_TILES
+  int64_t ld_b, ld_stage;         // packed B / staged y row strides, 0: used in place
+  size_t off_h, off_cnt, off_slots, off_b, off_y;
   size_t bytes;
 };
 
 bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
+
+// Rows up to which lora_rows_kernel runs (tensor-core tiles above).
+constexpr int64_t kRowsMax = 128;
 
 int make_plan(const ck_lora_args& a, LoraPlan& pl) {
   if (a.dtype != CK_F32 && a.dtype != CK_BF16) return CK_ERR_UNSUPPORTED;
@@ -213,7 +558,26 @@ int make_plan(const ck_lora_args& a, LoraPlan& pl) {
   if (((a.M + 63) / 64) * ((a.N + 63) / 64) > INT32_MAX || (a.M * a.rank + 7) / 8 > INT32_MAX)
     return CK_ERR_UNSUPPORTED;
   pl.p.a = a;
-  pl.bytes = (size_t)a.M * a.rank * 4;
+  auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+  const bool tma = a.dtype == CK_BF16 && a.K % 8 == 0 && a.ldx % 8 == 0 && a.ldw % 8 == 0 &&
+                   aligned16(a.x) && aligned16(a.w) && aligned16(a.a) && aligned16(a.b) &&
+                   (int64_t)a.n_adapters * a.N <= INT32_MAX - 256;
+  pl.path = !tma ? PATH_SIMT : (a.M <= kRowsMax ? PATH_ROWS : PATH_TILES);
+  if (pl.path != PATH_TILES) {
+    pl.bytes = up((size_t)a.M * a.rank * 4);
+    return CK_OK;
+  }
+  pl.ld_h = (a.rank + 63) / 64 * 64;
+  pl.tiles = (int)((a.M + 127) / 128);
+  pl.max_slots = a.n_adapters < 1 ? 1 : (a.n_adapters < 128 ? a.n_adapters : 128);
+  pl.ld_b = a.rank % 8 == 0 ? 0 : (a.rank + 7) / 8 * 8;
+  pl.ld_stage = a.ldy % 8 == 0 && aligned16(a.y) ? 0 : (a.N + 7) / 8 * 8;
+  pl.off_h = 0;
+  pl.off_cnt = up((size_t)a.M * pl.ld_h * 2);
+  pl.off_slots = pl.off_cnt + up((size_t)pl.tiles * 4);
+  pl.off_b = pl.off_slots + up((size_t)pl.tiles * pl.max_slots * 32);
+  pl.off_y = pl.off_b + up((size_t)a.n_adapters * a.N * pl.ld_b * 2);
+  pl.bytes = pl.off_y + up((size_t)a.M * pl.ld_stage * 2);
   return CK_OK;
 }
 
@@ -234,6 +598,101 @@ int shrink(const LoraParams& p, cudaStream_t st) {
              : launch_pdl(lora_shrink_kernel<T, 1, false>, grid, dim3(256), 0, st, p, jblocks);
 }
 
+template <int NTOK, int SK>
+int launch_rows(const LoraParams& p, cudaStream_t st) {
+  using C = RowsCfg<NTOK, SK>;
+  const ck_lora_args& a = p.a;
+  CUtensorMap tw, tx;
+  if (!make_tmap_2d(&tw, a.w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.K, a.N, a.ldw, 64, 128, 128) ||
+      !make_tmap_2d(&tx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.K, a.M, a.ldx, 64, NTOK, 128))
+    return CK_ERR_INVALID_ARG;
+  auto kern = lora_rows_kernel<NTOK, SK>;
+  if (!smem_attr_ready(reinterpret_cast<const void*>(kern), C::SMEM)) return record_cuda_error();
+  const int n_tiles = (int)((a.N + 127) / 128);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = SK;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n_tiles * ((a.M + NTOK - 1) / NTOK) * SK));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = (size_t)C::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return launch_cfg(cfg, kern, tw, tx, p, n_tiles);
+}
+
+template <int NTOK>
+int launch_rows_k(const LoraParams& p, cudaStream_t st) {
+  // K split until the tiles give every SM a CTA (or a CTA one K block)
+  const int64_t units = (p.a.N + 127) / 128 * ((p.a.M + NTOK - 1) / NTOK);
+  const int64_t kb = (p.a.K + 63) / 64;
+  const int sms = num_sms() > 0 ? num_sms() : 148;
+  int sk = 1;
+  while (sk < 8 && units * sk < sms && kb >= 2 * sk) sk *= 2;
+  if (sk == 8) return launch_rows<NTOK, 8>(p, st);
+  if (sk == 4) return launch_rows<NTOK, 4>(p, st);
+  if (sk == 2) return launch_rows<NTOK, 2>(p, st);
+  return launch_rows<NTOK, 1>(p, st);
+}
+
+int copy_strided(const void* src, int64_t ld_src, void* dst, int64_t ld_dst, int64_t rows,
+                 int64_t cols, cudaStream_t st) {
+  int64_t blocks = (rows * cols + 1023) / 1024;
+  const int64_t most = 16 * (int64_t)num_sms();
+  if (blocks > most) blocks = most;
+  return launch_pdl(lora_copy_kernel, dim3((unsigned)blocks), dim3(256), 0, st,
+                    reinterpret_cast<const __nv_bfloat16*>(src), ld_src,
+                    reinterpret_cast<__nv_bfloat16*>(dst), ld_dst, rows, cols);
+}
+
+int run_tiles(const LoraPlan& pl, uint8_t* ws, cudaStream_t st) {
+  const ck_lora_args& a = pl.p.a;
+  int rc;
+  const void* b = a.b;
+  if (pl.ld_b > 0 && a.n_adapters > 0) {
+    b = ws + pl.off_b;
+    rc = copy_strided(a.b, a.rank, ws + pl.off_b, pl.ld_b, a.n_adapters * a.N, a.rank, st);
+    if (rc != CK_OK) return rc;
+  }
+  TileParams t;
+  t.a = a;
+  t.h = reinterpret_cast<__nv_bfloat16*>(ws + pl.off_h);
+  t.ld_h = pl.ld_h;
+  t.max_slots = pl.max_slots;
+  t.groups = (int32_t)((a.M + 15) / 16);
+  t.cnt = reinterpret_cast<int32_t*>(ws + pl.off_cnt);
+  t.slots = reinterpret_cast<uint4*>(ws + pl.off_slots);
+  const dim3 grid((unsigned)(t.groups + pl.tiles));
+  if (a.rank <= 16)
+    rc = launch_pdl(lora_tiles_kernel<2>, grid, dim3(128), 0, st, t);
+  else if (a.rank <= 32)
+    rc = launch_pdl(lora_tiles_kernel<4>, grid, dim3(128), 0, st, t);
+  else
+    rc = launch_pdl(lora_tiles_kernel<8>, grid, dim3(128), 0, st, t);
+  if (rc != CK_OK) return rc;
+  GemmFusion fz;
+  fz.lora_h = t.h;
+  // without any adapter no slot is listed and no block reads b
+  fz.lora_b = a.n_adapters > 0 ? b : a.w;
+  fz.lora_n = a.n_adapters > 0 ? a.n_adapters : 1;
+  fz.lora_b_ld = pl.ld_b > 0 ? pl.ld_b : a.rank;
+  fz.lora_rank = a.rank;
+  fz.lora_max = pl.max_slots;
+  fz.lora_cnt = t.cnt;
+  fz.lora_slots = t.slots;
+  void* y = pl.ld_stage > 0 ? ws + pl.off_y : a.y;
+  const int64_t ldy = pl.ld_stage > 0 ? pl.ld_stage : a.ldy;
+  rc = gemm_tc(a.x, a.M, a.K, a.ldx, a.w, CK_BF16, CK_W_NK, a.N, a.ldw, nullptr,
+               a.bias != nullptr ? CK_EPI_BIAS : CK_EPI_STORE, a.bias, 0, 0, y, ldy, st, &fz);
+  if (rc != CK_OK || pl.ld_stage == 0) return rc;
+  return copy_strided(y, ldy, a.y, a.ldy, a.M, a.N, st);
+}
+
 }  // namespace
 
 int lora_linear(const ck_lora_args& a, void* ws, size_t ws_bytes, cudaStream_t st) {
@@ -244,7 +703,16 @@ int lora_linear(const ck_lora_args& a, void* ws, size_t ws_bytes, cudaStream_t s
   if (!a.x || !a.w || !a.y || !a.ids || (a.n_adapters > 0 && (!a.a || !a.b)))
     return CK_ERR_INVALID_ARG;
   if (ws == nullptr || ws_bytes < pl.bytes || !aligned16(ws)) return CK_ERR_WORKSPACE;
+  if (pl.path == PATH_TILES) return run_tiles(pl, reinterpret_cast<uint8_t*>(ws), st);
   pl.p.h = reinterpret_cast<float*>(ws);
+  if (pl.path == PATH_ROWS) {
+    rc = shrink<__nv_bfloat16>(pl.p, st);
+    if (rc != CK_OK) return rc;
+    if (a.M <= 16) return launch_rows_k<16>(pl.p, st);
+    if (a.M <= 32) return launch_rows_k<32>(pl.p, st);
+    if (a.M <= 64) return launch_rows_k<64>(pl.p, st);
+    return launch_rows_k<128>(pl.p, st);
+  }
   const bool bf = a.dtype == CK_BF16;
   rc = bf ? shrink<__nv_bfloat16>(pl.p, st) : shrink<float>(pl.p, st);
   if (rc != CK_OK) return rc;
