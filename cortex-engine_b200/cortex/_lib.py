@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -128,6 +129,15 @@ class LoraArgs(ctypes.Structure):
     ]
 
 
+# The argument blocks of the serving operators as struct formats (native layout,
+# the fields of PagedAttentionArgs, EvictArgs and LoraArgs in order): packing a
+# block this way costs a tenth of filling a ctypes.Structure, on calls whose
+# kernels take a few microseconds.
+PAGED_ATTENTION_ARGS = struct.Struct("@5iP2qP3q2iPqPP2q2P3qf0q")
+EVICT_ARGS = struct.Struct("@2iP3q2iPq4i6P4q2i0q")
+LORA_ARGS = struct.Struct("@3i3qPqPq2PPPPPq0q")
+
+
 class TraceRecord(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 96), ("stream", _vp), ("ms", _f32)]
 
@@ -183,12 +193,12 @@ _SIGS = {
     "ck_copy_rows": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp]),
     "ck_collate_bins_workspace_bytes": (_sz, [_i32, _i32]),
     "ck_collate_bins": (_int, [_vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _sz, _vp, _vp]),
-    "ck_paged_attention_workspace_bytes": (_sz, [ctypes.POINTER(PagedAttentionArgs)]),
-    "ck_evict_workspace_bytes": (_sz, [ctypes.POINTER(EvictArgs)]),
-    "ck_evict_by_weight": (_int, [ctypes.POINTER(EvictArgs), _vp, _sz, _vp]),
-    "ck_lora_workspace_bytes": (_sz, [ctypes.POINTER(LoraArgs)]),
-    "ck_lora_linear": (_int, [ctypes.POINTER(LoraArgs), _vp, _sz, _vp]),
-    "ck_paged_attention": (_int, [ctypes.POINTER(PagedAttentionArgs), _vp, _sz, _vp]),
+    "ck_paged_attention_workspace_bytes": (_sz, [_vp]),
+    "ck_evict_workspace_bytes": (_sz, [_vp]),
+    "ck_evict_by_weight": (_int, [_vp, _vp, _sz, _vp]),
+    "ck_lora_workspace_bytes": (_sz, [_vp]),
+    "ck_lora_linear": (_int, [_vp, _vp, _sz, _vp]),
+    "ck_paged_attention": (_int, [_vp, _vp, _sz, _vp]),
 }
 
 CK_BATCH_HEADER_WORDS = 4
@@ -291,6 +301,19 @@ def stream_of(device: torch.device) -> int:
         idx = device.index
         return _raw_stream(torch.cuda.current_device() if idx is None else idx)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_ws_bytes: dict = {}
+
+
+def workspace_bytes(query, key: tuple, block: bytes) -> int:
+    """``query(block)``, remembered per ``key`` (the call's sizes)."""
+    n = _ws_bytes.get(key)
+    if n is None:
+        if len(_ws_bytes) > 4096:
+            _ws_bytes.clear()
+        n = _ws_bytes[key] = query(block)
+    return n
 
 
 class _NoGuard:

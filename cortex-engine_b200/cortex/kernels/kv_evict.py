@@ -11,12 +11,12 @@ per call.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from cortex import _lib as L
-from cortex.kernels.paged_attention import check_pages
+from cortex.kernels.paged_attention import check_pages, rows_contiguous
+
+_pack = L.EVICT_ARGS.pack
 
 
 def _table(what: str, t: torch.Tensor, dtype: torch.dtype, B: int, width: int) -> None:
@@ -24,7 +24,7 @@ def _table(what: str, t: torch.Tensor, dtype: torch.dtype, B: int, width: int) -
         raise TypeError(f"evict_by_weight: {what} must be {dtype}, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] != B or t.shape[1] < width:
         raise ValueError(f"evict_by_weight: {what} must be ({B}, >= {width}), got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    if not rows_contiguous(t):
         raise ValueError(f"evict_by_weight: {what} rows must be contiguous")
 
 
@@ -61,50 +61,53 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
     A length outside [0, pages * page_size] (its sequence is left alone) or a page
     outside the pool (its rows are not copied) is recorded in the device status.
     """
-    dev = L.require_cuda(pool, page_table, lengths, weights, positions, *(out or ()),
-                         what="evict_by_weight")
-    B = check_pages("evict_by_weight", pool, page_table, lengths)
-    if pool.dtype not in (torch.float32, torch.bfloat16):
+    d = pool.get_device()
+    if d < 0 or page_table.get_device() != d or lengths.get_device() != d or \
+            weights.get_device() != d or positions.get_device() != d or out is not None:
+        L.require_cuda(pool, page_table, lengths, weights, positions, *(out or ()),
+                       what="evict_by_weight")
+    check_pages("evict_by_weight", pool, page_table, lengths)
+    if pool.dtype != torch.bfloat16 and pool.dtype != torch.float32:
         raise NotImplementedError(f"evict_by_weight: rows of {pool.dtype}")
-    if pool.shape[2] < 1:
-        raise ValueError("evict_by_weight: rows must hold at least one element")
     if not 1 <= budget < 2 ** 31 or not 0 <= recent <= budget:
         raise ValueError(f"evict_by_weight: needs 1 <= budget and 0 <= recent <= budget, "
                          f"got {budget} and {recent}")
-    cap = page_table.shape[1] * pool.shape[1]
+    B = lengths.shape[0]
+    pages, page_size, width = pool.shape
+    table_width = page_table.shape[1]
+    cap = table_width * page_size
     _table("weights", weights, torch.float32, B, cap)
     _table("positions", positions, torch.int32, B, cap)
+    dev = pool.device
     fill = out is None
     if fill:
-        out = (torch.empty(B, dtype=torch.int32, device=dev),
-               torch.empty(B, budget, dtype=torch.float32, device=dev),
-               torch.empty(B, budget, dtype=torch.int32, device=dev))
-    new_len, new_w, new_pos = out
-    if not fill:
+        new_len = torch.empty(B, dtype=torch.int32, device=dev)
+        new_w = torch.empty(B, budget, dtype=torch.float32, device=dev)
+        new_pos = torch.empty(B, budget, dtype=torch.int32, device=dev)
+        if not rows_contiguous(lengths):
+            lengths = lengths.contiguous()
+    else:
+        new_len, new_w, new_pos = out
         if new_len.dtype != torch.int32 or new_len.shape != lengths.shape:
             raise ValueError("evict_by_weight: out lengths must be like lengths")
-        if B > 1 and (new_len.stride(0) != 1 or lengths.stride(0) != 1):
+        if not rows_contiguous(new_len) or not rows_contiguous(lengths):
             raise ValueError("evict_by_weight: lengths must be contiguous")
         _table("out weights", new_w, torch.float32, B, min(budget, cap))
         _table("out positions", new_pos, torch.int32, B, min(budget, cap))
-    elif B > 1 and lengths.stride(0) != 1:
-        lengths = lengths.contiguous()
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+    if not rows_contiguous(page_table):
         page_table = page_table.contiguous()
-    a = L.EvictArgs(
-        pool.element_size(), B, pool.data_ptr(), pool.shape[0], pool.stride(0), pool.stride(1),
-        pool.shape[1], pool.shape[2], page_table.data_ptr(), page_table.stride(0),
-        page_table.shape[1], budget, recent, fill, lengths.data_ptr(), new_len.data_ptr(),
-        weights.data_ptr(), new_w.data_ptr(), positions.data_ptr(), new_pos.data_ptr(),
-        weights.stride(0), new_w.stride(0), positions.stride(0), new_pos.stride(0),
-        min(weights.shape[1], positions.shape[1]), min(new_w.shape[1], new_pos.shape[1]))
+    page_ld, row_ld, _ = pool.stride()
+    block = _pack(pool.element_size(), B, pool.data_ptr(), pages, page_ld, row_ld, page_size, width,
+                  page_table.data_ptr(), page_table.stride(0), table_width, budget, recent, fill,
+                  lengths.data_ptr(), new_len.data_ptr(), weights.data_ptr(), new_w.data_ptr(),
+                  positions.data_ptr(), new_pos.data_ptr(), weights.stride(0), new_w.stride(0),
+                  positions.stride(0), new_pos.stride(0),
+                  min(weights.shape[1], positions.shape[1]), min(new_w.shape[1], new_pos.shape[1]))
     lib = L.load()
-    ref = ctypes.byref(a)
     with L.on_device(dev):
-        n = lib.ck_evict_workspace_bytes(ref)
+        n = L.workspace_bytes(lib.ck_evict_workspace_bytes, ("evict", d, B, cap, budget), block)
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        rc = lib.ck_evict_by_weight(ref, None if ws is None else ws.data_ptr(), n,
-                                    L.stream_of(dev))
+        rc = lib.ck_evict_by_weight(block, ws.data_ptr() if n else 0, n, L.stream_of(dev))
     if rc != L.CK_OK:
         L.check(rc, "ck_evict_by_weight")
     return new_len, new_w, new_pos

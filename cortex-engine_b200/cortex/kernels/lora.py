@@ -11,11 +11,12 @@ synchronises, and allocates its workspace per call.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from cortex import _lib as L
+from cortex.kernels.paged_attention import rows_contiguous
+
+_pack = L.LORA_ARGS.pack
 
 
 def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
@@ -38,63 +39,81 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     device status (IndexError from ``_lib.check_device_status``) and its row gets
     no adapter.
     """
-    dev = L.require_cuda(x, w, lora_a, lora_b, adapter_ids, scaling, bias, out,
-                         what="lora_linear")
+    d = x.get_device()
+    if d < 0 or w.get_device() != d or lora_a.get_device() != d or lora_b.get_device() != d or \
+            adapter_ids.get_device() != d or \
+            (scaling is not None and scaling.get_device() != d) or \
+            (bias is not None and bias.get_device() != d) or out is not None:
+        L.require_cuda(x, w, lora_a, lora_b, adapter_ids, scaling, bias, out, what="lora_linear")
+    dtype, lead = x.dtype, x.shape[:-1]
     K = x.shape[-1] if x.dim() > 0 else -1
     if w.dim() != 2 or w.shape[1] != K or K < 1:
         raise ValueError(f"lora_linear: w must be (N, K) with K = {K}, got {tuple(w.shape)}")
     N = w.shape[0]
     if lora_a.dim() != 3 or lora_a.shape[2] != K or lora_a.shape[1] < 1:
         raise ValueError(f"lora_linear: lora_a must be (n, rank, {K}), got {tuple(lora_a.shape)}")
-    n, rank = lora_a.shape[0], lora_a.shape[1]
+    n, rank, _ = lora_a.shape
     if lora_b.shape != (n, N, rank):
         raise ValueError(f"lora_linear: lora_b must be {(n, N, rank)}, got {tuple(lora_b.shape)}")
-    if not x.dtype == w.dtype == lora_a.dtype == lora_b.dtype:
-        raise TypeError(f"lora_linear: x, w, lora_a and lora_b differ in dtype ({x.dtype}, "
+    if dtype != w.dtype or dtype != lora_a.dtype or dtype != lora_b.dtype:
+        raise TypeError(f"lora_linear: x, w, lora_a and lora_b differ in dtype ({dtype}, "
                         f"{w.dtype}, {lora_a.dtype}, {lora_b.dtype})")
     if adapter_ids.dtype != torch.int32:
         raise TypeError(f"lora_linear: adapter_ids must be int32, got {adapter_ids.dtype}")
-    lead = x.shape[:-1]
     if adapter_ids.shape != lead:
         raise ValueError(f"lora_linear: adapter_ids must be {tuple(lead)}, "
                          f"got {tuple(adapter_ids.shape)}")
-    if scaling is not None and (scaling.dtype != torch.float32 or scaling.shape != (n,)):
-        raise ValueError(f"lora_linear: scaling must be float32 ({n},)")
-    if bias is not None and (bias.dtype != x.dtype or bias.shape != (N,)):
-        raise ValueError(f"lora_linear: bias must be {x.dtype} ({N},)")
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    if x2.stride(1) != 1:
+    ids, x2 = adapter_ids, x
+    if len(lead) != 1:
+        ids, x2 = ids.reshape(-1), x.reshape(-1, K)
+    if not rows_contiguous(x2):
         x2 = x2.contiguous()
-    if w.stride(1) != 1:
+    if not rows_contiguous(w):
         w = w.contiguous()
-    M = x2.shape[0]
-    ids = adapter_ids.reshape(-1).contiguous()
-    lora_a, lora_b = lora_a.contiguous(), lora_b.contiguous()
+    if not rows_contiguous(ids):
+        ids = ids.contiguous()
+    if not lora_a.is_contiguous():
+        lora_a = lora_a.contiguous()
+    if not lora_b.is_contiguous():
+        lora_b = lora_b.contiguous()
+    scaling_ptr = bias_ptr = 0
     if scaling is not None:
+        if scaling.dtype != torch.float32 or scaling.shape != (n,):
+            raise ValueError(f"lora_linear: scaling must be float32 ({n},)")
         scaling = scaling.contiguous()
+        scaling_ptr = scaling.data_ptr()
     if bias is not None:
+        if bias.dtype != dtype or bias.shape != (N,):
+            raise ValueError(f"lora_linear: bias must be {dtype} ({N},)")
         bias = bias.contiguous()
+        bias_ptr = bias.data_ptr()
+    M, dev = x2.shape[0], x.device
     if out is None:
-        y = torch.empty(M, N, dtype=x.dtype, device=dev)
+        y = torch.empty(M, N, dtype=dtype, device=dev)
     else:
-        if out.shape != (*lead, N) or out.dtype != x.dtype:
-            raise ValueError(f"lora_linear: out must be {x.dtype} {(*lead, N)}")
+        if out.shape != (*lead, N) or out.dtype != dtype:
+            raise ValueError(f"lora_linear: out must be {dtype} {(*lead, N)}")
         y = out if out.dim() == 2 else out.view(M, N)
-        if N > 1 and y.stride(1) != 1:
+        if not rows_contiguous(y):
             raise ValueError("lora_linear: out rows must be contiguous")
-    a = L.LoraArgs(
-        L.dtype_code(x.dtype), n, rank, M, K, N, x2.data_ptr(), x2.stride(0), w.data_ptr(),
-        w.stride(0), lora_a.data_ptr(), lora_b.data_ptr(), ids.data_ptr(), L.ptr(scaling),
-        L.ptr(bias), y.data_ptr(), y.stride(0))
+    x_ptr, w_ptr, y_ptr = x2.data_ptr(), w.data_ptr(), y.data_ptr()
+    a_ptr, b_ptr = lora_a.data_ptr(), lora_b.data_ptr()
+    ldx, ldw, ldy = x2.stride(0), w.stride(0), y.stride(0)
+    block = _pack(L.dtype_code(dtype), n, rank, M, K, N, x_ptr, ldx, w_ptr, ldw, a_ptr, b_ptr,
+                  ids.data_ptr(), scaling_ptr, bias_ptr, y_ptr, ldy)
     lib = L.load()
-    ref = ctypes.byref(a)
     with L.on_device(dev):
-        nb = lib.ck_lora_workspace_bytes(ref)
+        # everything the size depends on, alignment included
+        key = ("lora", d, dtype, M, K, N, rank, n, (ldx | ldw | ldy) & 7, ldy & 7,
+               (x_ptr | w_ptr | a_ptr | b_ptr) & 15, y_ptr & 15)
+        nb = L.workspace_bytes(lib.ck_lora_workspace_bytes, key, block)
         ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        rc = lib.ck_lora_linear(ref, None if ws is None else ws.data_ptr(), nb, L.stream_of(dev))
+        rc = lib.ck_lora_linear(block, ws.data_ptr() if nb else 0, nb, L.stream_of(dev))
     if rc != L.CK_OK:
         L.check(rc, "ck_lora_linear")
-    return out if out is not None else (y if x.dim() == 2 else y.reshape(*lead, N))
+    if out is not None:
+        return out
+    return y if len(lead) == 1 else y.reshape(*lead, N)
 
 
 __all__ = ["lora_linear"]

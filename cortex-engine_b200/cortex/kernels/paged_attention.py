@@ -13,31 +13,33 @@ and captured graphs do not share memory.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from cortex import _lib as L
 
+_pack = L.PAGED_ATTENTION_ARGS.pack
+
 
 def check_pages(what: str, pool: torch.Tensor, page_table: torch.Tensor,
-                lengths: torch.Tensor) -> int:
-    """Shape checks shared by the operators over a paged pool; returns B."""
+                lengths: torch.Tensor) -> None:
+    """Checks shared by the operators over a paged pool."""
     if pool.dim() != 3:
         raise ValueError(f"{what}: pool must be (num_pages, page_size, width), "
                          f"got {tuple(pool.shape)}")
     if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
         raise TypeError(f"{what}: page_table and lengths must be int32, got "
                         f"{page_table.dtype} and {lengths.dtype}")
-    B = lengths.shape[0] if lengths.dim() == 1 else -1
-    if page_table.dim() != 2 or page_table.shape[0] != B:
+    if page_table.dim() != 2 or lengths.dim() != 1 or page_table.shape[0] != lengths.shape[0]:
         raise ValueError(f"{what}: page_table must be (B, pages) beside lengths (B,), got "
                          f"{tuple(page_table.shape)} and {tuple(lengths.shape)}")
-    if pool.shape[1] < 1:
-        raise ValueError(f"{what}: pages must hold at least one row")
+    if pool.shape[1] < 1 or pool.shape[2] < 1:
+        raise ValueError(f"{what}: pages must hold at least one row of one element")
     if pool.stride(2) != 1 and pool.shape[2] > 1:
         raise ValueError(f"{what}: pool rows must be contiguous")
-    return B
+
+
+def rows_contiguous(t: torch.Tensor) -> bool:
+    return t.stride(-1) == 1 or t.shape[-1] <= 1
 
 
 def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
@@ -66,60 +68,68 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
     [0, pages * page_size] (clamped) is recorded in the device status
     (``_lib.check_device_status`` raises IndexError), as for event indices.
     """
-    dev = L.require_cuda(q, pool, page_table, lengths, weights, out, weights_out,
-                         what="paged_attention")
-    B = check_pages("paged_attention", pool, page_table, lengths)
+    d = q.get_device()
+    if d < 0 or pool.get_device() != d or page_table.get_device() != d or \
+            lengths.get_device() != d or (weights is not None and weights.get_device() != d) or \
+            out is not None or weights_out is not None:
+        L.require_cuda(q, pool, page_table, lengths, weights, out, weights_out,
+                       what="paged_attention")
+    check_pages("paged_attention", pool, page_table, lengths)
+    dtype = q.dtype
+    if dtype != pool.dtype:
+        raise TypeError(f"paged_attention: q is {dtype}, the pool {pool.dtype}")
+    B = lengths.shape[0]
+    pages, page_size, width = pool.shape
     if q.dim() != 3 or q.shape[0] != B:
         raise ValueError(f"paged_attention: q must be (B, H, Dh) with B = {B}, got {tuple(q.shape)}")
-    if q.dtype != pool.dtype:
-        raise TypeError(f"paged_attention: q is {q.dtype}, the pool {pool.dtype}")
     _, H, Dh = q.shape
-    width = pool.shape[2]
-    if Dh == 0 or width == 0 or width % (2 * Dh) != 0:
+    if Dh == 0 or width % (2 * Dh) != 0:
         raise ValueError(f"paged_attention: rows of {width} are not K | V of heads of {Dh}")
     Hkv = width // (2 * Dh)
     if H == 0 or H % Hkv != 0:
         raise ValueError(f"paged_attention: {H} query heads over {Hkv} K|V heads")
-    if q.stride(2) != 1:
+    if not rows_contiguous(q):
         q = q.contiguous()
-    table_ld = page_table.stride(0)
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+    if not rows_contiguous(page_table):
         page_table = page_table.contiguous()
-        table_ld = page_table.stride(0)
-    if B > 1 and lengths.stride(0) != 1:
+    if not rows_contiguous(lengths):
         lengths = lengths.contiguous()
+    dev = q.device
     if out is None:
-        out = torch.empty(B, H, Dh, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        out = torch.empty(B, H, Dh, dtype=dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != dtype or not rows_contiguous(out):
         raise ValueError("paged_attention: out must be like q with contiguous heads")
-    a = L.PagedAttentionArgs(
-        L.dtype_code(q.dtype), B, H, Hkv, Dh, q.data_ptr(), q.stride(0), q.stride(1),
-        pool.data_ptr(), pool.shape[0], pool.stride(0), pool.stride(1), pool.shape[1],
-        page_table.shape[1], page_table.data_ptr(), table_ld, lengths.data_ptr(),
-        out.data_ptr(), out.stride(0), out.stride(1))
-    a.scale = Dh ** -0.5 if scale is None else scale
+    table_width = page_table.shape[1]
+    W = w_in = w_out = w_in_ld = w_out_ld = 0
     if weights is not None:
         if weights.dtype != torch.float32 or weights.dim() != 2 or weights.shape[0] != B or \
-                weights.shape[1] < page_table.shape[1] * pool.shape[1]:
+                weights.shape[1] < table_width * page_size:
             raise ValueError("paged_attention: weights must be float32 (B, >= pages * page_size)")
-        if weights.shape[1] > 1 and weights.stride(1) != 1:
-            raise ValueError("paged_attention: weights rows must be contiguous")
         if weights_out is None:
             weights_out = torch.empty(weights.shape, dtype=torch.float32, device=dev)
-        elif weights_out.shape != weights.shape or weights_out.dtype != torch.float32 or \
-                (weights.shape[1] > 1 and weights_out.stride(1) != 1):
+        elif weights_out.shape != weights.shape or weights_out.dtype != torch.float32:
             raise ValueError("paged_attention: weights_out must be like weights")
-        a.w_in, a.w_out = weights.data_ptr(), weights_out.data_ptr()
-        a.w_in_ld, a.w_out_ld, a.w_width = weights.stride(0), weights_out.stride(0), weights.shape[1]
+        if not rows_contiguous(weights) or not rows_contiguous(weights_out):
+            raise ValueError("paged_attention: weights rows must be contiguous")
+        W, w_in, w_out = weights.shape[1], weights.data_ptr(), weights_out.data_ptr()
+        w_in_ld, w_out_ld = weights.stride(0), weights_out.stride(0)
     elif weights_out is not None:
         raise ValueError("paged_attention: weights_out without weights")
+    qb, qh, _ = q.stride()
+    pb, pr, _ = pool.stride()
+    ob, oh, _ = out.stride()
+    q_ptr, pool_ptr = q.data_ptr(), pool.data_ptr()
+    block = _pack(L.dtype_code(dtype), B, H, Hkv, Dh, q_ptr, qb, qh, pool_ptr, pages, pb, pr, page_size, table_width, page_table.data_ptr(), page_table.stride(0),
+                  lengths.data_ptr(), out.data_ptr(), ob, oh, w_in, w_out, w_in_ld, w_out_ld, W,
+                  Dh ** -0.5 if scale is None else scale)
     lib = L.load()
-    ref = ctypes.byref(a)
     with L.on_device(dev):
-        n = lib.ck_paged_attention_workspace_bytes(ref)
+        # everything the size depends on, alignment included
+        key = (d, dtype, B, H, Hkv, Dh, page_size, table_width, W, (pb | pr | qb | qh) & 7,
+               (q_ptr | pool_ptr) & 15)
+        n = L.workspace_bytes(lib.ck_paged_attention_workspace_bytes, key, block)
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        rc = lib.ck_paged_attention(ref, None if ws is None else ws.data_ptr(), n,
-                                    L.stream_of(dev))
+        rc = lib.ck_paged_attention(block, ws.data_ptr() if n else 0, n, L.stream_of(dev))
     if rc != L.CK_OK:
         L.check(rc, "ck_paged_attention")
     return out if weights is None else (out, weights_out)

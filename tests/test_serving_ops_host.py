@@ -1,0 +1,136 @@
+"""Host side of the serving operators: argument blocks, the C entry points'
+refusals (which launch nothing), and the wrappers' answers to CPU tensors."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from cortex import _lib as L
+from cortex.kernels.kv_evict import evict_by_weight
+from cortex.kernels.lora import lora_linear
+from cortex.kernels.paged_attention import paged_attention
+
+
+@pytest.mark.parametrize("packed,struct", [
+    (L.PAGED_ATTENTION_ARGS, L.PagedAttentionArgs),
+    (L.EVICT_ARGS, L.EvictArgs),
+    (L.LORA_ARGS, L.LoraArgs),
+])
+def test_packed_blocks_have_the_struct_layout(packed, struct):
+    assert packed.size == ctypes.sizeof(struct)
+    values = list(range(1, len(struct._fields_) + 1))
+    block = struct.from_buffer_copy(packed.pack(*values))
+    assert [getattr(block, name) or 0 for name, _ in struct._fields_] == values
+
+
+def _paged(**kw):
+    base = dict(dtype=L.CK_BF16, B=2, H=8, Hkv=4, Dh=64, q=16, q_ld_b=512, q_ld_h=64, pool=16,
+                num_pages=4, page_ld=16 * 512, row_ld=512, page_size=16, page_table_width=4,
+                page_table=16, page_table_ld=4, lengths=16, o=16, o_ld_b=512, o_ld_h=64, scale=0.1)
+    base.update(kw)
+    return bytes(L.PagedAttentionArgs(**base))
+
+
+def test_paged_attention_refusals():
+    lib = L.load()
+
+    def rc(ws=0, n=0, **kw):
+        return lib.ck_paged_attention(_paged(**kw), ws, n, 0)
+
+    assert lib.ck_paged_attention(None, 0, 0, 0) == L.CK_ERR_INVALID_ARG
+    assert rc(dtype=L.CK_I8) == L.CK_ERR_UNSUPPORTED
+    assert rc(Dh=257) == L.CK_ERR_UNSUPPORTED
+    for bad in (dict(B=-1), dict(H=0), dict(Hkv=0), dict(H=6), dict(Dh=0), dict(page_size=0),
+                dict(page_table_width=-1), dict(num_pages=-1), dict(scale=float("nan")),
+                dict(page_table_width=2 ** 28), dict(w_out=16), dict(w_out=16, w_in=16, w_width=63)):
+        assert rc(**bad) == L.CK_ERR_INVALID_ARG, bad
+    assert rc(B=0) == L.CK_OK
+    big = dict(page_table_width=512)
+    need = lib.ck_paged_attention_workspace_bytes(_paged(**big))
+    assert need > 0
+    assert rc(**big) == L.CK_ERR_WORKSPACE
+    assert rc(ws=16, n=need - 1, **big) == L.CK_ERR_WORKSPACE
+    assert rc(ws=8, n=need, **big) == L.CK_ERR_WORKSPACE
+    for missing in ("q", "o", "lengths", "pool", "page_table"):
+        assert rc(ws=16, n=need, **big, **{missing: None}) == L.CK_ERR_INVALID_ARG
+    assert lib.ck_paged_attention_workspace_bytes(None) == 0
+
+
+def _evict(**kw):
+    base = dict(elem_bytes=2, B=2, pool=16, num_pages=8, page_ld=16 * 64, row_ld=64, page_size=16,
+                width=64, page_table=16, page_table_ld=4, page_table_width=4, budget=20, recent=3,
+                fill=1, lengths=16, lengths_out=32, w_in=16, w_out=32, pos_in=16, pos_out=32,
+                w_in_ld=64, w_out_ld=20, pos_in_ld=64, pos_out_ld=20, in_width=64, out_width=20)
+    base.update(kw)
+    return bytes(L.EvictArgs(**base))
+
+
+def test_evict_refusals():
+    lib = L.load()
+    need = lib.ck_evict_workspace_bytes(_evict())
+    assert need > 0
+
+    def rc(ws=16, n=need, **kw):
+        return lib.ck_evict_by_weight(_evict(**kw), ws, n, 0)
+
+    assert lib.ck_evict_by_weight(None, 0, 0, 0) == L.CK_ERR_INVALID_ARG
+    assert rc(elem_bytes=1) == L.CK_ERR_UNSUPPORTED
+    for bad in (dict(B=-1), dict(budget=0), dict(recent=21), dict(recent=-1), dict(width=0),
+                dict(page_size=0), dict(in_width=63), dict(out_width=19), dict(num_pages=-1),
+                dict(page_table_width=2 ** 28), dict(w_out=16), dict(pos_out=16)):
+        assert rc(**bad) == L.CK_ERR_INVALID_ARG, bad
+    for missing in ("lengths", "lengths_out", "w_in", "w_out", "pos_in", "pos_out", "pool",
+                    "page_table"):
+        assert rc(**{missing: None}) == L.CK_ERR_INVALID_ARG
+    assert rc(ws=0) == L.CK_ERR_WORKSPACE
+    assert rc(n=need - 1) == L.CK_ERR_WORKSPACE
+    assert rc(B=0) == L.CK_OK
+    # a budget that no sequence can pass needs no workspace
+    assert lib.ck_evict_workspace_bytes(_evict(budget=64, out_width=64)) == 0
+    assert lib.ck_evict_workspace_bytes(None) == 0
+
+
+def _lora(**kw):
+    base = dict(dtype=L.CK_BF16, n_adapters=3, rank=8, M=300, K=64, N=32, x=16, ldx=64, w=16,
+                ldw=64, a=16, b=16, ids=16, y=16, ldy=32)
+    base.update(kw)
+    return bytes(L.LoraArgs(**base))
+
+
+def test_lora_refusals():
+    lib = L.load()
+
+    def rc(ws=16, n=1 << 40, **kw):
+        return lib.ck_lora_linear(_lora(**kw), ws, n, 0)
+
+    assert lib.ck_lora_linear(None, 0, 0, 0) == L.CK_ERR_INVALID_ARG
+    assert rc(dtype=L.CK_I8) == L.CK_ERR_UNSUPPORTED
+    assert rc(rank=257) == L.CK_ERR_UNSUPPORTED
+    for bad in (dict(M=-1), dict(N=-1), dict(K=0), dict(rank=0), dict(n_adapters=-1)):
+        assert rc(**bad) == L.CK_ERR_INVALID_ARG, bad
+    for missing in ("x", "w", "a", "b", "ids", "y"):
+        for M in (3, 300):
+            assert rc(M=M, **{missing: None}) == L.CK_ERR_INVALID_ARG
+    assert rc(M=0) == L.CK_OK and rc(N=0) == L.CK_OK
+    for M in (3, 300):
+        for dtype in (L.CK_BF16, L.CK_F32):
+            need = lib.ck_lora_workspace_bytes(_lora(M=M, dtype=dtype))
+            assert need > 0
+            assert rc(M=M, dtype=dtype, n=need - 1) == L.CK_ERR_WORKSPACE
+            assert rc(M=M, dtype=dtype, ws=0) == L.CK_ERR_WORKSPACE
+    assert lib.ck_lora_workspace_bytes(None) == 0
+
+
+def test_cpu_tensors_are_refused():
+    i32 = torch.int32
+    pool, table, n = torch.zeros(4, 16, 512), torch.zeros(2, 3, dtype=i32), torch.zeros(2, dtype=i32)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        paged_attention(torch.zeros(2, 4, 64), pool, table, n)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        evict_by_weight(pool, table, n, torch.zeros(2, 48), torch.zeros(2, 48, dtype=i32), budget=3)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        lora_linear(torch.zeros(2, 8), torch.zeros(4, 8), torch.zeros(1, 2, 8), torch.zeros(1, 4, 2),
+                    torch.zeros(2, dtype=i32))
