@@ -11,10 +11,11 @@
 //
 // select_kernel: a cluster of CS CTAs per sequence finds the budget-th largest
 // key by radix selection (8 bits a pass, most significant first) and numbers
-// holes and movers. Each CTA holds a contiguous part of the slots, its keys in
+// holes and movers. A warp holds a contiguous part of the slots, their keys in
 // shared memory when they fit; histograms and per-warp counts are exchanged
-// through distributed shared memory, so the slots' order decides every rank
-// and no result depends on timing. move_kernel copies the rows, a warp a row.
+// through distributed shared memory, so the slots' order decides every rank and
+// no result depends on timing. move_kernel then moves the rows with their
+// weights and positions, a warp a row.
 //
 // Bytes: weights and positions once (8 B a slot), 2 row reads / writes a mover.
 #include "common.cuh"
@@ -24,9 +25,10 @@ namespace ck {
 
 namespace {
 
-constexpr int ST = 1024;         // threads of a selecting CTA
+constexpr int ST = 512;          // threads of a selecting CTA
 constexpr int SW = ST / 32;
-constexpr int kKeyCap = 49152;   // keys a CTA keeps in shared memory
+constexpr int kKeyCap = 24576;   // slots whose key and position a CTA keeps in shared memory
+constexpr int kFewMoves = 128;   // rows that the selecting kernel moves itself
 constexpr uint32_t kProtected = 0xFFFFFFFFu;
 
 struct EvictParams {
@@ -36,8 +38,9 @@ struct EvictParams {
   int32_t* counts;    // [B] moves
   int32_t* holes;     // [B][max_moves]
   int32_t* movers;    // [B][max_moves]
-  int32_t key_cap;    // keys per CTA that shared memory holds
-  int32_t move_blocks;  // move_kernel: blocks per sequence
+  int32_t key_cap;    // slots per CTA that shared memory holds
+  int32_t move_blocks;  // move_kernel: blocks per sequence; 0: select_kernel moves the rows
+  int32_t vec_bytes;    // bytes that a lane copies at a time
 };
 
 // Order-preserving key of a weight: NaN lowest, -0 as +0; below kProtected.
@@ -53,20 +56,86 @@ __device__ __forceinline__ uint32_t cl_ld(uint32_t addr) {
   return v;
 }
 
+// Rows of the movers into the holes, their weights and positions with them:
+// moves [32 k, 32 k + 32) of sequence b for k = w, w + workers, ... by a warp.
+// The lanes look up a move each, then the warp copies row after row, 8 vectors
+// a lane in flight.
+template <typename V>
+__device__ __forceinline__ void move_rows(const EvictParams& p, int b, const int32_t* holes,
+                                          const int32_t* movers, int total, int w, int workers) {
+  const ck_evict_args& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t vecs = (int64_t)a.width * a.elem_bytes / (int64_t)sizeof(V);
+  const int32_t* table = a.page_table + (int64_t)b * a.page_table_ld;
+  auto row_of = [&](int j) -> int64_t {
+    const int slot = j / a.page_size;
+    const int32_t page = table[slot];
+    if (page < 0 || page >= a.num_pages) {
+      set_status(CK_ERR_INDEX, b, page);
+      return -1;
+    }
+    return ((int64_t)page * a.page_ld + (int64_t)(j - slot * a.page_size) * a.row_ld) * a.elem_bytes;
+  };
+  // few moves: fewer than 32 to a warp, so that every warp has some
+  const int per = max(1, min(32, (total + workers - 1) / workers));
+  uint8_t* pool = reinterpret_cast<uint8_t*>(a.pool);
+  for (int64_t i0 = (int64_t)w * per; i0 < total; i0 += (int64_t)workers * per) {
+    const int cnt = (int)min((int64_t)per, total - i0);
+    int64_t from = -1, to = -1;
+    if (lane < cnt) {
+      const int hole = holes[i0 + lane], mover = movers[i0 + lane];
+      to = row_of(hole);
+      from = row_of(mover);
+      a.w_out[(int64_t)b * a.w_out_ld + hole] = a.w_in[(int64_t)b * a.w_in_ld + mover];
+      a.pos_out[(int64_t)b * a.pos_out_ld + hole] = a.pos_in[(int64_t)b * a.pos_in_ld + mover];
+    }
+    for (int k = 0; k < cnt; ++k) {
+      const int64_t f = __shfl_sync(0xffffffffu, from, k), t = __shfl_sync(0xffffffffu, to, k);
+      if (f < 0 || t < 0) continue;
+      const V* src = reinterpret_cast<const V*>(pool + f);
+      V* dst = reinterpret_cast<V*>(pool + t);
+      for (int64_t c = lane; c < vecs; c += 8 * 32) {
+        V v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (c + 32 * u < vecs) v[u] = src[c + 32 * u];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (c + 32 * u < vecs) dst[c + 32 * u] = v[u];
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ int4 cl_ld4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 template <int CS>
-__global__ void __launch_bounds__(ST, 1) evict_select_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p) {
+  constexpr int WARPS = CS * SW;  // warps of the cluster
   __shared__ uint32_t s_hist[4][256];
   __shared__ uint32_t s_sum[256];
-  __shared__ int32_t s_max[1];
-  __shared__ int32_t s_cnt[3][SW];  // per warp: equal keys, holes, movers
-  __shared__ uint32_t s_pick[2];
-  extern __shared__ uint32_t s_key[];
+  __shared__ int32_t s_max;
+  __shared__ uint32_t s_pick[4][2];
+  __shared__ int4 s_cnt[SW];       // per warp: front keys equal, greater; back equal, greater
+  __shared__ int4 s_all[WARPS];    // the same of the whole cluster
+  __shared__ int32_t s_list[2][CS == 1 ? kFewMoves : 1];  // holes, movers that one CTA moves itself
+  extern __shared__ uint32_t s_key[];  // [key_cap] keys, [key_cap] positions
   grid_dep_wait();
   grid_dep_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = CS > 1 ? (int)cl_rank() : 0;
   const int b = blockIdx.x / CS;
   const ck_evict_args& a = p.a;
+  if (CS == 1 && p.move_blocks == 0)  // the rows' addresses are needed at the end: fetch them now
+    for (int i = tid * 32; i < a.page_table_width; i += ST * 32)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(a.page_table + (int64_t)b * a.page_table_ld + i));
   const int64_t raw = a.lengths[b];
   const bool bad = raw < 0 || raw > p.cap;
   if (bad && rank == 0 && tid == 0) set_status(CK_ERR_INDEX, b, (int)raw);
@@ -78,8 +147,8 @@ __global__ void __launch_bounds__(ST, 1) evict_select_kernel(const EvictParams p
   int32_t* pos_out = a.pos_out + (int64_t)b * a.pos_out_ld;
   const int kept_n = min(n, budget);
 
-  // tables of the rows that stay where they are (holes are written further
-  // down), and with fill the columns behind them
+  // tables of the rows that stay where they are (move_kernel overwrites the
+  // holes'), and with fill the columns behind them
   auto copy_tables = [&]() {
     const int end = a.fill ? a.out_width : kept_n;
     if (a.w_out != a.w_in)
@@ -91,44 +160,68 @@ __global__ void __launch_bounds__(ST, 1) evict_select_kernel(const EvictParams p
     copy_tables();
     if (rank == 0 && tid == 0) {
       a.lengths_out[b] = (int32_t)raw;
-      if (p.counts != nullptr) p.counts[b] = 0;
+      if (p.move_blocks > 0) p.counts[b] = 0;
     }
     return;
   }
 
-  // this CTA's slots [s0, s1), this warp's [w0, w1): contiguous, in order
-  const int per_warp = ((n + CS * SW - 1) / (CS * SW) + 31) / 32 * 32;
+  // this CTA's slots begin at s0, this warp's are [w0, w1): contiguous, in order
+  const int per_warp = ((n + WARPS - 1) / WARPS + 31) / 32 * 32;
   const int s0 = min(n, rank * SW * per_warp);
-  const int s1 = min(n, s0 + SW * per_warp);
   const int w0 = min(n, s0 + warp * per_warp);
-  const int w1 = min(s1, w0 + per_warp);
+  const int w1 = min(n, w0 + per_warp);
   const bool cached = SW * per_warp <= p.key_cap;
+  int32_t* s_pos = reinterpret_cast<int32_t*>(s_key + p.key_cap);
 
   for (int i = tid; i < 4 * 256; i += ST) (&s_hist[0][0])[i] = 0u;
-  if (tid == 0) s_max[0] = INT32_MIN;
-  __syncthreads();
+  if (tid == 0) s_max = INT32_MIN;
+  // one pass over the tables, 8 slots a lane in flight
+  int mx = INT32_MIN;
+  for (int jb = w0 + lane; jb - lane < w1; jb += 8 * 32) {
+    float w[8];
+    int32_t q[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int j = jb + 32 * u;
+      q[u] = j < w1 && a.recent > 0 ? __ldg(pos_in + j) : INT32_MIN;
+      w[u] = j < w1 && cached ? __ldg(w_in + j) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int j = jb + 32 * u;
+      mx = max(mx, q[u]);
+      if (j < w1 && cached) {
+        s_key[j - s0] = weight_key(w[u]);
+        s_pos[j - s0] = q[u];
+      }
+    }
+  }
   int64_t guard = INT64_MAX;  // positions above it are protected
+  __syncthreads();
   if (a.recent > 0) {
-    int mx = INT32_MIN;
-    for (int j = w0 + lane; j < w1; j += 32) mx = max(mx, pos_in[j]);
     mx = __reduce_max_sync(0xffffffffu, mx);
-    if (lane == 0) atomicMax(&s_max[0], mx);
+    if (lane == 0) atomicMax(&s_max, mx);
     if (CS > 1) {
       cl_sync();
-      mx = INT32_MIN;
-#pragma unroll
-      for (int r = 0; r < CS; ++r) mx = max(mx, (int)cl_ld(cl_map(&s_max[0], r)));
+      mx = lane < CS ? (int)cl_ld(cl_map(&s_max, lane)) : INT32_MIN;
+      mx = __reduce_max_sync(0xffffffffu, mx);
     } else {
       __syncthreads();
-      mx = s_max[0];
+      mx = s_max;
     }
     guard = (int64_t)mx - a.recent;
   }
+  // keys of the slots, from here on with the protection applied
+  if (cached) {
+    for (int j = w0 + lane; j < w1; j += 32)
+      if ((int64_t)s_pos[j - s0] > guard) s_key[j - s0] = kProtected;
+    __syncwarp();
+  }
   auto make_key = [&](int j) -> uint32_t {
-    if (a.recent > 0 && (int64_t)pos_in[j] > guard) return kProtected;
-    return weight_key(w_in[j]);
+    if (cached) return s_key[j - s0];
+    if (a.recent > 0 && (int64_t)__ldg(pos_in + j) > guard) return kProtected;
+    return weight_key(__ldg(w_in + j));
   };
-  auto key_at = [&](int j) -> uint32_t { return cached ? s_key[j - s0] : make_key(j); };
 
   // radix selection of the budget-th largest key
   uint32_t prefix = 0u;
@@ -136,42 +229,45 @@ __global__ void __launch_bounds__(ST, 1) evict_select_kernel(const EvictParams p
 #pragma unroll 1
   for (int pass = 0; pass < 4; ++pass) {
     const int shift = 24 - 8 * pass;
-    for (int j = w0 + lane; j - lane < w1; j += 32) {
-      uint32_t k = 0u;
-      bool in = j < w1;
-      if (in) {
-        if (pass == 0) {
-          k = make_key(j);
-          if (cached) s_key[j - s0] = k;
-        } else {
-          k = key_at(j);
-          in = (k >> (shift + 8)) == (prefix >> (shift + 8));
-        }
+    // adds of 1 with no result: the lanes that meet in a bin are counted by the
+    // hardware, however few exponents the first digit has
+    auto count = [&](uint32_t k) {
+      if (pass == 0 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
+        atomicAdd(&s_hist[pass][(k >> shift) & 255u], 1u);
+    };
+    if (cached) {
+      int j = w0 + 4 * lane;
+#pragma unroll 2
+      for (; j + 3 < w1; j += 128) {
+        const uint4 k = *reinterpret_cast<const uint4*>(s_key + (j - s0));
+        count(k.x);
+        count(k.y);
+        count(k.z);
+        count(k.w);
       }
-      // lanes with the same digit add once (the first digit is a handful of
-      // exponents: one address would take most of the adds)
-      const uint32_t digit = in ? (k >> shift) & 255u : 256u;
-      const uint32_t peers = __match_any_sync(0xffffffffu, digit);
-      if (in && (peers & ((1u << lane) - 1u)) == 0u) atomicAdd(&s_hist[pass][digit], __popc(peers));
+      for (int i = 0; i < 4; ++i)
+        if (j + i < w1) count(s_key[j + i - s0]);
+    } else {
+#pragma unroll 4
+      for (int j = w0 + lane; j < w1; j += 32) count(make_key(j));
     }
     if (CS > 1) cl_sync(); else __syncthreads();
-    if (tid < 256) {
-      uint32_t h = 0u;
-      if (CS > 1) {
+    if (CS > 1) {
+      if (tid < 256) {
+        uint32_t h = 0u;
 #pragma unroll
         for (int r = 0; r < CS; ++r) h += cl_ld(cl_map(&s_hist[pass][tid], r));
-      } else {
-        h = s_hist[pass][tid];
+        s_sum[tid] = h;
       }
-      s_sum[tid] = h;
+      __syncthreads();
     }
-    __syncthreads();
-    if (warp == 0) {
+    if (CS == 1 || warp == 0) {  // (one CTA: every warp for itself, no second barrier)
       // lane owns digits 255 - 8 lane down to 248 - 8 lane
+      const uint32_t* sum = CS > 1 ? s_sum : s_hist[pass];
       uint32_t own[8], tot = 0u;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        own[i] = s_sum[255 - 8 * lane - i];
+        own[i] = sum[255 - 8 * lane - i];
         tot += own[i];
       }
       uint32_t before = tot;
@@ -181,129 +277,143 @@ __global__ void __launch_bounds__(ST, 1) evict_select_kernel(const EvictParams p
         if (lane >= o) before += v;
       }
       before -= tot;
-      if (before < want && want <= before + tot) {
+      uint32_t digit = 0u, left = 0u;
+      const bool here = before < want && want <= before + tot;
+      if (here) {
         uint32_t acc = before;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (acc < want && want <= acc + own[i]) {
-            s_pick[0] = (uint32_t)(255 - 8 * lane - i);
-            s_pick[1] = want - acc;
+            digit = (uint32_t)(255 - 8 * lane - i);
+            left = want - acc;
           }
           acc += own[i];
         }
       }
+      const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+      digit = __shfl_sync(0xffffffffu, digit, src);
+      left = __shfl_sync(0xffffffffu, left, src);
+      if (CS > 1) {
+        if (lane == 0) {
+          s_pick[pass][0] = digit;
+          s_pick[pass][1] = left;
+        }
+      } else {
+        prefix |= digit << shift;
+        want = left;
+      }
     }
-    __syncthreads();
-    prefix |= s_pick[0] << shift;
-    want = s_pick[1];
-    __syncthreads();
+    if (CS > 1) {
+      __syncthreads();
+      prefix |= s_pick[pass][0] << shift;
+      want = s_pick[pass][1];
+    }
   }
   // kept: key > prefix, and the first `want` slots whose key equals it
 
-  int eq = 0;
-  for (int j = w0 + lane; j < w1; j += 32) eq += key_at(j) == prefix;
-  eq = __reduce_add_sync(0xffffffffu, eq);
-  if (lane == 0) s_cnt[0][warp] = eq;
-  // prefix over the warps of every CTA before this one and of this CTA
-  auto base_of = [&](int which) -> int {
-    if (CS > 1) cl_sync(); else __syncthreads();
-    int sum = 0;
-    if (CS > 1) {
-      for (int r = 0; r < rank; ++r) sum += (int)cl_ld(cl_map(&s_cnt[which][lane], r));
-    }
-    if (lane < warp) sum += s_cnt[which][lane];
-    return __reduce_add_sync(0xffffffffu, sum);
-  };
-  const int eq_base = base_of(0);
-
-  auto sweep = [&](int& nh, int& nm, bool write) {
-    int e = eq_base;
-    for (int jb = w0; jb < w1; jb += 32) {
-      const int j = jb + lane;
-      const bool in = j < w1;
-      const uint32_t k = in ? key_at(j) : 0u;
-      const bool is_eq = in && k == prefix;
-      const uint32_t em = __ballot_sync(0xffffffffu, is_eq);
-      const uint32_t lt = (1u << lane) - 1u;
-      const bool keep = in && (k > prefix || (is_eq && (uint32_t)(e + __popc(em & lt)) < want));
-      e += __popc(em);
-      const bool hole = in && !keep && j < budget;
-      const bool mover = keep && j >= budget;
-      const uint32_t hm = __ballot_sync(0xffffffffu, hole);
-      const uint32_t mm = __ballot_sync(0xffffffffu, mover);
-      if (write) {
-        if (hole) p.holes[(int64_t)b * p.max_moves + nh + __popc(hm & lt)] = j;
-        if (mover) p.movers[(int64_t)b * p.max_moves + nm + __popc(mm & lt)] = j;
-      }
-      nh += __popc(hm);
-      nm += __popc(mm);
-    }
-  };
-  int nh = 0, nm = 0;
-  sweep(nh, nm, false);
-  if (lane == 0) {
-    s_cnt[1][warp] = nh;
-    s_cnt[2][warp] = nm;
+  int4 c = make_int4(0, 0, 0, 0);
+#pragma unroll 8
+  for (int j = w0 + lane; j < w1; j += 32) {
+    const uint32_t k = make_key(j);
+    const bool back = j >= budget;
+    c.x += !back && k == prefix;
+    c.y += !back && k > prefix;
+    c.z += back && k == prefix;
+    c.w += back && k > prefix;
   }
-  int hbase = base_of(1);
-  int mbase = base_of(2);
-  copy_tables();  // (the holes' entries are overwritten after the next barrier)
-  nh = hbase;
-  nm = mbase;
-  sweep(nh, nm, true);
-  if (rank == CS - 1 && warp == SW - 1 && lane == 0) {
-    p.counts[b] = nh;  // the last warp ends with the totals; holes == movers
+  c.x = __reduce_add_sync(0xffffffffu, c.x);
+  c.y = __reduce_add_sync(0xffffffffu, c.y);
+  c.z = __reduce_add_sync(0xffffffffu, c.z);
+  c.w = __reduce_add_sync(0xffffffffu, c.w);
+  if (lane == 0) s_cnt[warp] = c;
+  if (CS > 1) cl_sync(); else __syncthreads();
+  for (int i = tid; i < WARPS; i += ST) {
+    if (CS > 1) s_all[i] = cl_ld4(cl_map(&s_cnt[i % SW], i / SW));
+    else s_all[i] = s_cnt[i];
+  }
+  copy_tables();
+  __syncthreads();
+  // What the warps before this one hold: equal keys, of which the first `want`
+  // are kept, holes and movers. Equal keys come in slot order, so of a warp's
+  // kept ones those in front come first.
+  const int me = rank * SW + warp;
+  int eq_base = 0, hole_base = 0, mover_base = 0, moves = 0;
+  {
+    int eq_sum = 0;
+    for (int i0 = 0; i0 < WARPS; i0 += 32) {
+      const int i = i0 + lane;
+      const int4 v = i < WARPS ? s_all[i] : make_int4(0, 0, 0, 0);
+      int eq = v.x + v.z, run = eq;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += u;
+      }
+      const int kept_eq = max(0, min(eq, (int)want - (eq_sum + run - eq)));
+      const int kept_front = min(kept_eq, v.x);
+      const int f0 = min(n, i * per_warp), f1 = min(n, f0 + per_warp);
+      const int front = i < WARPS ? max(0, min(f1, budget) - min(f0, budget)) : 0;
+      const int holes = front - v.y - kept_front;
+      const int movers = v.w + kept_eq - kept_front;
+      const bool mine = i < me;
+      eq_base += __reduce_add_sync(0xffffffffu, mine ? eq : 0);
+      hole_base += __reduce_add_sync(0xffffffffu, mine ? holes : 0);
+      mover_base += __reduce_add_sync(0xffffffffu, mine ? movers : 0);
+      moves += __reduce_add_sync(0xffffffffu, holes);
+      eq_sum += __shfl_sync(0xffffffffu, run, 31);
+    }
+  }
+  const uint32_t lt = (1u << lane) - 1u;
+  const bool here = CS == 1 && p.move_blocks == 0;
+  int32_t* holes = here ? s_list[0] : p.holes + (int64_t)b * p.max_moves;
+  int32_t* movers = here ? s_list[1] : p.movers + (int64_t)b * p.max_moves;
+  for (int jb = w0; jb < w1; jb += 32) {
+    const int j = jb + lane;
+    const bool in = j < w1;
+    const uint32_t k = in ? make_key(j) : 0u;
+    const bool is_eq = in && k == prefix;
+    const uint32_t em = __ballot_sync(0xffffffffu, is_eq);
+    const bool keep = in && (k > prefix || (is_eq && eq_base + __popc(em & lt) < (int)want));
+    eq_base += __popc(em);
+    const bool hole = in && !keep && j < budget;
+    const bool mover = keep && j >= budget;
+    const uint32_t hm = __ballot_sync(0xffffffffu, hole);
+    const uint32_t mm = __ballot_sync(0xffffffffu, mover);
+    if (hole) holes[hole_base + __popc(hm & lt)] = j;
+    if (mover) movers[mover_base + __popc(mm & lt)] = j;
+    hole_base += __popc(hm);
+    mover_base += __popc(mm);
+  }
+  if (rank == 0 && tid == 0) {
+    if (p.move_blocks > 0) p.counts[b] = moves;
     a.lengths_out[b] = budget;
   }
-  __threadfence();
-  if (CS > 1) cl_sync(); else __syncthreads();
-  const int total = __ldcg(p.counts + b);
-  for (int i = rank * ST + tid; i < total; i += CS * ST) {
-    const int h = __ldcg(p.holes + (int64_t)b * p.max_moves + i);
-    const int m = __ldcg(p.movers + (int64_t)b * p.max_moves + i);
-    w_out[h] = w_in[m];
-    pos_out[h] = pos_in[m];
+  if (p.move_blocks > 0) {
+    if (CS > 1) cl_sync();  // no CTA leaves while another may read its counts
+    return;
   }
-  if (CS > 1) cl_sync();  // no CTA leaves while another may read its counts
+  // a handful of movers at most: moved here
+  if (CS > 1) {
+    __threadfence();
+    cl_sync();
+  } else {
+    __syncthreads();
+  }
+  switch (p.vec_bytes) {
+    case 16: move_rows<uint4>(p, b, holes, movers, moves, me, WARPS); break;
+    case 4: move_rows<uint32_t>(p, b, holes, movers, moves, me, WARPS); break;
+    default: move_rows<uint16_t>(p, b, holes, movers, moves, me, WARPS);
+  }
 }
 
-// Rows of the movers into the holes: a warp a row, VEC bytes a lane.
 template <typename V>
-__global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p, int64_t row_vecs) {
+__global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
   grid_dep_wait();
   grid_dep_launch();
   const int b = blockIdx.x / p.move_blocks;
-  const int lane = threadIdx.x & 31;
-  const int w = (blockIdx.x - b * p.move_blocks) * 8 + (threadIdx.x >> 5);
-  const int total = p.counts[b];
-  const ck_evict_args& a = p.a;
-  const int32_t* table = a.page_table + (int64_t)b * a.page_table_ld;
-  auto row_of = [&](int j) -> int64_t {
-    const int slot = j / a.page_size;
-    const int32_t page = table[slot];
-    if (page < 0 || page >= a.num_pages) {
-      if (lane == 0) set_status(CK_ERR_INDEX, b, page);
-      return -1;
-    }
-    return ((int64_t)page * a.page_ld + (int64_t)(j - slot * a.page_size) * a.row_ld) * a.elem_bytes;
-  };
-  uint8_t* pool = reinterpret_cast<uint8_t*>(a.pool);
-  for (int i = w; i < total; i += p.move_blocks * 8) {
-    const int64_t to = row_of(p.holes[(int64_t)b * p.max_moves + i]);
-    const int64_t from = row_of(p.movers[(int64_t)b * p.max_moves + i]);
-    if (to < 0 || from < 0) continue;
-    const V* src = reinterpret_cast<const V*>(pool + from);
-    V* dst = reinterpret_cast<V*>(pool + to);
-    int64_t c = lane;
-    for (; c + 96 < row_vecs; c += 128) {
-      V v[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = src[c + 32 * u];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) dst[c + 32 * u] = v[u];
-    }
-    for (; c < row_vecs; c += 32) dst[c] = src[c];
-  }
+  move_rows<V>(p, b, p.holes + (int64_t)b * p.max_moves, p.movers + (int64_t)b * p.max_moves,
+               p.counts[b], (int)(blockIdx.x - b * p.move_blocks) * 8 + (threadIdx.x >> 5),
+               p.move_blocks * 8);
 }
 
 struct EvictPlan {
@@ -325,9 +435,9 @@ int make_plan(const ck_evict_args& a, EvictPlan& pl) {
     return CK_ERR_INVALID_ARG;
   const int64_t behind = p.cap - a.budget;
   p.max_moves = behind <= 0 ? 0 : (int32_t)(behind < a.budget ? behind : a.budget);
-  // A cluster of 8 per sequence once a CTA's threads would take several slots each.
-  pl.cs = p.cap > 4096 ? 8 : 1;
-  if ((int64_t)a.B * 8 > INT32_MAX) return CK_ERR_UNSUPPORTED;
+  // A cluster per sequence once a CTA's threads would take several slots each.
+  pl.cs = p.cap > 65536 ? 16 : (p.cap > 4096 ? 8 : 1);
+  if ((int64_t)a.B * 16 > INT32_MAX) return CK_ERR_UNSUPPORTED;
   const int64_t per_cta = (p.cap + pl.cs - 1) / pl.cs + 32 * SW;
   p.key_cap = (int32_t)(per_cta < kKeyCap ? per_cta : kKeyCap);
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
@@ -341,7 +451,10 @@ int make_plan(const ck_evict_args& a, EvictPlan& pl) {
 template <int CS>
 int launch_select(const EvictParams& p, cudaStream_t st) {
   auto kern = evict_select_kernel<CS>;
-  if (!smem_attr_ready(reinterpret_cast<const void*>(kern), kKeyCap * 4)) return record_cuda_error();
+  if (!smem_attr_ready(reinterpret_cast<const void*>(kern), kKeyCap * 8)) return record_cuda_error();
+  if (CS > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
+                    cudaSuccess)
+    return record_cuda_error();
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = CS;
@@ -352,7 +465,7 @@ int launch_select(const EvictParams& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.a.B * CS));
   cfg.blockDim = dim3(ST);
-  cfg.dynamicSmemBytes = (size_t)p.key_cap * 4;
+  cfg.dynamicSmemBytes = (size_t)p.key_cap * 8;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
@@ -378,20 +491,25 @@ int evict_by_weight(const ck_evict_args& a, void* ws, size_t ws_bytes, cudaStrea
   p.counts = p.max_moves > 0 ? reinterpret_cast<int32_t*>(w) : nullptr;
   p.holes = reinterpret_cast<int32_t*>(w + pl.off_holes);
   p.movers = reinterpret_cast<int32_t*>(w + pl.off_movers);
-  rc = pl.cs == 1 ? launch_select<1>(p, st) : launch_select<8>(p, st);
-  if (rc != CK_OK || p.max_moves == 0) return rc;
-  // blocks for the longest possible list, and no more than fill the card
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.pool) | (uintptr_t)(a.page_ld * a.elem_bytes) |
+                         (uintptr_t)(a.row_ld * a.elem_bytes) |
+                         (uintptr_t)((int64_t)a.width * a.elem_bytes);
+  p.vec_bytes = bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : 2);
+  // Blocks for the longest possible list, and no more than fill the card. A
+  // list of at most kFewMoves rows (sessions that stay at their budget) is
+  // moved by the selecting kernel, without a second launch.
   const int64_t need = (p.max_moves + 7) / 8;
   int64_t fill = (8 * (int64_t)num_sms() + a.B - 1) / a.B;
   if (fill < 1) fill = 1;
-  p.move_blocks = (int32_t)(need < fill ? need : fill);
-  const int64_t row_bytes = (int64_t)a.width * a.elem_bytes;
+  p.move_blocks = p.max_moves <= kFewMoves ? 0 : (int32_t)(need < fill ? need : fill);
+  rc = pl.cs == 1   ? launch_select<1>(p, st)
+       : pl.cs == 8 ? launch_select<8>(p, st)
+                    : launch_select<16>(p, st);
+  if (rc != CK_OK || p.move_blocks == 0) return rc;
   const dim3 grid((unsigned)((int64_t)a.B * p.move_blocks));
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.pool) | (uintptr_t)(a.page_ld * a.elem_bytes) |
-                         (uintptr_t)(a.row_ld * a.elem_bytes) | (uintptr_t)row_bytes;
-  if (bits % 16 == 0) return launch_pdl(evict_move_kernel<uint4>, grid, dim3(256), 0, st, p, row_bytes / 16);
-  if (bits % 4 == 0) return launch_pdl(evict_move_kernel<uint32_t>, grid, dim3(256), 0, st, p, row_bytes / 4);
-  return launch_pdl(evict_move_kernel<uint16_t>, grid, dim3(256), 0, st, p, row_bytes / 2);
+  if (p.vec_bytes == 16) return launch_pdl(evict_move_kernel<uint4>, grid, dim3(256), 0, st, p);
+  if (p.vec_bytes == 4) return launch_pdl(evict_move_kernel<uint32_t>, grid, dim3(256), 0, st, p);
+  return launch_pdl(evict_move_kernel<uint16_t>, grid, dim3(256), 0, st, p);
 }
 
 }  // namespace ck
