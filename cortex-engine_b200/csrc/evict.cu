@@ -27,7 +27,7 @@ namespace {
 
 constexpr int ST = 512;          // threads of a selecting CTA
 constexpr int SW = ST / 32;
-constexpr int kKeyCap = 24576;   // slots whose key and position a CTA keeps in shared memory
+constexpr int kKeyCap = 49152;   // slots whose key a CTA keeps in shared memory
 constexpr int kFewMoves = 128;   // rows that the selecting kernel moves itself
 constexpr uint32_t kProtected = 0xFFFFFFFFu;
 
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
   __shared__ int4 s_cnt[SW];       // per warp: front keys equal, greater; back equal, greater
   __shared__ int4 s_all[WARPS];    // the same of the whole cluster
   __shared__ int32_t s_list[2][CS == 1 ? kFewMoves : 1];  // holes, movers that one CTA moves itself
-  extern __shared__ uint32_t s_key[];  // [key_cap] keys, [key_cap] positions
+  extern __shared__ __align__(16) uint32_t s_key[];  // [key_cap]
   grid_dep_wait();
   grid_dep_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -171,7 +171,6 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
   const int w0 = min(n, s0 + warp * per_warp);
   const int w1 = min(n, w0 + per_warp);
   const bool cached = SW * per_warp <= p.key_cap;
-  int32_t* s_pos = reinterpret_cast<int32_t*>(s_key + p.key_cap);
 
   for (int i = tid; i < 4 * 256; i += ST) (&s_hist[0][0])[i] = 0u;
   if (tid == 0) s_max = INT32_MIN;
@@ -190,10 +189,7 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
     for (int u = 0; u < 8; ++u) {
       const int j = jb + 32 * u;
       mx = max(mx, q[u]);
-      if (j < w1 && cached) {
-        s_key[j - s0] = weight_key(w[u]);
-        s_pos[j - s0] = q[u];
-      }
+      if (j < w1 && cached) s_key[j - s0] = weight_key(w[u]);
     }
   }
   int64_t guard = INT64_MAX;  // positions above it are protected
@@ -212,11 +208,12 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
     guard = (int64_t)mx - a.recent;
   }
   // keys of the slots, from here on with the protection applied
-  if (cached) {
+  if (cached && a.recent > 0) {
+#pragma unroll 8
     for (int j = w0 + lane; j < w1; j += 32)
-      if ((int64_t)s_pos[j - s0] > guard) s_key[j - s0] = kProtected;
-    __syncwarp();
+      if ((int64_t)__ldg(pos_in + j) > guard) s_key[j - s0] = kProtected;
   }
+  __syncwarp();
   auto make_key = [&](int j) -> uint32_t {
     if (cached) return s_key[j - s0];
     if (a.recent > 0 && (int64_t)__ldg(pos_in + j) > guard) return kProtected;
@@ -435,8 +432,13 @@ int make_plan(const ck_evict_args& a, EvictPlan& pl) {
     return CK_ERR_INVALID_ARG;
   const int64_t behind = p.cap - a.budget;
   p.max_moves = behind <= 0 ? 0 : (int32_t)(behind < a.budget ? behind : a.budget);
-  // A cluster per sequence once a CTA's threads would take several slots each.
-  pl.cs = p.cap > 65536 ? 16 : (p.cap > 4096 ? 8 : 1);
+  // CTAs per sequence, measured on B200 (whole call, us, by CTAs): 24 sequences
+  // of 4096 slots 28.7 / 28.7 / 32.8 (1 / 4 / 8), of 16384 slots 45.1 / 32.8 /
+  // 34.8; one of 16384 slots 34.8 / 22.5 / 22.5, one of 131072 47.1 / 41.0 (8 /
+  // 16). 16 CTAs only where they all find an SM: 24 sequences of 16384 slots
+  // took 57.3.
+  pl.cs = p.cap <= 2048 ? 1 : (p.cap <= 16384 ? 4 : 8);
+  if (p.cap > 65536 && 16 * (int64_t)a.B <= num_sms()) pl.cs = 16;
   if ((int64_t)a.B * 16 > INT32_MAX) return CK_ERR_UNSUPPORTED;
   const int64_t per_cta = (p.cap + pl.cs - 1) / pl.cs + 32 * SW;
   p.key_cap = (int32_t)(per_cta < kKeyCap ? per_cta : kKeyCap);
@@ -451,7 +453,7 @@ int make_plan(const ck_evict_args& a, EvictPlan& pl) {
 template <int CS>
 int launch_select(const EvictParams& p, cudaStream_t st) {
   auto kern = evict_select_kernel<CS>;
-  if (!smem_attr_ready(reinterpret_cast<const void*>(kern), kKeyCap * 8)) return record_cuda_error();
+  if (!smem_attr_ready(reinterpret_cast<const void*>(kern), kKeyCap * 4)) return record_cuda_error();
   if (CS > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
                     cudaSuccess)
     return record_cuda_error();
@@ -465,7 +467,7 @@ int launch_select(const EvictParams& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.a.B * CS));
   cfg.blockDim = dim3(ST);
-  cfg.dynamicSmemBytes = (size_t)p.key_cap * 8;
+  cfg.dynamicSmemBytes = (size_t)p.key_cap * 4;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
@@ -503,6 +505,7 @@ int evict_by_weight(const ck_evict_args& a, void* ws, size_t ws_bytes, cudaStrea
   if (fill < 1) fill = 1;
   p.move_blocks = p.max_moves <= kFewMoves ? 0 : (int32_t)(need < fill ? need : fill);
   rc = pl.cs == 1   ? launch_select<1>(p, st)
+       : pl.cs == 4 ? launch_select<4>(p, st)
        : pl.cs == 8 ? launch_select<8>(p, st)
                     : launch_select<16>(p, st);
   if (rc != CK_OK || p.move_blocks == 0) return rc;

@@ -117,7 +117,7 @@ def test_against_definition(lens, page, width, dtype, budget, recent, weights):
 
 
 def test_more_slots_than_shared_memory_holds():
-    run_case(make([450001, 100], 512, 2, torch.float32, weights="few"), 77777, 50)
+    run_case(make([450001] + [100] * 9, 512, 2, torch.float32, weights="few"), 77777, 50)
 
 
 def test_budget_beyond_the_table():
