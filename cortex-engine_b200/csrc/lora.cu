@@ -374,10 +374,10 @@ struct RowsCfg {
   static constexpr int W_BYTES = 128 * 128;
   static constexpr int X_BYTES = NTOK * 128;
   static constexpr int STAGE = W_BYTES + X_BYTES;
-  static constexpr int STAGES = 5;
+  static constexpr int STAGES = 96 * 1024 / STAGE;  // two CTAs an SM
   static constexpr int PART = 128 * NTOK * 4;  // partials, over the ring once it is drained
   static constexpr int RING = STAGES * STAGE > PART ? STAGES * STAGE : PART;
-  static constexpr int SMEM = 1024 + RING + 256;
+  static constexpr int SMEM = 1024 + RING + 256 + NTOK * 4;
   static constexpr uint32_t COLS = NTOK < 32 ? 32 : NTOK;
 };
 
@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
   uint64_t* done = empty + C::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_id = reinterpret_cast<int*>(smem + C::RING + 256);  // [NTOK] adapters of the rows
   const ck_lora_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = SK > 1 ? (int)cl_rank() : 0;
@@ -428,7 +429,23 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  constexpr int PER = (NTOK + SK - 1) / SK;  // rows of x that this CTA finishes
+  const int c0 = rank * PER;
+  const int rows = max(0, min(min(PER, NTOK - c0), (int)min((int64_t)NTOK, a.M - m0) - c0));
   bool ok = true;
+  if (warp >= 2) {
+    // the idle warps fetch the adapters' rows that the epilogue will read
+    for (int c = tid - 64; c < rows; c += 64) s_id[c] = adapter_of(a, m0 + c0 + c, false);
+    asm volatile("bar.sync 1, 64;" ::: "memory");
+    const int64_t line = (int64_t)min((int64_t)128, a.N - n0) * a.rank * 2;  // bytes of B_i's 128 rows
+    for (int c = 0; c < rows; ++c)
+      if (s_id[c] >= 0) {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(a.b) +
+                             ((int64_t)s_id[c] * a.N + n0) * a.rank * 2;
+        for (int64_t o = (tid - 64) * 128; o < line; o += 64 * 128)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(src + o));
+      }
+  }
   if (warp == 0 && lane == 0) {
     int issued = 0;
     for (int kb = kb0; kb < kb1; ++kb, ++issued) {
@@ -489,46 +506,76 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
   }
   const int n = n0 + tid;
   if (ok && n < a.N) {
-    constexpr int PER = (NTOK + SK - 1) / SK;
+    constexpr int UB = PER < 4 ? PER : 4;  // rows in flight
     uint32_t src[SK];
 #pragma unroll
     for (int r = 0; r < SK; ++r) src[r] = SK > 1 ? cl_map(part + tid, r) : smem_u32(part + tid);
     const float bias = a.bias != nullptr ? bf2f(reinterpret_cast<const __nv_bfloat16*>(a.bias)[n]) : 0.f;
     const __nv_bfloat16* B = reinterpret_cast<const __nv_bfloat16*>(a.b);
-    const bool vec = a.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(B) & 15u) == 0;
-    for (int i = 0; i < PER; ++i) {
-      const int c = rank * PER + i;
-      const int64_t m = m0 + c;
-      if (c >= NTOK || m >= a.M) break;
-      float v = 0.f;
+    const bool vec = a.rank % 8 == 0;  // (b is 16-byte aligned)
+    for (int c = 0; c < rows; c += UB) {
+      float v[UB];
 #pragma unroll
-      for (int r = 0; r < SK; ++r) {
-        float f;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(src[r] + c * 512) : "memory");
-        v += f;
-      }
-      const int id = adapter_of(a, m, false);
-      if (id >= 0) {
-        const __nv_bfloat16* br = B + ((int64_t)id * a.N + n) * a.rank;
-        const float* h = p.h + m * a.rank;
-        float d = 0.f;
-        if (vec) {
-          for (int j = 0; j < a.rank; j += 8) {
-            float f[8];
-            load16(br + j, f);
-            const float4 h0 = *reinterpret_cast<const float4*>(h + j);
-            const float4 h1 = *reinterpret_cast<const float4*>(h + j + 4);
-            d = fmaf(f[0], h0.x, d); d = fmaf(f[1], h0.y, d);
-            d = fmaf(f[2], h0.z, d); d = fmaf(f[3], h0.w, d);
-            d = fmaf(f[4], h1.x, d); d = fmaf(f[5], h1.y, d);
-            d = fmaf(f[6], h1.z, d); d = fmaf(f[7], h1.w, d);
-          }
-        } else {
-          for (int j = 0; j < a.rank; ++j) d = fmaf(bf2f(br[j]), h[j], d);
+      for (int u = 0; u < UB; ++u) {
+        v[u] = bias;
+#pragma unroll
+        for (int r = 0; r < SK; ++r) {
+          float f = 0.f;
+          if (c + u < rows)
+            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                         : "=f"(f)
+                         : "r"(src[r] + (c0 + c + u) * 512)
+                         : "memory");
+          v[u] += f;
         }
-        v += d;
       }
-      reinterpret_cast<__nv_bfloat16*>(a.y)[m * a.ldy + n] = f2bf(v + bias);
+      for (int j = 0; j < a.rank; j += 8) {
+        uint4 w[UB];
+        float4 h0[UB], h1[UB];
+#pragma unroll
+        for (int u = 0; u < UB; ++u) {
+          const int id = c + u < rows ? s_id[c + u] : -1;
+          w[u] = make_uint4(0u, 0u, 0u, 0u);
+          h0[u] = h1[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (id < 0) continue;
+          const __nv_bfloat16* br = B + ((int64_t)id * a.N + n) * a.rank + j;
+          const float* h = p.h + (m0 + c0 + c + u) * a.rank + j;
+          if (vec) {
+            w[u] = __ldg(reinterpret_cast<const uint4*>(br));
+            h0[u] = *reinterpret_cast<const float4*>(h);
+            h1[u] = *reinterpret_cast<const float4*>(h + 4);
+          } else {
+            uint32_t e[8];
+            float g[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              e[i] = j + i < a.rank ? (uint32_t)__bfloat16_as_ushort(br[i]) : 0u;
+              g[i] = j + i < a.rank ? h[i] : 0.f;
+            }
+            w[u] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+            h0[u] = make_float4(g[0], g[1], g[2], g[3]);
+            h1[u] = make_float4(g[4], g[5], g[6], g[7]);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < UB; ++u) {
+          if (c + u >= rows || s_id[c + u] < 0) continue;
+          float f[8];
+          unpack8(w[u], f);
+          v[u] = fmaf(f[0], h0[u].x, v[u]);
+          v[u] = fmaf(f[1], h0[u].y, v[u]);
+          v[u] = fmaf(f[2], h0[u].z, v[u]);
+          v[u] = fmaf(f[3], h0[u].w, v[u]);
+          v[u] = fmaf(f[4], h1[u].x, v[u]);
+          v[u] = fmaf(f[5], h1[u].y, v[u]);
+          v[u] = fmaf(f[6], h1[u].z, v[u]);
+          v[u] = fmaf(f[7], h1[u].w, v[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UB; ++u)
+        if (c + u < rows)
+          reinterpret_cast<__nv_bfloat16*>(a.y)[(m0 + c0 + c + u) * a.ldy + n] = f2bf(v[u]);
     }
   }
   if (SK > 1) cl_sync();  // no CTA leaves while another reads its partials
