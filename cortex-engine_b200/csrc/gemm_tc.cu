@@ -1129,8 +1129,8 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
                       32, 128))
       return CK_ERR_INVALID_ARG;
   } else if (lora) {
-    if (!make_tmap_2d(&ty2, fz->lora_h, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.lora_blocks * BK, M,
-                      a.lora_blocks * BK, BK, BM, 128))
+    if (!make_tmap_2d(&ty2, fz->lora_h, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, fz->lora_h_ld, M,
+                      fz->lora_h_ld, BK, BM, 128))
       return CK_ERR_INVALID_ARG;
   } else {
     ty2 = ty;

@@ -34,10 +34,9 @@ struct LoraParams {
 // tensor-core path: h as bf16 rows and the adapters of every 128-row tile
 struct TileParams {
   ck_lora_args a;
-  __nv_bfloat16* h;  // [M][ld_h], zero behind rank
+  __nv_bfloat16* h;   // [M][ld_h], ld_h = rank rounded up to 8, zero behind rank
   int32_t ld_h;
   int32_t max_slots;  // per tile
-  int32_t groups;     // 16-row groups: blocks [0, groups); then a block per tile
   int32_t* cnt;       // [tiles]
   uint4* slots;       // [tiles][max_slots][2]
 };
@@ -219,130 +218,195 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
   }
 }
 
-// h = s_i A_i x as bf16 for 16 rows a block, its four warps each a quarter of K
-// (matrix instructions fed from registers as in paged_attention.cu: any order of
-// the K sum will do, so every lane takes 16 bytes of a row of x and of A). One
-// pass over K per adapter that the 16 rows name, one for rows of one request.
-// Blocks behind the groups list the adapters of a 128-row tile, in the order of
-// their first row, with the rows that are not theirs.
-__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
+// ── many rows: h and the tiles' adapters ─────────────────────────────────────
+//
+// A cluster of SK CTAs per 128-row tile of x. It lists the tile's adapters in
+// the order of their first row (with, for each, the rows that are not its own)
+// and computes D_i[128 x RP] = x_tile A_i^T for SL of them at a time: both
+// operands by TMA into a ring of 64-wide K blocks, the SL accumulators side by
+// side in TMEM, each CTA an SK-th of K. A row then takes the columns of its own
+// adapter; the ranks' partials meet in distributed shared memory, each CTA
+// finishing RP / SK columns: sum in rank order, times s_i, rounded to bf16 for
+// the GEMM's operand. Bound by x, read once for up to SL adapters a tile (every
+// further SL read it again, from L2).
+template <int RP, int SK>
+struct TilesCfg {
+  static constexpr int SL = 2;
+  static constexpr int X_BYTES = 128 * 128;
+  static constexpr int A_BYTES = RP * 128;
+  static constexpr int STAGE = X_BYTES + SL * A_BYTES;
+  static constexpr int STAGES = RP == 64 ? 4 : 5;
+  static constexpr int PART = RP * 128 * 4;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + PART + 256;
+  static constexpr uint32_t COLS = SL * RP < 32 ? 32 : SL * RP;
+};
 
-__device__ void list_tile(const TileParams& p, int tile, int* s_id, uint32_t* s_first) {
+template <int RP, int SK>
+__global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__ CUtensorMap tmX,
+                                                         const __grid_constant__ CUtensorMap tmA,
+                                                         const TileParams p) {
+  using C = TilesCfg<RP, SK>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int s_id[128], s_list[128];
+  __shared__ uint32_t s_first[4];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint8_t* sX = smem;
+  uint8_t* sA = smem + C::STAGES * C::X_BYTES;
+  float* part = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE);  // [RP][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE + C::PART);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* done = empty + C::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const ck_lora_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = SK > 1 ? (int)cl_rank() : 0;
+  const int tile = blockIdx.x / SK;
+  const int kb_all = (int)((a.K + 63) / 64);
+  const int kb_per = (kb_all + SK - 1) / SK;
+  const int kb0 = min(kb_all, rank * kb_per), kb1 = min(kb_all, kb0 + kb_per);
+
+  if (tid == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    prefetch_tmap(&tmX);
+    prefetch_tmap(&tmA);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+  grid_dep_launch();
+
+  // the tile's adapters
   const int64_t m = (int64_t)tile * 128 + tid;
-  const int id = m < p.a.M ? adapter_of(p.a, m, true) : -1;
+  const int id = m < a.M ? adapter_of(a, m, rank == 0) : -1;
   s_id[tid] = id;
   __syncthreads();
-  const uint32_t peers = __match_any_sync(0xffffffffu, id);
-  bool first = id >= 0 && (peers & ((1u << lane) - 1u)) == 0u;
+  const uint32_t lt = (1u << lane) - 1u;
+  const uint32_t peers = __match_any_sync(0xffffffffu, id);  // (every lane, with an adapter or without)
+  bool first = id >= 0 && (peers & lt) == 0u;
   for (int j = 0; j < warp * 32; ++j) first = first && s_id[j] != id;
   const uint32_t fm = __ballot_sync(0xffffffffu, first);
   if (lane == 0) s_first[warp] = fm;
   __syncthreads();
-  int before = __popc(fm & ((1u << lane) - 1u)), total = 0;
+  int before = __popc(fm & lt), total = 0;
+#pragma unroll
   for (int w = 0; w < 4; ++w) {
     if (w < warp) before += __popc(s_first[w]);
     total += __popc(s_first[w]);
   }
-  if (tid == 0) p.cnt[tile] = total;
-  if (first) {
-    uint32_t off[4];
-    for (int w = 0; w < 4; ++w) {
-      off[w] = 0u;
-      for (int j = 0; j < 32; ++j) off[w] |= (uint32_t)(s_id[w * 32 + j] != id) << j;
-    }
-    uint4* dst = p.slots + 2 * ((int64_t)tile * p.max_slots + before);
-    dst[0] = make_uint4((uint32_t)id, 0u, 0u, 0u);
-    dst[1] = make_uint4(off[0], off[1], off[2], off[3]);
-  }
-}
-
-template <int NT>
-__global__ void __launch_bounds__(128) lora_tiles_kernel(const TileParams p) {
-  __shared__ float s_part[4][16][8 * NT + 1];
-  __shared__ int s_id[128];
-  __shared__ uint32_t s_first[4];
-  grid_dep_wait();
-  grid_dep_launch();
-  if ((int)blockIdx.x >= p.groups) {
-    list_tile(p, blockIdx.x - p.groups, s_id, s_first);
-    return;
-  }
-  const ck_lora_args& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int64_t m0 = (int64_t)blockIdx.x * 16;
-  if (tid < 16) s_id[tid] = m0 + tid < a.M ? adapter_of(a, m0 + tid, false) : -1;
+  if (first) s_list[before] = id;
   __syncthreads();
-  const int64_t kq = (a.K + 127) / 128 * 32;  // K per warp
-  const int64_t k_begin = warp * kq, k_end = min(a.K, k_begin + kq);
-  const bool r0 = m0 + g < a.M, r1 = m0 + g + 8 < a.M;
-  const __nv_bfloat16* x0 =
-      reinterpret_cast<const __nv_bfloat16*>(a.x) + (r0 ? m0 + g : m0) * a.ldx + 8 * t;
-  const __nv_bfloat16* x1 =
-      reinterpret_cast<const __nv_bfloat16*>(a.x) + (r1 ? m0 + g + 8 : m0) * a.ldx + 8 * t;
-  const int rows = (int)min((int64_t)16, a.M - m0);
-  for (int j0 = 0; j0 < p.ld_h; j0 += 8 * NT) {
-    // rows without an adapter, and the columns behind the rank, are zero
-    for (int i = tid; i < rows * 8 * NT; i += 128) {
-      const int r = i / (8 * NT), j = j0 + i - r * (8 * NT);
-      if (j < p.ld_h && (s_id[r] < 0 || j >= a.rank)) p.h[(m0 + r) * p.ld_h + j] = f2bf(0.f);
-    }
-    if (j0 >= a.rank) continue;
-    for (int i = 0; i < 16; ++i) {
-      const int id = s_id[i];
-      bool first = id >= 0;
-      for (int q = 0; q < i; ++q) first = first && s_id[q] != id;
-      if (!first) continue;  // (the same for every thread)
-      float acc[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
-      const __nv_bfloat16* A = reinterpret_cast<const __nv_bfloat16*>(a.a) +
-                               ((int64_t)id * a.rank + j0 + g) * a.K + 8 * t;
-#pragma unroll 2
-      for (int64_t k = k_begin; k < k_end; k += 32) {
-        const bool in = k + 8 * t < a.K;  // (K is a multiple of 8)
-        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-        const uint4 u0 = in && r0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : z;
-        const uint4 u1 = in && r1 ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : z;
-        uint4 v[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          v[nt] = in && j0 + 8 * nt + g < a.rank
-                      ? __ldg(reinterpret_cast<const uint4*>(A + (int64_t)8 * nt * a.K + k))
-                      : z;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16(acc[nt], u0.x, u1.x, u0.y, u1.y, v[nt].x, v[nt].y);
-          mma_bf16(acc[nt], u0.z, u1.z, u0.w, u1.w, v[nt].z, v[nt].w);
-        }
-      }
-      __syncthreads();  // the last adapter's sums have been read
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        s_part[warp][g][8 * nt + 2 * t] = acc[nt][0];
-        s_part[warp][g][8 * nt + 2 * t + 1] = acc[nt][1];
-        s_part[warp][g + 8][8 * nt + 2 * t] = acc[nt][2];
-        s_part[warp][g + 8][8 * nt + 2 * t + 1] = acc[nt][3];
-      }
-      __syncthreads();
-      const float s = a.scaling != nullptr ? __ldg(a.scaling + id) : 1.f;
-      for (int q = tid; q < 16 * 8 * NT; q += 128) {
-        const int r = q / (8 * NT), j = q - r * (8 * NT);
-        if (s_id[r] == id && j0 + j < a.rank)
-          p.h[(m0 + r) * p.ld_h + j0 + j] =
-              f2bf(s * (s_part[0][r][j] + s_part[1][r][j] + s_part[2][r][j] + s_part[3][r][j]));
-      }
+  int slot = -1;  // this row's place in the list
+  for (int i = 0; i < total; ++i) {
+    const bool mine = id == s_list[i];
+    const uint32_t mask = __ballot_sync(0xffffffffu, mine);
+    if (mine) slot = i;
+    if (rank == 0) {
+      uint4* dst = p.slots + 2 * ((int64_t)tile * p.max_slots + i);
+      if (lane == 0) reinterpret_cast<uint32_t*>(dst + 1)[warp] = ~mask;
+      if (tid == 0) dst[0] = make_uint4((uint32_t)s_list[i], 0u, 0u, 0u);
     }
   }
+  if (rank == 0 && tid == 0) p.cnt[tile] = total;
+  const float scale = id >= 0 && a.scaling != nullptr ? __ldg(a.scaling + id) : 1.f;
+
+  const int rank_blocks = (a.rank + RP - 1) / RP;
+  const int passes = (total + C::SL - 1) / C::SL * rank_blocks;
+  int it = 0;  // K blocks so far, of the producing and of the multiplying thread
+  for (int pass = 0; pass < passes; ++pass) {
+    const int slot0 = pass / rank_blocks * C::SL, j0 = pass % rank_blocks * RP;
+    const int n_slots = min(C::SL, total - slot0);
+    if (warp == 0 && lane == 0) {
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, 30)) break;
+        mbar_arrive_expect_tx(&full[s], C::X_BYTES + n_slots * C::A_BYTES);
+        tma_load_2d(sX + s * C::X_BYTES, &tmX, &full[s], kb * 64, tile * 128);
+        for (int i = 0; i < n_slots; ++i)  // (rows past the rank are columns that nobody takes)
+          tma_load_2d(sA + (s * C::SL + i) * C::A_BYTES, &tmA, &full[s], kb * 64,
+                      s_list[slot0 + i] * a.rank + j0);
+      }
+    } else if (warp == 1 && lane == 0) {
+      constexpr uint32_t idesc = idesc_bf16(128, RP, 0u);
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(&full[s], (uint32_t)((it / C::STAGES) & 1), abort_flag, 31)) break;
+        tc_fence_after();
+        const uint32_t xa = smem_u32(sX + s * C::X_BYTES);
+        for (int i = 0; i < n_slots; ++i) {
+          const uint32_t aa = smem_u32(sA + (s * C::SL + i) * C::A_BYTES);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_ss(tmem + i * RP, sw128_desc(xa + k * 32, 16, 1024),
+                      sw128_desc(aa + k * 32, 16, 1024), idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+        }
+        tc_commit(&empty[s]);
+      }
+      tc_commit(done);
+      mbar_wait(done, (uint32_t)(pass & 1), nullptr, 32);
+    }
+    __syncthreads();
+    tc_fence_after();
+    const int mine = slot - slot0;  // 0 .. n_slots - 1: this row's columns are here
+    const bool take = mine >= 0 && mine < n_slots;
+#pragma unroll
+    for (int c = 0; c < RP; c += 16) {
+      uint32_t v[C::SL][16];
+#pragma unroll
+      for (int i = 0; i < C::SL; ++i) tmem_ld16w(tmem + ((uint32_t)(warp * 32) << 16) + i * RP + c, v[i]);
+      tc_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        part[(c + e) * 128 + tid] = kb1 > kb0 ? __uint_as_float(mine == 1 ? v[1][e] : v[0][e]) : 0.f;
+    }
+    tc_fence_before();
+    if (SK > 1) cl_sync(); else __syncthreads();
+    if (take && *abort_flag == 0) {
+      constexpr int PER = RP / SK;
+      const int c0 = rank * PER;
+      uint32_t src[SK];
+#pragma unroll
+      for (int r = 0; r < SK; ++r) src[r] = SK > 1 ? cl_map(part + tid, r) : smem_u32(part + tid);
+#pragma unroll
+      for (int c = 0; c < PER; c += 2) {
+        float v[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          v[e] = 0.f;
+#pragma unroll
+          for (int r = 0; r < SK; ++r) {
+            float f;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                         : "=f"(f)
+                         : "r"(src[r] + (c0 + c + e) * 512)
+                         : "memory");
+            v[e] += f;
+          }
+          v[e] = j0 + c0 + c + e < a.rank ? v[e] * scale : 0.f;
+        }
+        if (j0 + c0 + c < p.ld_h)
+          *reinterpret_cast<uint32_t*>(p.h + m * p.ld_h + j0 + c0 + c) = cvt_bf16x2(v[0], v[1]);
+      }
+    }
+    // the partials and the accumulators are free again
+    if (SK > 1) cl_sync(); else __syncthreads();
+    tc_fence_after();
+  }
+  if (warp == 1) tmem_dealloc(tmem, C::COLS);
 }
 
 // Row copies with a change of stride: B rows padded to 16-byte rows (rank not
@@ -608,13 +672,14 @@ int make_plan(const ck_lora_args& a, LoraPlan& pl) {
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
   const bool tma = a.dtype == CK_BF16 && a.K % 8 == 0 && a.ldx % 8 == 0 && a.ldw % 8 == 0 &&
                    aligned16(a.x) && aligned16(a.w) && aligned16(a.a) && aligned16(a.b) &&
-                   (int64_t)a.n_adapters * a.N <= INT32_MAX - 256;
+                   (int64_t)a.n_adapters * a.N <= INT32_MAX - 256 &&
+                   (int64_t)a.n_adapters * a.rank <= INT32_MAX - 256;
   pl.path = !tma ? PATH_SIMT : (a.M <= kRowsMax ? PATH_ROWS : PATH_TILES);
   if (pl.path != PATH_TILES) {
     pl.bytes = up((size_t)a.M * a.rank * 4);
     return CK_OK;
   }
-  pl.ld_h = (a.rank + 63) / 64 * 64;
+  pl.ld_h = (a.rank + 7) / 8 * 8;
   pl.tiles = (int)((a.M + 127) / 128);
   pl.max_slots = a.n_adapters < 1 ? 1 : (a.n_adapters < 128 ? a.n_adapters : 128);
   pl.ld_b = a.rank % 8 == 0 ? 0 : (a.rank + 7) / 8 * 8;
@@ -687,6 +752,50 @@ int launch_rows_k(const LoraParams& p, cudaStream_t st) {
   return launch_rows<NTOK, 1>(p, st);
 }
 
+template <int RP, int SK>
+int launch_tiles(const TileParams& t, int tiles, cudaStream_t st) {
+  using C = TilesCfg<RP, SK>;
+  const ck_lora_args& a = t.a;
+  CUtensorMap tx, ta;
+  // (without adapters no tile lists one, and no block reads this map)
+  const bool any = a.n_adapters > 0;
+  if (!make_tmap_2d(&tx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.K, a.M, a.ldx, 64, 128, 128) ||
+      !make_tmap_2d(&ta, any ? a.a : a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.K,
+                    any ? (uint64_t)a.n_adapters * a.rank : (uint64_t)a.M, any ? a.K : a.ldx, 64, RP,
+                    128))
+    return CK_ERR_INVALID_ARG;
+  auto kern = lora_tiles_kernel<RP, SK>;
+  if (!smem_attr_ready(reinterpret_cast<const void*>(kern), C::SMEM)) return record_cuda_error();
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = SK;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * SK));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = (size_t)C::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return launch_cfg(cfg, kern, tx, ta, t);
+}
+
+template <int RP>
+int launch_tiles_k(const TileParams& t, int tiles, cudaStream_t st) {
+  // K split while the SMs have room and every CTA keeps two K blocks
+  const int64_t kb = (t.a.K + 63) / 64;
+  const int sms = num_sms() > 0 ? num_sms() : 148;
+  int sk = 1;
+  while (sk < 8 && 2 * (int64_t)tiles * sk <= sms && kb >= 4 * sk) sk *= 2;
+  if (sk == 8) return launch_tiles<RP, 8>(t, tiles, st);
+  if (sk == 4) return launch_tiles<RP, 4>(t, tiles, st);
+  if (sk == 2) return launch_tiles<RP, 2>(t, tiles, st);
+  return launch_tiles<RP, 1>(t, tiles, st);
+}
+
 int copy_strided(const void* src, int64_t ld_src, void* dst, int64_t ld_dst, int64_t rows,
                  int64_t cols, cudaStream_t st) {
   int64_t blocks = (rows * cols + 1023) / 1024;
@@ -711,16 +820,11 @@ int run_tiles(const LoraPlan& pl, uint8_t* ws, cudaStream_t st) {
   t.h = reinterpret_cast<__nv_bfloat16*>(ws + pl.off_h);
   t.ld_h = pl.ld_h;
   t.max_slots = pl.max_slots;
-  t.groups = (int32_t)((a.M + 15) / 16);
   t.cnt = reinterpret_cast<int32_t*>(ws + pl.off_cnt);
   t.slots = reinterpret_cast<uint4*>(ws + pl.off_slots);
-  const dim3 grid((unsigned)(t.groups + pl.tiles));
-  if (a.rank <= 16)
-    rc = launch_pdl(lora_tiles_kernel<2>, grid, dim3(128), 0, st, t);
-  else if (a.rank <= 32)
-    rc = launch_pdl(lora_tiles_kernel<4>, grid, dim3(128), 0, st, t);
-  else
-    rc = launch_pdl(lora_tiles_kernel<8>, grid, dim3(128), 0, st, t);
+  rc = a.rank <= 16 ? launch_tiles_k<16>(t, pl.tiles, st)
+       : a.rank <= 32 ? launch_tiles_k<32>(t, pl.tiles, st)
+                      : launch_tiles_k<64>(t, pl.tiles, st);
   if (rc != CK_OK) return rc;
   GemmFusion fz;
   fz.lora_h = t.h;
@@ -729,6 +833,7 @@ int run_tiles(const LoraPlan& pl, uint8_t* ws, cudaStream_t st) {
   fz.lora_n = a.n_adapters > 0 ? a.n_adapters : 1;
   fz.lora_b_ld = pl.ld_b > 0 ? pl.ld_b : a.rank;
   fz.lora_rank = a.rank;
+  fz.lora_h_ld = t.ld_h;
   fz.lora_max = pl.max_slots;
   fz.lora_cnt = t.cnt;
   fz.lora_slots = t.slots;
