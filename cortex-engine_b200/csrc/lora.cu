@@ -13,7 +13,8 @@
 //     MMAs and the rows of x as its narrow one, K split over a cluster;
 //   * many rows (bf16): gemm_tc.cu's tiles with the adapters as further K
 //     blocks (h rounded to bf16, rows of other adapters masked off);
-//   * fp32, and layouts that TMA does not take: lora_simt_kernel.
+//   * fp32: lora_gemv_kernel (few rows) and lora_sgemm_kernel, on the CUDA cores;
+//   * bf16 layouts that TMA does not take: lora_simt_kernel.
 // Order of the launches: a kernel of the first kind waits for all earlier work
 // before it lets its successor start, and writes h and the slot lists alone.
 // The second may therefore read x and W, and write y, before its own wait for
@@ -46,8 +47,6 @@ __device__ __forceinline__ float tofl(__nv_bfloat16 v) { return bf2f(v); }
 template <typename T>
 __device__ __forceinline__ T fromf(float v);
 template <>
-__device__ __forceinline__ float fromf<float>(float v) { return v; }
-template <>
 __device__ __forceinline__ __nv_bfloat16 fromf<__nv_bfloat16>(float v) { return f2bf(v); }
 
 // 16 bytes as floats (4 fp32 or 8 bf16)
@@ -75,9 +74,9 @@ __device__ __forceinline__ int adapter_of(const ck_lora_args& a, int64_t m, bool
 // h: a warp per row and JB ranks, its lanes over K; the JB sums are reduced
 // together (a lane gives half of its sums away at each step).
 template <typename T, int JB, bool VEC>
-__global__ void __launch_bounds__(256) lora_shrink_kernel(const LoraParams p, int jblocks) {
+__global__ void __launch_bounds__(256) lora_shrink_kernel(const LoraParams p, int jblocks, int early) {
   grid_dep_wait();
-  grid_dep_launch();
+  if (early) grid_dep_launch();
   const ck_lora_args& a = p.a;
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -141,12 +140,258 @@ __global__ void __launch_bounds__(256) lora_shrink_kernel(const LoraParams p, in
   }
 }
 
-// The product with W on the CUDA cores, for fp32 (which TF32 tensor-core
-// products would not match) and for bf16 whose strides break the 16-byte
-// rules: 64 x 64 tiles, 4 x 4 a thread, the next K slice in registers while
-// this one is multiplied.
-template <typename T>
+// ── fp32 ─────────────────────────────────────────────────────────────────────
+//
+// On the CUDA cores: TF32 tensor-core products would not match fp32.
+
+__device__ __forceinline__ float adapter_part(const LoraParams& p, int id, int64_t m, int64_t n) {
+  const float* b = reinterpret_cast<const float*>(p.a.b) + ((int64_t)id * p.a.N + n) * p.a.rank;
+  const float* h = p.h + m * p.a.rank;
+  float d = 0.f;
+  for (int j = 0; j < p.a.rank; ++j) d = fmaf(h[j], __ldg(b + j), d);
+  return d;
+}
+
+// Up to MR rows of x at a time: a warp a row of W, read once for them; bound by W.
+template <int MR, bool VEC>
+__global__ void __launch_bounds__(256) lora_gemv_kernel(const LoraParams p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const ck_lora_args& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (n >= a.N) return;
+  const int64_t m0 = (int64_t)blockIdx.y * MR;
+  const float* w = reinterpret_cast<const float*>(a.w) + n * a.ldw;
+  const float* x = reinterpret_cast<const float*>(a.x) + m0 * a.ldx;
+  const int rows = (int)min((int64_t)MR, a.M - m0);
+  float acc[MR];
+#pragma unroll
+  for (int r = 0; r < MR; ++r) acc[r] = 0.f;
+  if constexpr (VEC) {
+#pragma unroll 4
+    for (int64_t k = 4 * lane; k < a.K; k += 128) {
+      float wv[4];
+      load16(w + k, wv);
+#pragma unroll
+      for (int r = 0; r < MR; ++r) {
+        if (r < rows) {
+          float xv[4];
+          load16(x + r * a.ldx + k, xv);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[r] = fmaf(wv[e], xv[e], acc[r]);
+        }
+      }
+    }
+  } else {
+    for (int64_t k = lane; k < a.K; k += 32) {
+      const float wv = __ldg(w + k);
+#pragma unroll
+      for (int r = 0; r < MR; ++r)
+        if (r < rows) acc[r] = fmaf(wv, __ldg(x + r * a.ldx + k), acc[r]);
+    }
+  }
+  float mine = 0.f;  // lane r: row r's sum
+#pragma unroll
+  for (int r = 0; r < MR; ++r) {
+    const float s = warp_sum(acc[r]);
+    if (lane == r) mine = s;
+  }
+  if (lane < rows) {
+    const int64_t m = m0 + lane;
+    const int id = adapter_of(a, m, false);
+    if (id >= 0) mine += adapter_part(p, id, m, n);
+    if (a.bias != nullptr) mine += __ldg(reinterpret_cast<const float*>(a.bias) + n);
+    reinterpret_cast<float*>(a.y)[m * a.ldy + n] = mine;
+  }
+}
+
+// Tiles of 4 MT WM x 32 WN: a thread MT x 4 elements, rows lm + 4 i and columns
+// ln + 8 j of its warp's 4 MT x 32. Both operands come in by asynchronous
+// copies (16 bytes each, or 4 where rows are not 16-byte aligned), slices of 32
+// along K, three slices ahead; rows padded to 36 floats, so that the 16-byte
+// reads of 4 and 8 rows meet in no bank. The adapters are further slices: 32
+// ranks of h against 32 ranks of B_i for each adapter i of the tile's rows, added to the
+// rows that name it alone (chosen, not multiplied by zero: an infinity of one
+// adapter stays with its rows). A slice is summed by itself, even and odd k in
+// the two halves of paired FMAs, and added to the total: K / 32 + 16 roundings
+// in a row instead of K.
+template <int MT, int WM, int WN, bool VEC>
+__global__ void __launch_bounds__(32 * WM * WN, MT == 8 ? 1 : 3)
+    lora_sgemm_kernel(const LoraParams p, int n_tiles) {
+  constexpr int TM = 4 * MT * WM, TN = 32 * WN, TK = 32, LD = TK + 4, NS = 4;
+  constexpr int THREADS = 32 * WM * WN;
+  static_assert(TM <= THREADS, "a thread lists one row's adapter");
+  extern __shared__ __align__(16) float sm[];  // [NS][TM + TN][LD]
+  __shared__ int s_id[TM], s_list[TM];
+  __shared__ int s_first[THREADS / 32];
+  grid_dep_wait();
+  grid_dep_launch();
+  const ck_lora_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lm = lane >> 3, ln = lane & 7;
+  const int wm = warp / WN, wn = warp % WN;
+  const int64_t m0 = (int64_t)(blockIdx.x / n_tiles) * TM;
+  const int64_t n0 = (int64_t)(blockIdx.x % n_tiles) * TN;
+  const float* x = reinterpret_cast<const float*>(a.x);
+  const float* w = reinterpret_cast<const float*>(a.w);
+  const float* B = reinterpret_cast<const float*>(a.b);
+  const int slices = (int)((a.K + TK - 1) / TK);
+  const int rank_slices = (a.rank + TK - 1) / TK;
+  int total = slices;  // and those of the adapters, once they are listed
+
+  // columns [c, c + TK) of TM rows of `left` and TN rows of `right` into the
+  // ring slot of slice s
+  auto fetch = [&](int s, const float* left, int64_t ld_l, const float* right, int64_t ld_r,
+                   int64_t c0, int64_t width, bool vec) {
+    const uint32_t dst = smem_u32(sm + (s % NS) * (TM + TN) * LD);
+    auto copy = [&](int r, int c, int n) {
+      const int64_t k = c0 + c;
+      const bool in = k < width && (r < TM ? m0 + r < a.M : n0 + r - TM < a.N);
+      const float* src = r < TM ? left + (in ? r * ld_l + k : 0) : right + (in ? (r - TM) * ld_r + k : 0);
+      const uint32_t to = dst + (r * LD + c) * 4;
+      if (n == 4)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(in ? 16 : 0) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(src), "r"(in ? 4 : 0) : "memory");
+    };
+    if (vec) {  // (width a multiple of 4)
+#pragma unroll
+      for (int i = tid; i < (TM + TN) * (TK / 4); i += THREADS) copy(i / (TK / 4), i % (TK / 4) * 4, 4);
+    } else {
+      for (int i = tid; i < (TM + TN) * TK; i += THREADS) copy(i / TK, i % TK, 1);
+    }
+  };
+  // slices of K: this thread's pieces of them, whose addresses advance by a slice
+  constexpr int PIECES = (TM + TN) * (TK / 4) / THREADS;
+  static_assert((TM + TN) * (TK / 4) % THREADS == 0, "whole pieces per thread");
+  const float* src[VEC ? PIECES : 1];
+  uint32_t there = 0u;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      const int i = tid + q * THREADS, r = i / (TK / 4), c = i % (TK / 4) * 4;
+      const int64_t row = r < TM ? m0 + r : n0 + r - TM;
+      const bool in = row < (r < TM ? a.M : a.N);
+      src[q] = r < TM ? x + (in ? row : 0) * a.ldx + c : w + (in ? row : 0) * a.ldw + c;
+      there |= (uint32_t)in << q;
+    }
+  }
+  auto fetch_slice = [&](int s) {
+    if (s < slices) {
+      if constexpr (VEC) {
+        const uint32_t dst = smem_u32(sm + (s % NS) * (TM + TN) * LD);
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q) {
+          const int i = tid + q * THREADS, r = i / (TK / 4), c = i % (TK / 4) * 4;
+          const bool in = ((there >> q) & 1u) && (s + 1 < slices || s * (int64_t)TK + c < a.K);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (r * LD + c) * 4),
+                       "l"(in ? src[q] : x), "r"(in ? 16 : 0)
+                       : "memory");
+          src[q] += TK;
+        }
+      } else {
+        fetch(s, x + m0 * a.ldx, a.ldx, w + n0 * a.ldw, a.ldw, (int64_t)s * TK, a.K, false);
+      }
+    } else if (s < total) {
+      const int item = (s - slices) / rank_slices, c0 = (s - slices) % rank_slices * TK;
+      fetch(s, p.h + m0 * a.rank, a.rank, B + ((int64_t)s_list[item] * a.N + n0) * a.rank, a.rank, c0,
+            a.rank, a.rank % 4 == 0 && (reinterpret_cast<uintptr_t>(B) & 15u) == 0);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // the first slices are on their way before the adapters are listed, unless K
+  // ends within them
+  if (slices >= NS - 1)
+    for (int s = 0; s < NS - 1; ++s) fetch_slice(s);
+  // the tile's adapters, in the order of their first row
+  if (tid < TM) s_id[tid] = m0 + tid < a.M ? adapter_of(a, m0 + tid, false) : -1;
+  __syncthreads();
+  {
+    const int id = tid < TM ? s_id[tid] : -1;
+    const uint32_t peers = __match_any_sync(0xffffffffu, id);
+    bool first = id >= 0 && (peers & ((1u << lane) - 1u)) == 0u;
+    for (int j = 0; j < min(warp * 32, TM); ++j) first = first && s_id[j] != id;
+    const uint32_t fm = __ballot_sync(0xffffffffu, first);
+    if (lane == 0) s_first[warp] = __popc(fm);
+    __syncthreads();
+    int before = __popc(fm & ((1u << lane) - 1u)), count = 0;
+#pragma unroll
+    for (int v = 0; v < THREADS / 32; ++v) {
+      if (v < warp) before += s_first[v];
+      count += s_first[v];
+    }
+    if (first) s_list[before] = id;
+    __syncthreads();
+    total = slices + count * rank_slices;
+  }
+  if (slices < NS - 1)
+    for (int s = 0; s < NS - 1; ++s) fetch_slice(s);
+  int my_id[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) my_id[i] = s_id[wm * 4 * MT + lm + 4 * i];
+
+  float acc[MT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+  for (int s = 0; s < total; ++s) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
+    __syncthreads();  // the slice is there, and everyone has left the one before
+    fetch_slice(s + NS - 1);
+    const float* A = sm + (s % NS) * (TM + TN) * LD + (wm * 4 * MT + lm) * LD;
+    const float* W = sm + (s % NS) * (TM + TN) * LD + (TM + wn * 32 + ln) * LD;
+    unsigned long long part[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[i][j] = 0ull;
+#pragma unroll
+    for (int k = 0; k < TK; k += 4) {
+      ulonglong2 wv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) wv[j] = *reinterpret_cast<const ulonglong2*>(W + 8 * j * LD + k);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const ulonglong2 av = *reinterpret_cast<const ulonglong2*>(A + 4 * i * LD + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          part[i][j] = ffma2(av.x, wv[j].x, part[i][j]);
+          part[i][j] = ffma2(av.y, wv[j].y, part[i][j]);
+        }
+      }
+    }
+    const int only = s < slices ? -2 : s_list[(s - slices) / rank_slices];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        f2up(part[i][j], lo, hi);
+        if (only == -2 || my_id[i] == only) acc[i][j] += lo + hi;
+      }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  const float* bias = reinterpret_cast<const float*>(a.bias);
+  float* y = reinterpret_cast<float*>(a.y);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t n = n0 + wn * 32 + ln + 8 * j;
+    if (n >= a.N) continue;
+    const float bj = bias != nullptr ? __ldg(bias + n) : 0.f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = m0 + wm * 4 * MT + lm + 4 * i;
+      if (m < a.M) y[m * a.ldy + n] = acc[i][j] + bj;
+    }
+  }
+}
+
+// bf16 whose strides break TMA's 16-byte rules: 64 x 64 tiles, 4 x 4 a thread,
+// the next K slice in registers while this one is multiplied.
 __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int n_tiles) {
+  using T = __nv_bfloat16;
   constexpr int TM = 64, TN = 64, TK = 16;
   __shared__ __align__(16) float As[TK][TM + 4];
   __shared__ __align__(16) float Ws[TK][TN + 4];
@@ -645,7 +890,9 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
   if (SK > 1) cl_sync();  // no CTA leaves while another reads its partials
 }
 
-enum Path { PATH_ROWS, PATH_TILES, PATH_SIMT };
+constexpr int64_t kGemvMax = 16;  // rows up to which lora_gemv_kernel runs
+
+enum Path { PATH_ROWS, PATH_TILES, PATH_F32, PATH_SIMT };
 
 struct LoraPlan {
   LoraParams p;
@@ -659,14 +906,14 @@ struct LoraPlan {
 bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 
 // Rows up to which lora_rows_kernel runs (tensor-core tiles above).
-constexpr int64_t kRowsMax = 128;
+constexpr int64_t kRowsMax = 64;
 
 int make_plan(const ck_lora_args& a, LoraPlan& pl) {
   if (a.dtype != CK_F32 && a.dtype != CK_BF16) return CK_ERR_UNSUPPORTED;
   if (a.M < 0 || a.N < 0 || a.K <= 0 || a.rank < 1 || a.n_adapters < 0) return CK_ERR_INVALID_ARG;
   if (a.M > INT32_MAX || a.N > INT32_MAX || a.K > INT32_MAX) return CK_ERR_UNSUPPORTED;
   if (a.rank > 256) return CK_ERR_UNSUPPORTED;
-  if (((a.M + 63) / 64) * ((a.N + 63) / 64) > INT32_MAX || (a.M * a.rank + 7) / 8 > INT32_MAX)
+  if (((a.M + 31) / 32) * ((a.N + 63) / 64) > INT32_MAX || (a.M * a.rank + 7) / 8 > INT32_MAX)
     return CK_ERR_UNSUPPORTED;
   pl.p.a = a;
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
@@ -674,7 +921,7 @@ int make_plan(const ck_lora_args& a, LoraPlan& pl) {
                    aligned16(a.x) && aligned16(a.w) && aligned16(a.a) && aligned16(a.b) &&
                    (int64_t)a.n_adapters * a.N <= INT32_MAX - 256 &&
                    (int64_t)a.n_adapters * a.rank <= INT32_MAX - 256;
-  pl.path = !tma ? PATH_SIMT : (a.M <= kRowsMax ? PATH_ROWS : PATH_TILES);
+  pl.path = a.dtype == CK_F32 ? PATH_F32 : !tma ? PATH_SIMT : (a.M <= kRowsMax ? PATH_ROWS : PATH_TILES);
   if (pl.path != PATH_TILES) {
     pl.bytes = up((size_t)a.M * a.rank * 4);
     return CK_OK;
@@ -693,8 +940,12 @@ int make_plan(const ck_lora_args& a, LoraPlan& pl) {
   return CK_OK;
 }
 
+// early: its successor may start beside it. That pays where the successor streams
+// W with a CTA or two an SM (48 rows x 4096 x 4096: 24.6 against 28.7 us); the
+// fp32 tiles would crowd on the SMs that this kernel leaves free (100 rows x 4096 x
+// 1536: 238 against 129 us).
 template <typename T>
-int shrink(const LoraParams& p, cudaStream_t st) {
+int shrink(const LoraParams& p, int early, cudaStream_t st) {
   const ck_lora_args& a = p.a;
   constexpr int E = 16 / sizeof(T);
   const bool vec = a.K % E == 0 && a.ldx % E == 0 && aligned16(a.x) && aligned16(a.a);
@@ -704,10 +955,33 @@ int shrink(const LoraParams& p, cudaStream_t st) {
   const int jblocks = (a.rank + jb - 1) / jb;
   const dim3 grid((unsigned)((a.M * jblocks + 7) / 8));
   if (wide)
-    return vec ? launch_pdl(lora_shrink_kernel<T, 8, true>, grid, dim3(256), 0, st, p, jblocks)
-               : launch_pdl(lora_shrink_kernel<T, 8, false>, grid, dim3(256), 0, st, p, jblocks);
-  return vec ? launch_pdl(lora_shrink_kernel<T, 1, true>, grid, dim3(256), 0, st, p, jblocks)
-             : launch_pdl(lora_shrink_kernel<T, 1, false>, grid, dim3(256), 0, st, p, jblocks);
+    return vec ? launch_pdl(lora_shrink_kernel<T, 8, true>, grid, dim3(256), 0, st, p, jblocks, early)
+               : launch_pdl(lora_shrink_kernel<T, 8, false>, grid, dim3(256), 0, st, p, jblocks, early);
+  return vec ? launch_pdl(lora_shrink_kernel<T, 1, true>, grid, dim3(256), 0, st, p, jblocks, early)
+             : launch_pdl(lora_shrink_kernel<T, 1, false>, grid, dim3(256), 0, st, p, jblocks, early);
+}
+
+template <int MT, int WM, int WN, bool VEC>
+int launch_sgemm(const LoraParams& p, cudaStream_t st) {
+  constexpr int TM = 4 * MT * WM, TN = 32 * WN;
+  constexpr int smem = 4 * (TM + TN) * 36 * 4;
+  auto kern = lora_sgemm_kernel<MT, WM, WN, VEC>;
+  if (!smem_attr_ready(reinterpret_cast<const void*>(kern), smem)) return record_cuda_error();
+  const int n_tiles = (int)((p.a.N + TN - 1) / TN);
+  return launch_pdl(kern, dim3((unsigned)((p.a.M + TM - 1) / TM * n_tiles)), dim3(32 * WM * WN), smem,
+                    st, p, n_tiles);
+}
+
+template <bool VEC>
+int run_f32(const LoraParams& p, cudaStream_t st) {
+  const ck_lora_args& a = p.a;
+  const unsigned gx = (unsigned)((a.N + 7) / 8);
+  if (a.M == 1) return launch_pdl(lora_gemv_kernel<1, VEC>, dim3(gx), dim3(256), 0, st, p);
+  if (a.M <= kGemvMax)
+    return launch_pdl(lora_gemv_kernel<8, VEC>, dim3(gx, (unsigned)((a.M + 7) / 8)), dim3(256), 0, st, p);
+  // 128 x 64 tiles once they give every SM one, else 32 x 64
+  if ((a.M + 127) / 128 * ((a.N + 63) / 64) >= num_sms()) return launch_sgemm<8, 4, 2, VEC>(p, st);
+  return launch_sgemm<4, 2, 2, VEC>(p, st);
 }
 
 template <int NTOK, int SK>
@@ -858,20 +1132,24 @@ int lora_linear(const ck_lora_args& a, void* ws, size_t ws_bytes, cudaStream_t s
   if (pl.path == PATH_TILES) return run_tiles(pl, reinterpret_cast<uint8_t*>(ws), st);
   pl.p.h = reinterpret_cast<float*>(ws);
   if (pl.path == PATH_ROWS) {
-    rc = shrink<__nv_bfloat16>(pl.p, st);
+    rc = shrink<__nv_bfloat16>(pl.p, 1, st);
     if (rc != CK_OK) return rc;
     if (a.M <= 16) return launch_rows_k<16>(pl.p, st);
     if (a.M <= 32) return launch_rows_k<32>(pl.p, st);
     if (a.M <= 64) return launch_rows_k<64>(pl.p, st);
     return launch_rows_k<128>(pl.p, st);
   }
-  const bool bf = a.dtype == CK_BF16;
-  rc = bf ? shrink<__nv_bfloat16>(pl.p, st) : shrink<float>(pl.p, st);
+  if (pl.path == PATH_F32) {
+    rc = shrink<float>(pl.p, 0, st);
+    if (rc != CK_OK) return rc;
+    const bool vec = a.K % 4 == 0 && a.ldx % 4 == 0 && a.ldw % 4 == 0 && aligned16(a.x) && aligned16(a.w);
+    return vec ? run_f32<true>(pl.p, st) : run_f32<false>(pl.p, st);
+  }
+  rc = shrink<__nv_bfloat16>(pl.p, 0, st);
   if (rc != CK_OK) return rc;
   const int n_tiles = (int)((a.N + 63) / 64);
   const dim3 grid((unsigned)(((a.M + 63) / 64) * n_tiles));
-  return bf ? launch_pdl(lora_simt_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, pl.p, n_tiles)
-            : launch_pdl(lora_simt_kernel<float>, grid, dim3(256), 0, st, pl.p, n_tiles);
+  return launch_pdl(lora_simt_kernel, grid, dim3(256), 0, st, pl.p, n_tiles);
 }
 
 }  // namespace ck
