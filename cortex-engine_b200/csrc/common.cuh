@@ -708,6 +708,19 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo_byte
   return d;
 }
 
+// K-major descriptor of a tile with rows of `sw` bytes (32, 64 or 128) in the
+// swizzle of that width, 8-row groups 8 * sw bytes apart. Layouts: 6 = 32B, 4 =
+// 64B, 2 = 128B.
+__device__ __forceinline__ uint64_t sw_desc(uint32_t saddr, uint32_t sw) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(((8u * sw) >> 4) & 0x3FFFu) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)(sw == 32 ? 6u : sw == 64 ? 4u : 2u) << 61;
+  return d;
+}
+
 // Instruction descriptor, kind::f16: bf16 A/B, fp32 D, dense.
 //   [4,6) D fmt (1 = f32), [7,10) A fmt (1 = bf16), [10,13) B fmt (1 = bf16),
 //   [15] A major (0 = K), [16] B major (0 = K, 1 = MN), [17,23) N>>3, [24,29) M>>4.

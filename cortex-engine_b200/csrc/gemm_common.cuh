@@ -38,9 +38,11 @@ struct GemmArgs {
   // block per 64 ranks of every adapter its rows name: A operand h (tmY2), B
   // operand the adapter's (N, rank) matrix (tmR), the other rows' accumulator
   // lanes masked off. lora_cnt[row tile] slots of lora_slots[row tile * lora_max].
+  // The blocks' rows are lora_sw = 32, 64 or 128 bytes wide, the least that holds
+  // the rank: a tile of mixed rows takes many blocks, and they cost what they hold.
   const int* lora_cnt;
   const uint4* lora_slots;  // two uint4 a slot: (adapter, 0, 0, 0), masked-off lanes
-  int lora_max, lora_blocks;
+  int lora_max, lora_blocks, lora_sw, lora_rank;
 };
 
 enum Fuse { FUSE_NONE = 0, FUSE_LN = 3, FUSE_RMS = 4, FUSE_LORA = 5 };

@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
             const int slot = i / p.lora_blocks, rb = i - slot * p.lora_blocks;
             const int id = (int)p.lora_slots[2 * ((int64_t)mt * p.lora_max + slot)].x;
             if (!mbar_wait_park(&empty[stage], phase ^ 1, abort_flag, 1)) break;
-            mbar_arrive_expect_tx(&full[stage], C::TX_BYTES);
+            mbar_arrive_expect_tx(&full[stage], (uint32_t)((BM + BN) * p.lora_sw));
             tma_load_2d(sA + stage * C::A_BYTES, &tmY2, &full[stage], rb * BK, mt * BM);
             // (rows past the adapter's N are columns that the store drops)
             tma_load_2d(sB + stage * C::B_BYTES, &tmR, &full[stage], rb * BK, id * p.N + nt * BN);
@@ -405,10 +405,11 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
             tc_fence_after();
             const uint32_t a_addr = smem_u32(sA + stage * C::A_BYTES);
             const uint32_t b_addr = smem_u32(sB + stage * C::B_BYTES);
-#pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              tc_mma_ss_masked(d_tmem, sw128_desc(a_addr + k * 32, 16, 1024),
-                               sw128_desc(b_addr + k * 32, 16, 1024), idesc, 1u, off);
+            const int ranks = p.lora_rank - i % p.lora_blocks * BK;  // of this block and behind
+            const int steps = ranks >= BK ? BK / 16 : (ranks + 15) / 16;
+            for (int k = 0; k < steps; ++k)
+              tc_mma_ss_masked(d_tmem, sw_desc(a_addr + k * 32, (uint32_t)p.lora_sw),
+                               sw_desc(b_addr + k * 32, (uint32_t)p.lora_sw), idesc, 1u, off);
             tc_commit(&empty[stage]);
             if (++stage == C::STAGES) {
               stage = 0;
@@ -1059,7 +1060,7 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
   a.pre_b = (fz != nullptr && fz->w_static) ? 1 : 0;
   a.lora_cnt = nullptr;
   a.lora_slots = nullptr;
-  a.lora_max = a.lora_blocks = 0;
+  a.lora_max = a.lora_blocks = a.lora_sw = a.lora_rank = 0;
   int fuse = gemm::FUSE_NONE;
   if (lora) {
     if (w_dtype != CK_BF16 || w_layout != CK_W_NK || (epi != CK_EPI_STORE && epi != CK_EPI_BIAS))
@@ -1068,6 +1069,8 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
     a.lora_slots = reinterpret_cast<const uint4*>(fz->lora_slots);
     a.lora_max = fz->lora_max;
     a.lora_blocks = (fz->lora_rank + BK - 1) / BK;
+    a.lora_rank = fz->lora_rank;
+    a.lora_sw = fz->lora_rank <= 16 ? 32 : (fz->lora_rank <= 32 ? 64 : 128);
     fuse = gemm::FUSE_LORA;
   } else if (fz != nullptr && fz->ln_out != nullptr) {
     // LayerNorm of the residual output as a second output: whole rows of
@@ -1130,7 +1133,7 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
       return CK_ERR_INVALID_ARG;
   } else if (lora) {
     if (!make_tmap_2d(&ty2, fz->lora_h, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, fz->lora_h_ld, M,
-                      fz->lora_h_ld, BK, BM, 128))
+                      fz->lora_h_ld, a.lora_sw / 2, BM, a.lora_sw))
       return CK_ERR_INVALID_ARG;
   } else {
     ty2 = ty;
@@ -1144,7 +1147,7 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
       return CK_ERR_INVALID_ARG;
   } else if (lora) {
     if (!make_tmap_2d(&tr, fz->lora_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, fz->lora_rank,
-                      (uint64_t)fz->lora_n * N, fz->lora_b_ld, BK, BN, 128))
+                      (uint64_t)fz->lora_n * N, fz->lora_b_ld, a.lora_sw / 2, BN, a.lora_sw))
       return CK_ERR_INVALID_ARG;
   } else {
     tr = ty;

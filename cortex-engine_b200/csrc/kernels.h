@@ -56,7 +56,7 @@ int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cud
 
 bool make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int elem_bytes,
                   uint64_t inner, uint64_t outer, uint64_t ld_elems, uint32_t box_inner,
-                  uint32_t box_outer, int swizzle_bytes /* 0, 64 or 128 */);
+                  uint32_t box_outer, int swizzle_bytes /* 0, 32, 64 or 128 */);
 
 // tcgen05 GEMM (gemm_tc.cu)
 bool gemm_tc_supported(int64_t M, int64_t K, int64_t lda, int w_dtype, int w_layout, int64_t N,

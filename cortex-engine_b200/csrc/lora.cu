@@ -38,6 +38,7 @@ struct TileParams {
   __nv_bfloat16* h;   // [M][ld_h], ld_h = rank rounded up to 8, zero behind rank
   int32_t ld_h;
   int32_t max_slots;  // per tile
+  int32_t tiles;
   int32_t* cnt;       // [tiles]
   uint4* slots;       // [tiles][max_slots][2]
 };
@@ -465,25 +466,26 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
 
 // ── many rows: h and the tiles' adapters ─────────────────────────────────────
 //
-// A cluster of SK CTAs per 128-row tile of x. It lists the tile's adapters in
-// the order of their first row (with, for each, the rows that are not its own)
-// and computes D_i[128 x RP] = x_tile A_i^T for SL of them at a time: both
-// operands by TMA into a ring of 64-wide K blocks, the SL accumulators side by
+// A cluster of SK CTAs per 128-row tile of x and SL adapters. It lists the
+// tile's adapters in the order of their first row (with, for each, the rows that
+// are not its own) and computes D_i[128 x RP] = x_tile A_i^T for its SL of them:
+// both operands by TMA into a ring of 64-wide K blocks, the accumulators side by
 // side in TMEM, each CTA an SK-th of K. A row then takes the columns of its own
 // adapter; the ranks' partials meet in distributed shared memory, each CTA
 // finishing RP / SK columns: sum in rank order, times s_i, rounded to bf16 for
-// the GEMM's operand. Bound by x, read once for up to SL adapters a tile (every
-// further SL read it again, from L2).
+// the GEMM's operand. Bound by x, read once a cluster; clusters whose SL the tile
+// has no adapters for leave after the list. h of rows without an adapter stays
+// unwritten: no block of the GEMM uses it.
 template <int RP, int SK>
 struct TilesCfg {
-  static constexpr int SL = 2;
+  static constexpr int SL = RP == 16 ? 8 : 4;
   static constexpr int X_BYTES = 128 * 128;
   static constexpr int A_BYTES = RP * 128;
   static constexpr int STAGE = X_BYTES + SL * A_BYTES;
-  static constexpr int STAGES = RP == 64 ? 4 : 5;
-  static constexpr int PART = RP * 128 * 4;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + PART + 256;
-  static constexpr uint32_t COLS = SL * RP < 32 ? 32 : SL * RP;
+  static constexpr int STAGES = 96 * 1024 / STAGE;  // two CTAs an SM
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
+  static constexpr uint32_t COLS = SL * RP;
+  static_assert(RP * 128 * 4 <= STAGES * STAGE, "the partials lie over the drained ring");
 };
 
 template <int RP, int SK>
@@ -498,8 +500,8 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
                                              ~uintptr_t(1023));
   uint8_t* sX = smem;
   uint8_t* sA = smem + C::STAGES * C::X_BYTES;
-  float* part = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE);  // [RP][128]
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE + C::PART);
+  float* part = reinterpret_cast<float*>(smem);  // [RP][128], once the ring is drained
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE);
   uint64_t* empty = full + C::STAGES;
   uint64_t* done = empty + C::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -507,7 +509,8 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
   const ck_lora_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = SK > 1 ? (int)cl_rank() : 0;
-  const int tile = blockIdx.x / SK;
+  const int tile = (int)(blockIdx.x / SK) % p.tiles;
+  const int slot0 = (int)(blockIdx.x / SK) / p.tiles * C::SL;  // this cluster's first adapter of the tile
   const int kb_all = (int)((a.K + 63) / 64);
   const int kb_per = (kb_all + SK - 1) / SK;
   const int kb0 = min(kb_all, rank * kb_per), kb1 = min(kb_all, kb0 + kb_per);
@@ -537,7 +540,8 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
 
   // the tile's adapters
   const int64_t m = (int64_t)tile * 128 + tid;
-  const int id = m < a.M ? adapter_of(a, m, rank == 0) : -1;
+  const bool lists = rank == 0 && slot0 == 0;  // the CTA that writes the tile's list
+  const int id = m < a.M ? adapter_of(a, m, lists) : -1;
   s_id[tid] = id;
   __syncthreads();
   const uint32_t lt = (1u << lane) - 1u;
@@ -560,21 +564,21 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
     const bool mine = id == s_list[i];
     const uint32_t mask = __ballot_sync(0xffffffffu, mine);
     if (mine) slot = i;
-    if (rank == 0) {
+    if (lists) {
       uint4* dst = p.slots + 2 * ((int64_t)tile * p.max_slots + i);
       if (lane == 0) reinterpret_cast<uint32_t*>(dst + 1)[warp] = ~mask;
       if (tid == 0) dst[0] = make_uint4((uint32_t)s_list[i], 0u, 0u, 0u);
     }
   }
-  if (rank == 0 && tid == 0) p.cnt[tile] = total;
+  if (lists && tid == 0) p.cnt[tile] = total;
   const float scale = id >= 0 && a.scaling != nullptr ? __ldg(a.scaling + id) : 1.f;
 
-  const int rank_blocks = (a.rank + RP - 1) / RP;
-  const int passes = (total + C::SL - 1) / C::SL * rank_blocks;
+  // a pass per RP ranks (one, up to 64); none without adapters from slot0 on
+  const int n_slots = min(C::SL, total - slot0);
+  const int passes = n_slots > 0 ? (a.rank + RP - 1) / RP : 0;
   int it = 0;  // K blocks so far, of the producing and of the multiplying thread
   for (int pass = 0; pass < passes; ++pass) {
-    const int slot0 = pass / rank_blocks * C::SL, j0 = pass % rank_blocks * RP;
-    const int n_slots = min(C::SL, total - slot0);
+    const int j0 = pass * RP;
     if (warp == 0 && lane == 0) {
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
         const int s = it % C::STAGES;
@@ -608,15 +612,20 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
     tc_fence_after();
     const int mine = slot - slot0;  // 0 .. n_slots - 1: this row's columns are here
     const bool take = mine >= 0 && mine < n_slots;
+    for (int i = 0; i < n_slots; ++i) {
+      if (!__any_sync(0xffffffffu, mine == i)) continue;
 #pragma unroll
-    for (int c = 0; c < RP; c += 16) {
-      uint32_t v[C::SL][16];
+      for (int c = 0; c < RP; c += 16) {
+        uint32_t v[16];
+        tmem_ld16w(tmem + ((uint32_t)(warp * 32) << 16) + i * RP + c, v);
+        tc_wait_ld();
+        if (mine == i) {
 #pragma unroll
-      for (int i = 0; i < C::SL; ++i) tmem_ld16w(tmem + ((uint32_t)(warp * 32) << 16) + i * RP + c, v[i]);
-      tc_wait_ld();
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        part[(c + e) * 128 + tid] = kb1 > kb0 ? __uint_as_float(mine == 1 ? v[1][e] : v[0][e]) : 0.f;
+          for (int e = 0; e < 16; ++e)
+            part[(c + e) * 128 + tid] = kb1 > kb0 ? __uint_as_float(v[e]) : 0.f;
+        }
+        __syncwarp();
+      }
     }
     tc_fence_before();
     if (SK > 1) cl_sync(); else __syncthreads();
@@ -647,7 +656,8 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
           *reinterpret_cast<uint32_t*>(p.h + m * p.ld_h + j0 + c0 + c) = cvt_bf16x2(v[0], v[1]);
       }
     }
-    // the partials and the accumulators are free again
+    // the partials (for the next pass's copies) and the accumulators are free again
+    fence_proxy_async_smem();
     if (SK > 1) cl_sync(); else __syncthreads();
     tc_fence_after();
   }
@@ -913,7 +923,7 @@ int make_plan(const ck_lora_args& a, LoraPlan& pl) {
   if (a.M < 0 || a.N < 0 || a.K <= 0 || a.rank < 1 || a.n_adapters < 0) return CK_ERR_INVALID_ARG;
   if (a.M > INT32_MAX || a.N > INT32_MAX || a.K > INT32_MAX) return CK_ERR_UNSUPPORTED;
   if (a.rank > 256) return CK_ERR_UNSUPPORTED;
-  if (((a.M + 31) / 32) * ((a.N + 63) / 64) > INT32_MAX || (a.M * a.rank + 7) / 8 > INT32_MAX)
+  if (a.M > (int64_t)1 << 28 || ((a.M + 31) / 32) * ((a.N + 63) / 64) > INT32_MAX || (a.M * a.rank + 7) / 8 > INT32_MAX)
     return CK_ERR_UNSUPPORTED;
   pl.p.a = a;
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
@@ -1048,7 +1058,8 @@ int launch_tiles(const TileParams& t, int tiles, cudaStream_t st) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * SK));
+  const int groups = (t.max_slots + C::SL - 1) / C::SL;
+  cfg.gridDim = dim3((unsigned)((int64_t)tiles * groups * SK));
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = (size_t)C::SMEM;
   cfg.stream = st;
@@ -1094,6 +1105,7 @@ int run_tiles(const LoraPlan& pl, uint8_t* ws, cudaStream_t st) {
   t.h = reinterpret_cast<__nv_bfloat16*>(ws + pl.off_h);
   t.ld_h = pl.ld_h;
   t.max_slots = pl.max_slots;
+  t.tiles = pl.tiles;
   t.cnt = reinterpret_cast<int32_t*>(ws + pl.off_cnt);
   t.slots = reinterpret_cast<uint4*>(ws + pl.off_slots);
   rc = a.rank <= 16 ? launch_tiles_k<16>(t, pl.tiles, st)
