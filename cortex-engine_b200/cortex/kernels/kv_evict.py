@@ -19,13 +19,17 @@ from cortex.kernels.paged_attention import check_pages, rows_contiguous
 _pack = L.EVICT_ARGS.pack
 
 
-def _table(what: str, t: torch.Tensor, dtype: torch.dtype, B: int, width: int) -> None:
-    if t.dtype != dtype:
+def _table(what: str, t: torch.Tensor, dtype: torch.dtype, B: int, width: int) -> tuple[int, int]:
+    """(row stride, columns) of a (B, >= width) table."""
+    if t.dtype is not dtype:
         raise TypeError(f"evict_by_weight: {what} must be {dtype}, got {t.dtype}")
-    if t.dim() != 2 or t.shape[0] != B or t.shape[1] < width:
-        raise ValueError(f"evict_by_weight: {what} must be ({B}, >= {width}), got {tuple(t.shape)}")
-    if not rows_contiguous(t):
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != B or shape[1] < width:
+        raise ValueError(f"evict_by_weight: {what} must be ({B}, >= {width}), got {tuple(shape)}")
+    ld, step = t.stride()
+    if step != 1 and shape[1] > 1:
         raise ValueError(f"evict_by_weight: {what} rows must be contiguous")
+    return ld, shape[1]
 
 
 def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -67,23 +71,23 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
         L.require_cuda(pool, page_table, lengths, weights, positions, *(out or ()),
                        what="evict_by_weight")
     check_pages("evict_by_weight", pool, page_table, lengths)
-    if pool.dtype != torch.bfloat16 and pool.dtype != torch.float32:
+    if pool.dtype is not torch.bfloat16 and pool.dtype is not torch.float32:
         raise NotImplementedError(f"evict_by_weight: rows of {pool.dtype}")
     if not 1 <= budget < 2 ** 31 or not 0 <= recent <= budget:
         raise ValueError(f"evict_by_weight: needs 1 <= budget and 0 <= recent <= budget, "
                          f"got {budget} and {recent}")
-    B = lengths.shape[0]
+    B, table_width = page_table.shape
     pages, page_size, width = pool.shape
-    table_width = page_table.shape[1]
     cap = table_width * page_size
-    _table("weights", weights, torch.float32, B, cap)
-    _table("positions", positions, torch.int32, B, cap)
+    w_ld, w_cols = _table("weights", weights, torch.float32, B, cap)
+    pos_ld, pos_cols = _table("positions", positions, torch.int32, B, cap)
     dev = pool.device
     fill = out is None
     if fill:
         new_len = torch.empty(B, dtype=torch.int32, device=dev)
         new_w = torch.empty(B, budget, dtype=torch.float32, device=dev)
         new_pos = torch.empty(B, budget, dtype=torch.int32, device=dev)
+        new_w_ld = new_pos_ld = new_cols = budget
         if not rows_contiguous(lengths):
             lengths = lengths.contiguous()
     else:
@@ -92,17 +96,17 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
             raise ValueError("evict_by_weight: out lengths must be like lengths")
         if not rows_contiguous(new_len) or not rows_contiguous(lengths):
             raise ValueError("evict_by_weight: lengths must be contiguous")
-        _table("out weights", new_w, torch.float32, B, min(budget, cap))
-        _table("out positions", new_pos, torch.int32, B, min(budget, cap))
+        new_w_ld, new_cols = _table("out weights", new_w, torch.float32, B, min(budget, cap))
+        new_pos_ld, n = _table("out positions", new_pos, torch.int32, B, min(budget, cap))
+        new_cols = min(new_cols, n)
     if not rows_contiguous(page_table):
         page_table = page_table.contiguous()
     page_ld, row_ld, _ = pool.stride()
     block = _pack(pool.element_size(), B, pool.data_ptr(), pages, page_ld, row_ld, page_size, width,
-                  page_table.data_ptr(), page_table.stride(0), table_width, budget, recent, fill,
+                  page_table.data_ptr(), page_table.stride()[0], table_width, budget, recent, fill,
                   lengths.data_ptr(), new_len.data_ptr(), weights.data_ptr(), new_w.data_ptr(),
-                  positions.data_ptr(), new_pos.data_ptr(), weights.stride(0), new_w.stride(0),
-                  positions.stride(0), new_pos.stride(0),
-                  min(weights.shape[1], positions.shape[1]), min(new_w.shape[1], new_pos.shape[1]))
+                  positions.data_ptr(), new_pos.data_ptr(), w_ld, new_w_ld, pos_ld, new_pos_ld,
+                  min(w_cols, pos_cols), new_cols)
     lib = L.load()
     with L.on_device(dev):
         n = L.workspace_bytes(lib.ck_evict_workspace_bytes, ("evict", d, B, cap, budget), block)

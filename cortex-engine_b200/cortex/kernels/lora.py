@@ -19,6 +19,13 @@ from cortex.kernels.paged_attention import rows_contiguous
 _pack = L.LORA_ARGS.pack
 
 
+def _three(what: str, t: torch.Tensor) -> tuple[int, int, int]:
+    shape = tuple(t.shape)
+    if len(shape) != 3:
+        raise ValueError(f"lora_linear: {what} must have 3 dimensions, got {shape}")
+    return shape
+
+
 def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                 adapter_ids: torch.Tensor, *, scaling: torch.Tensor | None = None,
                 bias: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -45,20 +52,20 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
             (scaling is not None and scaling.get_device() != d) or \
             (bias is not None and bias.get_device() != d) or out is not None:
         L.require_cuda(x, w, lora_a, lora_b, adapter_ids, scaling, bias, out, what="lora_linear")
-    dtype, lead = x.dtype, x.shape[:-1]
-    K = x.shape[-1] if x.dim() > 0 else -1
-    if w.dim() != 2 or w.shape[1] != K or K < 1:
-        raise ValueError(f"lora_linear: w must be (N, K) with K = {K}, got {tuple(w.shape)}")
-    N = w.shape[0]
-    if lora_a.dim() != 3 or lora_a.shape[2] != K or lora_a.shape[1] < 1:
+    dtype, xs, ws, (n, rank, a_k) = x.dtype, x.shape, w.shape, _three("lora_a", lora_a)
+    K = xs[-1] if len(xs) > 0 else -1
+    lead = xs[:-1]
+    if len(ws) != 2 or ws[1] != K or K < 1:
+        raise ValueError(f"lora_linear: w must be (N, K) with K = {K}, got {tuple(ws)}")
+    N = ws[0]
+    if a_k != K or rank < 1:
         raise ValueError(f"lora_linear: lora_a must be (n, rank, {K}), got {tuple(lora_a.shape)}")
-    n, rank, _ = lora_a.shape
-    if lora_b.shape != (n, N, rank):
+    if _three("lora_b", lora_b) != (n, N, rank):
         raise ValueError(f"lora_linear: lora_b must be {(n, N, rank)}, got {tuple(lora_b.shape)}")
-    if dtype != w.dtype or dtype != lora_a.dtype or dtype != lora_b.dtype:
+    if dtype is not w.dtype or dtype is not lora_a.dtype or dtype is not lora_b.dtype:
         raise TypeError(f"lora_linear: x, w, lora_a and lora_b differ in dtype ({dtype}, "
                         f"{w.dtype}, {lora_a.dtype}, {lora_b.dtype})")
-    if adapter_ids.dtype != torch.int32:
+    if adapter_ids.dtype is not torch.int32:
         raise TypeError(f"lora_linear: adapter_ids must be int32, got {adapter_ids.dtype}")
     if adapter_ids.shape != lead:
         raise ValueError(f"lora_linear: adapter_ids must be {tuple(lead)}, "
@@ -78,16 +85,18 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         lora_b = lora_b.contiguous()
     scaling_ptr = bias_ptr = 0
     if scaling is not None:
-        if scaling.dtype != torch.float32 or scaling.shape != (n,):
+        if scaling.dtype is not torch.float32 or scaling.shape != (n,):
             raise ValueError(f"lora_linear: scaling must be float32 ({n},)")
-        scaling = scaling.contiguous()
+        if not scaling.is_contiguous():
+            scaling = scaling.contiguous()
         scaling_ptr = scaling.data_ptr()
     if bias is not None:
         if bias.dtype != dtype or bias.shape != (N,):
             raise ValueError(f"lora_linear: bias must be {dtype} ({N},)")
-        bias = bias.contiguous()
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
         bias_ptr = bias.data_ptr()
-    M, dev = x2.shape[0], x.device
+    M, dev = len(x2), x.device
     if out is None:
         y = torch.empty(M, N, dtype=dtype, device=dev)
     else:
@@ -98,7 +107,7 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
             raise ValueError("lora_linear: out rows must be contiguous")
     x_ptr, w_ptr, y_ptr = x2.data_ptr(), w.data_ptr(), y.data_ptr()
     a_ptr, b_ptr = lora_a.data_ptr(), lora_b.data_ptr()
-    ldx, ldw, ldy = x2.stride(0), w.stride(0), y.stride(0)
+    ldx, ldw, ldy = x2.stride()[0], w.stride()[0], y.stride()[0]
     block = _pack(L.dtype_code(dtype), n, rank, M, K, N, x_ptr, ldx, w_ptr, ldw, a_ptr, b_ptr,
                   ids.data_ptr(), scaling_ptr, bias_ptr, y_ptr, ldy)
     lib = L.load()

@@ -26,20 +26,22 @@ def check_pages(what: str, pool: torch.Tensor, page_table: torch.Tensor,
     if pool.dim() != 3:
         raise ValueError(f"{what}: pool must be (num_pages, page_size, width), "
                          f"got {tuple(pool.shape)}")
-    if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+    if page_table.dtype is not torch.int32 or lengths.dtype is not torch.int32:
         raise TypeError(f"{what}: page_table and lengths must be int32, got "
                         f"{page_table.dtype} and {lengths.dtype}")
-    if page_table.dim() != 2 or lengths.dim() != 1 or page_table.shape[0] != lengths.shape[0]:
+    if page_table.dim() != 2 or lengths.dim() != 1 or len(page_table) != len(lengths):
         raise ValueError(f"{what}: page_table must be (B, pages) beside lengths (B,), got "
                          f"{tuple(page_table.shape)} and {tuple(lengths.shape)}")
-    if pool.shape[1] < 1 or pool.shape[2] < 1:
+    _, page_size, width = pool.shape
+    if page_size < 1 or width < 1:
         raise ValueError(f"{what}: pages must hold at least one row of one element")
-    if pool.stride(2) != 1 and pool.shape[2] > 1:
+    if pool.stride()[2] != 1 and width > 1:
         raise ValueError(f"{what}: pool rows must be contiguous")
 
 
 def rows_contiguous(t: torch.Tensor) -> bool:
-    return t.stride(-1) == 1 or t.shape[-1] <= 1
+    """Whether the elements of a row (the last dimension) lie next to each other."""
+    return t.is_contiguous() or t.stride()[-1] == 1 or t.shape[-1] <= 1
 
 
 def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
@@ -76,11 +78,11 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
                        what="paged_attention")
     check_pages("paged_attention", pool, page_table, lengths)
     dtype = q.dtype
-    if dtype != pool.dtype:
+    if dtype is not pool.dtype:
         raise TypeError(f"paged_attention: q is {dtype}, the pool {pool.dtype}")
-    B = lengths.shape[0]
+    B = len(lengths)
     pages, page_size, width = pool.shape
-    if q.dim() != 3 or q.shape[0] != B:
+    if q.dim() != 3 or len(q) != B:
         raise ValueError(f"paged_attention: q must be (B, H, Dh) with B = {B}, got {tuple(q.shape)}")
     _, H, Dh = q.shape
     if Dh == 0 or width % (2 * Dh) != 0:
@@ -112,14 +114,14 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
         if not rows_contiguous(weights) or not rows_contiguous(weights_out):
             raise ValueError("paged_attention: weights rows must be contiguous")
         W, w_in, w_out = weights.shape[1], weights.data_ptr(), weights_out.data_ptr()
-        w_in_ld, w_out_ld = weights.stride(0), weights_out.stride(0)
+        w_in_ld, w_out_ld = weights.stride()[0], weights_out.stride()[0]
     elif weights_out is not None:
         raise ValueError("paged_attention: weights_out without weights")
     qb, qh, _ = q.stride()
     pb, pr, _ = pool.stride()
     ob, oh, _ = out.stride()
     q_ptr, pool_ptr = q.data_ptr(), pool.data_ptr()
-    block = _pack(L.dtype_code(dtype), B, H, Hkv, Dh, q_ptr, qb, qh, pool_ptr, pages, pb, pr, page_size, table_width, page_table.data_ptr(), page_table.stride(0),
+    block = _pack(L.dtype_code(dtype), B, H, Hkv, Dh, q_ptr, qb, qh, pool_ptr, pages, pb, pr, page_size, table_width, page_table.data_ptr(), page_table.stride()[0],
                   lengths.data_ptr(), out.data_ptr(), ob, oh, w_in, w_out, w_in_ld, w_out_ld, W,
                   Dh ** -0.5 if scale is None else scale)
     lib = L.load()

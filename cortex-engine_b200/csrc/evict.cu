@@ -446,7 +446,8 @@ int make_plan(const ck_evict_args& a, EvictPlan& pl) {
   const size_t list = up((size_t)a.B * p.max_moves * 4);
   pl.off_holes = up((size_t)a.B * 4);
   pl.off_movers = pl.off_holes + list;
-  pl.bytes = p.max_moves > 0 ? pl.off_movers + list : 0;
+  // (one CTA a sequence and few movers: they never leave shared memory)
+  pl.bytes = p.max_moves > 0 && !(pl.cs == 1 && p.max_moves <= kFewMoves) ? pl.off_movers + list : 0;
   return CK_OK;
 }
 
@@ -490,7 +491,7 @@ int evict_by_weight(const ck_evict_args& a, void* ws, size_t ws_bytes, cudaStrea
                        (reinterpret_cast<uintptr_t>(ws) & 15u) != 0))
     return CK_ERR_WORKSPACE;
   uint8_t* w = reinterpret_cast<uint8_t*>(ws);
-  p.counts = p.max_moves > 0 ? reinterpret_cast<int32_t*>(w) : nullptr;
+  p.counts = reinterpret_cast<int32_t*>(w);
   p.holes = reinterpret_cast<int32_t*>(w + pl.off_holes);
   p.movers = reinterpret_cast<int32_t*>(w + pl.off_movers);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(a.pool) | (uintptr_t)(a.page_ld * a.elem_bytes) |

@@ -61,9 +61,9 @@ def test_paged_attention_refusals():
 
 def _evict(**kw):
     base = dict(elem_bytes=2, B=2, pool=16, num_pages=8, page_ld=16 * 64, row_ld=64, page_size=16,
-                width=64, page_table=16, page_table_ld=4, page_table_width=4, budget=20, recent=3,
+                width=64, page_table=16, page_table_ld=100, page_table_width=100, budget=500, recent=3,
                 fill=1, lengths=16, lengths_out=32, w_in=16, w_out=32, pos_in=16, pos_out=32,
-                w_in_ld=64, w_out_ld=20, pos_in_ld=64, pos_out_ld=20, in_width=64, out_width=20)
+                w_in_ld=1600, w_out_ld=500, pos_in_ld=1600, pos_out_ld=500, in_width=1600, out_width=500)
     base.update(kw)
     return bytes(L.EvictArgs(**base))
 
@@ -78,8 +78,8 @@ def test_evict_refusals():
 
     assert lib.ck_evict_by_weight(None, 0, 0, 0) == L.CK_ERR_INVALID_ARG
     assert rc(elem_bytes=1) == L.CK_ERR_UNSUPPORTED
-    for bad in (dict(B=-1), dict(budget=0), dict(recent=21), dict(recent=-1), dict(width=0),
-                dict(page_size=0), dict(in_width=63), dict(out_width=19), dict(num_pages=-1),
+    for bad in (dict(B=-1), dict(budget=0), dict(recent=501), dict(recent=-1), dict(width=0),
+                dict(page_size=0), dict(in_width=1599), dict(out_width=499), dict(num_pages=-1),
                 dict(page_table_width=2 ** 28), dict(w_out=16), dict(pos_out=16)):
         assert rc(**bad) == L.CK_ERR_INVALID_ARG, bad
     for missing in ("lengths", "lengths_out", "w_in", "w_out", "pos_in", "pos_out", "pool",
@@ -88,8 +88,9 @@ def test_evict_refusals():
     assert rc(ws=0) == L.CK_ERR_WORKSPACE
     assert rc(n=need - 1) == L.CK_ERR_WORKSPACE
     assert rc(B=0) == L.CK_OK
-    # a budget that no sequence can pass needs no workspace
-    assert lib.ck_evict_workspace_bytes(_evict(budget=64, out_width=64)) == 0
+    # a budget that no sequence can pass, or by a few rows only, needs no workspace
+    assert lib.ck_evict_workspace_bytes(_evict(budget=1600, out_width=1600)) == 0
+    assert lib.ck_evict_workspace_bytes(_evict(budget=1580, out_width=1600)) == 0
     assert lib.ck_evict_workspace_bytes(None) == 0
 
 
