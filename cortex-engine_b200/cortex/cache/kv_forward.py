@@ -52,7 +52,8 @@ def forward_with_kv_cache(model, windows: list[dict], cache) -> torch.Tensor:
         if not len(e[0]) == len(e[1]) == len(e[2]):
             raise ValueError(f"window {b}: neuron_ids, time_bins and values differ in length")
     metas = [cache.lookup(w["session_id"], int(w["bin_start"])) for w in windows]
-    hit = [mt is not None and mt.n_events == counts[b] for b, mt in enumerate(metas)]
+    hit = [mt is not None and mt.n_events == counts[b] and not mt.edited
+           for b, mt in enumerate(metas)]
     miss = [b for b in range(B) if not hit[b]]
 
     m = model.native_model()

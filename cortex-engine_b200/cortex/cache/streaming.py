@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import time
 from collections import OrderedDict
+from collections.abc import Sequence
 from dataclasses import dataclass, field
 
 import torch
@@ -44,6 +45,7 @@ class PageMeta:
     n_events: int
     last_used_at: float
     pages: list[int] = field(default_factory=list)
+    edited: bool = False  # rows appended or evicted since the entry was written
 
 
 class StreamingKVCache:
@@ -148,6 +150,103 @@ class StreamingKVCache:
             out.append((b, p, n) if into_pool else (p, b, n))
         return out
 
+    # ── entries that grow and shrink ─────────────────────────────────────────
+
+    @property
+    def pool(self) -> torch.Tensor:
+        """(num_pages, page_size, hidden_dim), the pages themselves."""
+        return self._pool
+
+    def page_table(self, metas: Sequence[PageMeta]) -> tuple[torch.Tensor, torch.Tensor]:
+        """(page_table (B, pages) int32, lengths (B,) int32) of entries on the
+        device, as ``paged_attention`` takes them. The copy is queued on the
+        current stream. Entries may be listed more than once."""
+        self._check_live(metas, distinct=False)
+        width = max((len(m.pages) for m in metas), default=0)
+        host = torch.zeros(len(metas), width + 1, dtype=torch.int32)
+        for b, m in enumerate(metas):
+            host[b, 0] = m.n_events
+            host[b, 1:1 + len(m.pages)] = torch.tensor(m.pages, dtype=torch.int32)
+            self._lru.move_to_end(m.page_id)
+        dev = host.pin_memory().to(self.device, non_blocking=True)
+        return dev[:, 1:], dev[:, 0].contiguous()
+
+    def append_rows(self, metas: Sequence[PageMeta], rows: torch.Tensor) -> None:
+        """Add ``rows[b]`` ((B, n, hidden_dim), the pool's dtype) behind the rows
+        of every entry (all different), in pages taken from the pool; least
+        recently used entries that are not listed make room. Raises
+        ``RuntimeError``, changing nothing, when the pool cannot hold them."""
+        self._check_live(metas, distinct=True)
+        dev = L.require_cuda(rows, what="append_rows")
+        if rows.dim() != 3 or rows.shape[0] != len(metas) or rows.shape[2] != self.hidden_dim:
+            raise ValueError(f"append_rows: rows must be ({len(metas)}, n, {self.hidden_dim}), "
+                             f"got {tuple(rows.shape)}")
+        if rows.dtype != self._pool.dtype or dev != self.device:
+            raise ValueError(f"append_rows: rows must be {self._pool.dtype} on {self.device}")
+        n = rows.shape[1]
+        if not metas or n == 0:
+            return
+        row_bytes = self.hidden_dim * rows.element_size()
+        if row_bytes % 16 != 0:
+            raise NotImplementedError("append_rows: rows must be a multiple of 16 bytes")
+        need = [max(0, -(-(m.n_events + n) // self.page_size) - len(m.pages)) for m in metas]
+        listed = {m.page_id for m in metas}
+        spare = len(self._free) + sum(len(m.pages) for e, m in self._meta.items() if e not in listed)
+        if sum(need) > spare:
+            raise RuntimeError(f"append_rows: {sum(need)} pages needed, {spare} can be had")
+        for m in metas:  # most recent: never the ones that make room below
+            self._lru.move_to_end(m.page_id)
+        segs = []
+        for b, (m, k) in enumerate(zip(metas, need)):
+            m.pages.extend(self._allocate(k))
+            at, end = m.n_events, m.n_events + n
+            while at < end:
+                page, off = divmod(at, self.page_size)
+                take = min(self.page_size - off, end - at)
+                segs.append((b * n + at - m.n_events, m.pages[page] * self.page_size + off, take))
+                at += take
+            m.n_events = end
+            m.edited = True
+            m.last_used_at = time.monotonic()
+        src = rows.contiguous()
+        with L.on_device(self.device):
+            seg = torch.tensor(segs, dtype=torch.int32).pin_memory().to(self.device,
+                                                                       non_blocking=True)
+            rc = L.load().ck_copy_rows(src.data_ptr(), len(metas) * n, self.rows.data_ptr(),
+                                       self.num_pages * self.page_size, row_bytes, seg.data_ptr(),
+                                       len(segs), L.stream_of(self.device))
+        L.check(rc, "ck_copy_rows")
+
+    def evict_rows(self, metas: Sequence[PageMeta], weights: torch.Tensor,
+                   positions: torch.Tensor, *, budget: int, recent: int = 0) -> None:
+        """``evict_by_weight`` on the rows of entries (all different): each keeps
+        ``budget`` rows at most, ``weights`` and ``positions`` ((B, slots) float32
+        and int32, slots >= the longest entry's pages * page_size) change in place,
+        and the pages behind the budget go back to the pool."""
+        from cortex.kernels.kv_evict import evict_by_weight
+
+        self._check_live(metas, distinct=True)
+        if not metas:
+            return
+        table, lengths = self.page_table(metas)
+        evict_by_weight(self._pool, table, lengths, weights, positions, budget=budget,
+                        recent=recent, out=(lengths, weights, positions))
+        for m in metas:
+            if m.n_events > budget:
+                keep = max(1, -(-budget // self.page_size))
+                self._free.extend(m.pages[keep:])
+                del m.pages[keep:]
+                m.n_events = budget
+                m.edited = True
+            m.last_used_at = time.monotonic()
+
+    def _check_live(self, metas: Sequence[PageMeta], distinct: bool) -> None:
+        for m in metas:
+            if not self.is_live(m):
+                raise ValueError(f"entry ({m.session_id!r}, {m.bin_start}) is no longer in the cache")
+        if distinct and len({m.page_id for m in metas}) != len(metas):
+            raise ValueError("an entry is listed more than once")
+
     def is_live(self, meta: PageMeta) -> bool:
         """Whether ``meta`` is still the entry that owns its pages."""
         return self._meta.get(meta.page_id) is meta
@@ -172,6 +271,7 @@ class StreamingKVCache:
             self._meta[eid] = PageMeta(eid, session_id, bin_start, 0, time.monotonic(), pages)
             self._lru[eid] = None
         self._lru.move_to_end(eid)
+        self._meta[eid].edited = False
         return self._meta[eid]
 
     def _allocate(self, n_pages: int) -> list[int]:
