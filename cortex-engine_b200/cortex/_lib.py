@@ -316,22 +316,19 @@ def workspace_bytes(query, key: tuple, block: bytes) -> int:
     return n
 
 
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
+_get_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
-_NO_GUARD = _NoGuard()
+def current_device() -> int:
+    """Index of the current CUDA device."""
+    return _get_device() if _get_device is not None else torch.cuda.current_device()
 
 
-def on_device(device: torch.device):
-    """Context in which ``device`` is the current one (a no-op where it already is)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _NO_GUARD
-    return torch.cuda.device(device)
+def raw_stream(index: int) -> int:
+    """The handle of torch's current CUDA stream on device ``index``."""
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 def require_cuda(*tensors: torch.Tensor, what: str) -> torch.device:

@@ -209,7 +209,7 @@ class StreamingKVCache:
             m.edited = True
             m.last_used_at = time.monotonic()
         src = rows.contiguous()
-        with L.on_device(self.device):
+        with torch.cuda.device(self.device):
             seg = torch.tensor(segs, dtype=torch.int32).pin_memory().to(self.device,
                                                                        non_blocking=True)
             rc = L.load().ck_copy_rows(src.data_ptr(), len(metas) * n, self.rows.data_ptr(),

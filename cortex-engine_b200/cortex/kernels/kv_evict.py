@@ -70,6 +70,10 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
             weights.get_device() != d or positions.get_device() != d or out is not None:
         L.require_cuda(pool, page_table, lengths, weights, positions, *(out or ()),
                        what="evict_by_weight")
+    if d != L.current_device():
+        with torch.cuda.device(d):
+            return evict_by_weight(pool, page_table, lengths, weights, positions, budget=budget,
+                                   recent=recent, out=out)
     check_pages("evict_by_weight", pool, page_table, lengths)
     if pool.dtype is not torch.bfloat16 and pool.dtype is not torch.float32:
         raise NotImplementedError(f"evict_by_weight: rows of {pool.dtype}")
@@ -108,10 +112,9 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
                   positions.data_ptr(), new_pos.data_ptr(), w_ld, new_w_ld, pos_ld, new_pos_ld,
                   min(w_cols, pos_cols), new_cols)
     lib = L.load()
-    with L.on_device(dev):
-        n = L.workspace_bytes(lib.ck_evict_workspace_bytes, ("evict", d, B, cap, budget), block)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        rc = lib.ck_evict_by_weight(block, ws.data_ptr() if n else 0, n, L.stream_of(dev))
+    n = L.workspace_bytes(lib.ck_evict_workspace_bytes, ("evict", d, B, cap, budget), block)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    rc = lib.ck_evict_by_weight(block, ws.data_ptr() if n else 0, n, L.raw_stream(d))
     if rc != L.CK_OK:
         L.check(rc, "ck_evict_by_weight")
     return new_len, new_w, new_pos

@@ -52,6 +52,9 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
             (scaling is not None and scaling.get_device() != d) or \
             (bias is not None and bias.get_device() != d) or out is not None:
         L.require_cuda(x, w, lora_a, lora_b, adapter_ids, scaling, bias, out, what="lora_linear")
+    if d != L.current_device():
+        with torch.cuda.device(d):
+            return lora_linear(x, w, lora_a, lora_b, adapter_ids, scaling=scaling, bias=bias, out=out)
     dtype, xs, ws, (n, rank, a_k) = x.dtype, x.shape, w.shape, _three("lora_a", lora_a)
     K = xs[-1] if len(xs) > 0 else -1
     lead = xs[:-1]
@@ -73,10 +76,15 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     ids, x2 = adapter_ids, x
     if len(lead) != 1:
         ids, x2 = ids.reshape(-1), x.reshape(-1, K)
-    if not rows_contiguous(x2):
-        x2 = x2.contiguous()
-    if not rows_contiguous(w):
-        w = w.contiguous()
+    M, ldx, ldw = len(x2), x2.stride()[0], w.stride()[0]
+    if not rows_contiguous(x2) or (ldx < K and M > 1):  # (rows that share memory: expanded)
+        x2, ldx = x2.contiguous(), K
+    if not rows_contiguous(w) or (ldw < K and N > 1):
+        w, ldw = w.contiguous(), K
+    if M <= 1:
+        ldx = K  # the stride of a single row says nothing
+    if N <= 1:
+        ldw = K
     if not rows_contiguous(ids):
         ids = ids.contiguous()
     if not lora_a.is_contiguous():
@@ -96,7 +104,7 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         if not bias.is_contiguous():
             bias = bias.contiguous()
         bias_ptr = bias.data_ptr()
-    M, dev = len(x2), x.device
+    dev, ldy = x.device, N
     if out is None:
         y = torch.empty(M, N, dtype=dtype, device=dev)
     else:
@@ -105,19 +113,21 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         y = out if out.dim() == 2 else out.view(M, N)
         if not rows_contiguous(y):
             raise ValueError("lora_linear: out rows must be contiguous")
+        if M > 1:
+            ldy = y.stride()[0]
+            if ldy < N:
+                raise ValueError("lora_linear: out rows must not share memory")
     x_ptr, w_ptr, y_ptr = x2.data_ptr(), w.data_ptr(), y.data_ptr()
     a_ptr, b_ptr = lora_a.data_ptr(), lora_b.data_ptr()
-    ldx, ldw, ldy = x2.stride()[0], w.stride()[0], y.stride()[0]
     block = _pack(L.dtype_code(dtype), n, rank, M, K, N, x_ptr, ldx, w_ptr, ldw, a_ptr, b_ptr,
                   ids.data_ptr(), scaling_ptr, bias_ptr, y_ptr, ldy)
     lib = L.load()
-    with L.on_device(dev):
-        # everything the size depends on, alignment included
-        key = ("lora", d, dtype, M, K, N, rank, n, (ldx | ldw | ldy) & 7, ldy & 7,
-               (x_ptr | w_ptr | a_ptr | b_ptr) & 15, y_ptr & 15)
-        nb = L.workspace_bytes(lib.ck_lora_workspace_bytes, key, block)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        rc = lib.ck_lora_linear(block, ws.data_ptr() if nb else 0, nb, L.stream_of(dev))
+    # everything the size depends on, alignment included
+    key = ("lora", d, dtype, M, K, N, rank, n, (ldx | ldw) & 7, ldy & 7,
+           (x_ptr | w_ptr | a_ptr | b_ptr) & 15, y_ptr & 15)
+    nb = L.workspace_bytes(lib.ck_lora_workspace_bytes, key, block)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    rc = lib.ck_lora_linear(block, ws.data_ptr() if nb else 0, nb, L.raw_stream(d))
     if rc != L.CK_OK:
         L.check(rc, "ck_lora_linear")
     if out is not None:

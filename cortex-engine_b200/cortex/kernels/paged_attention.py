@@ -76,6 +76,10 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
             out is not None or weights_out is not None:
         L.require_cuda(q, pool, page_table, lengths, weights, out, weights_out,
                        what="paged_attention")
+    if d != L.current_device():
+        with torch.cuda.device(d):
+            return paged_attention(q, pool, page_table, lengths, scale=scale, weights=weights,
+                                   out=out, weights_out=weights_out)
     check_pages("paged_attention", pool, page_table, lengths)
     dtype = q.dtype
     if dtype is not pool.dtype:
@@ -120,18 +124,25 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
     qb, qh, _ = q.stride()
     pb, pr, _ = pool.stride()
     ob, oh, _ = out.stride()
+    if B == 1:  # the stride of a single row says nothing
+        qb = 0
+    if H == 1:
+        qh = 0
+    if pages == 1:
+        pb = 0
+    if page_size == 1:
+        pr = 0
     q_ptr, pool_ptr = q.data_ptr(), pool.data_ptr()
     block = _pack(L.dtype_code(dtype), B, H, Hkv, Dh, q_ptr, qb, qh, pool_ptr, pages, pb, pr, page_size, table_width, page_table.data_ptr(), page_table.stride()[0],
                   lengths.data_ptr(), out.data_ptr(), ob, oh, w_in, w_out, w_in_ld, w_out_ld, W,
                   Dh ** -0.5 if scale is None else scale)
     lib = L.load()
-    with L.on_device(dev):
-        # everything the size depends on, alignment included
-        key = (d, dtype, B, H, Hkv, Dh, page_size, table_width, W, (pb | pr | qb | qh) & 7,
-               (q_ptr | pool_ptr) & 15)
-        n = L.workspace_bytes(lib.ck_paged_attention_workspace_bytes, key, block)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        rc = lib.ck_paged_attention(block, ws.data_ptr() if n else 0, n, L.stream_of(dev))
+    # everything the size depends on, alignment included
+    key = ("attention", d, dtype, B, H, Hkv, Dh, page_size, table_width, W, (pb | pr | qb | qh) & 7,
+           (q_ptr | pool_ptr) & 15)
+    n = L.workspace_bytes(lib.ck_paged_attention_workspace_bytes, key, block)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    rc = lib.ck_paged_attention(block, ws.data_ptr() if n else 0, n, L.raw_stream(d))
     if rc != L.CK_OK:
         L.check(rc, "ck_paged_attention")
     return out if weights is None else (out, weights_out)

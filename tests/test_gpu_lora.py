@@ -254,3 +254,20 @@ def test_refusals():
     with pytest.raises(NotImplementedError):
         lora_linear(x, w, torch.zeros(3, 300, 64, dtype=BF, device=DEV),
                     torch.zeros(3, 32, 300, dtype=BF, device=DEV), ids)
+
+
+@pytest.mark.parametrize("M", [1, 6, 200])
+def test_expanded_and_single_rows(M):
+    """Rows that share memory, and size-one dimensions whose strides are arbitrary."""
+    x, w, a, b, ids, s, bias = make(M, 512, 264, 16, 5, BF)
+    row = x[:1].expand(M, 512)
+    check(lora_linear(row, w, a, b, ids, scaling=s, bias=bias), (row, w, a, b, ids, s, bias))
+    odd = torch.as_strided(x, (1, 512), (3, 1))
+    state = (odd, w, a, b, ids[:1], s, bias)
+    check(lora_linear(odd, w, a, b, ids[:1], scaling=s, bias=bias), state)
+    w1 = torch.as_strided(w, (1, 512), (5, 1))
+    b1 = b[:, :1].contiguous()
+    check(lora_linear(x, w1, a, b1, ids, scaling=s, bias=bias[:1]), (x, w1, a, b1, ids, s, bias[:1]))
+    if M > 1:
+        with pytest.raises(ValueError):
+            lora_linear(x, w, a, b, ids, out=torch.empty(264, dtype=BF, device=DEV).expand(M, 264))
