@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
   __shared__ uint32_t s_hist[4][256];
   __shared__ uint32_t s_sum[256];
   __shared__ int32_t s_max;
-  __shared__ uint32_t s_pick[4][2];
+  __shared__ uint32_t s_pick[4][3];  // digit, rank among its keys, its keys
   __shared__ int4 s_cnt[SW];       // per warp: front keys equal, greater; back equal, greater
   __shared__ int4 s_all[WARPS];    // the same of the whole cluster
   __shared__ int32_t s_list[2][CS == 1 ? kFewMoves : 1];  // holes, movers that one CTA moves itself
@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
 
   // radix selection of the budget-th largest key
   uint32_t prefix = 0u;
+  bool found = false;
   uint32_t want = (uint32_t)budget;  // rank of the wanted key among those under the prefix
 #pragma unroll 1
   for (int pass = 0; pass < 4; ++pass) {
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
         if (lane >= o) before += v;
       }
       before -= tot;
-      uint32_t digit = 0u, left = 0u;
+      uint32_t digit = 0u, left = 0u, keys = 0u;
       const bool here = before < want && want <= before + tot;
       if (here) {
         uint32_t acc = before;
@@ -283,6 +284,7 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
           if (acc < want && want <= acc + own[i]) {
             digit = (uint32_t)(255 - 8 * lane - i);
             left = want - acc;
+            keys = own[i];
           }
           acc += own[i];
         }
@@ -290,20 +292,31 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
       const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
       digit = __shfl_sync(0xffffffffu, digit, src);
       left = __shfl_sync(0xffffffffu, left, src);
+      keys = __shfl_sync(0xffffffffu, keys, src);
       if (CS > 1) {
         if (lane == 0) {
           s_pick[pass][0] = digit;
           s_pick[pass][1] = left;
+          s_pick[pass][2] = keys;
         }
       } else {
         prefix |= digit << shift;
         want = left;
+        found = left == keys;
       }
     }
     if (CS > 1) {
       __syncthreads();
       prefix |= s_pick[pass][0] << shift;
       want = s_pick[pass][1];
+      found = want == s_pick[pass][2];
+    }
+    if (found && pass < 3) {
+      // every key under this prefix is kept (with weights all different, mostly
+      // one key after three digits): the keys above prefix - 1
+      prefix -= 1u;  // (not 0: that would keep all n > budget rows)
+      want = 0u;
+      break;
     }
   }
   // kept: key > prefix, and the first `want` slots whose key equals it
