@@ -28,6 +28,9 @@ namespace {
 constexpr int ST = 512;          // threads of a selecting CTA
 constexpr int SW = ST / 32;
 constexpr int kKeyCap = 49152;   // slots whose key a CTA keeps in shared memory
+constexpr int kBulkRoom = 24576; // shared memory of a warp that moves rows by bulk copies
+constexpr int kBulkRow = 8192;   // bytes of the longest row moved that way
+constexpr int kListed = 1024;    // sequences that the moving kernel lists at a time
 constexpr int kFewMoves = 128;   // rows that the selecting kernel moves itself
 constexpr uint32_t kProtected = 0xFFFFFFFFu;
 
@@ -39,7 +42,7 @@ struct EvictParams {
   int32_t* holes;     // [B][max_moves]
   int32_t* movers;    // [B][max_moves]
   int32_t key_cap;    // slots per CTA that shared memory holds
-  int32_t move_blocks;  // move_kernel: blocks per sequence; 0: select_kernel moves the rows
+  int32_t move_blocks;  // move_kernel: blocks; 0: select_kernel moves the rows
   int32_t vec_bytes;    // bytes that a lane copies at a time
 };
 
@@ -56,16 +59,11 @@ __device__ __forceinline__ uint32_t cl_ld(uint32_t addr) {
   return v;
 }
 
-// Rows of the movers into the holes, their weights and positions with them:
-// moves [32 k, 32 k + 32) of sequence b for k = w, w + workers, ... by a warp.
-// The lanes look up a move each, then the warp copies row after row, 8 vectors
-// a lane in flight.
-template <typename V>
-__device__ __forceinline__ void move_rows(const EvictParams& p, int b, const int32_t* holes,
-                                          const int32_t* movers, int total, int w, int workers) {
+// One move of sequence b: the weight and position at once, and the byte offsets
+// of its rows in the pool (-1 for a page outside it, which is recorded).
+__device__ __forceinline__ void start_move(const EvictParams& p, int b, int hole, int mover,
+                                           int64_t& from, int64_t& to) {
   const ck_evict_args& a = p.a;
-  const int lane = threadIdx.x & 31;
-  const int64_t vecs = (int64_t)a.width * a.elem_bytes / (int64_t)sizeof(V);
   const int32_t* table = a.page_table + (int64_t)b * a.page_table_ld;
   auto row_of = [&](int j) -> int64_t {
     const int slot = j / a.page_size;
@@ -76,34 +74,47 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, const int
     }
     return ((int64_t)page * a.page_ld + (int64_t)(j - slot * a.page_size) * a.row_ld) * a.elem_bytes;
   };
-  // few moves: fewer than 32 to a warp, so that every warp has some
+  to = row_of(hole);
+  from = row_of(mover);
+  a.w_out[(int64_t)b * a.w_out_ld + hole] = a.w_in[(int64_t)b * a.w_in_ld + mover];
+  a.pos_out[(int64_t)b * a.pos_out_ld + hole] = a.pos_in[(int64_t)b * a.pos_in_ld + mover];
+}
+
+// The rows of the lanes' moves (cnt of them), one after the other by the whole
+// warp, 8 vectors a lane in flight.
+template <typename V>
+__device__ __forceinline__ void copy_rows_of(const EvictParams& p, int cnt, int64_t from, int64_t to) {
+  const int lane = threadIdx.x & 31;
+  const int64_t vecs = (int64_t)p.a.width * p.a.elem_bytes / (int64_t)sizeof(V);
+  uint8_t* pool = reinterpret_cast<uint8_t*>(p.a.pool);
+  for (int k = 0; k < cnt; ++k) {
+    const int64_t f = __shfl_sync(0xffffffffu, from, k), t = __shfl_sync(0xffffffffu, to, k);
+    if (f < 0 || t < 0) continue;
+    const V* src = reinterpret_cast<const V*>(pool + f);
+    V* dst = reinterpret_cast<V*>(pool + t);
+    for (int64_t c = lane; c < vecs; c += 8 * 32) {
+      V v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (c + 32 * u < vecs) v[u] = src[c + 32 * u];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (c + 32 * u < vecs) dst[c + 32 * u] = v[u];
+    }
+  }
+}
+
+// Moves w, w + workers, ... of one sequence, a lane each, then their rows.
+template <typename V>
+__device__ __forceinline__ void move_rows(const EvictParams& p, int b, const int32_t* holes,
+                                          const int32_t* movers, int total, int w, int workers) {
+  const int lane = threadIdx.x & 31;
   const int per = max(1, min(32, (total + workers - 1) / workers));
-  uint8_t* pool = reinterpret_cast<uint8_t*>(a.pool);
   for (int64_t i0 = (int64_t)w * per; i0 < total; i0 += (int64_t)workers * per) {
     const int cnt = (int)min((int64_t)per, total - i0);
     int64_t from = -1, to = -1;
-    if (lane < cnt) {
-      const int hole = holes[i0 + lane], mover = movers[i0 + lane];
-      to = row_of(hole);
-      from = row_of(mover);
-      a.w_out[(int64_t)b * a.w_out_ld + hole] = a.w_in[(int64_t)b * a.w_in_ld + mover];
-      a.pos_out[(int64_t)b * a.pos_out_ld + hole] = a.pos_in[(int64_t)b * a.pos_in_ld + mover];
-    }
-    for (int k = 0; k < cnt; ++k) {
-      const int64_t f = __shfl_sync(0xffffffffu, from, k), t = __shfl_sync(0xffffffffu, to, k);
-      if (f < 0 || t < 0) continue;
-      const V* src = reinterpret_cast<const V*>(pool + f);
-      V* dst = reinterpret_cast<V*>(pool + t);
-      for (int64_t c = lane; c < vecs; c += 8 * 32) {
-        V v[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (c + 32 * u < vecs) v[u] = src[c + 32 * u];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (c + 32 * u < vecs) dst[c + 32 * u] = v[u];
-      }
-    }
+    if (lane < cnt) start_move(p, b, holes[i0 + lane], movers[i0 + lane], from, to);
+    copy_rows_of<V>(p, cnt, from, to);
   }
 }
 
@@ -416,14 +427,108 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
   }
 }
 
-template <typename V>
-__global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
+// The same through shared memory by bulk copies, a row a lane: `room` bytes of it
+// are the warp's, for at most `slots` rows at a time.
+__device__ __forceinline__ void copy_rows_bulk(const EvictParams& p, int cnt, int64_t from, int64_t to,
+                                               uint32_t room, uint64_t* bar, uint32_t& phase) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t row = (uint32_t)(p.a.width * p.a.elem_bytes);
+  uint8_t* pool = reinterpret_cast<uint8_t*>(p.a.pool);
+  const bool mine = lane < cnt && from >= 0 && to >= 0;
+  const uint32_t rows = __popc(__ballot_sync(0xffffffffu, mine));
+  if (rows == 0u) return;
+  if (lane == 0) mbar_arrive_expect_tx(bar, rows * row);
+  __syncwarp();
+  const uint32_t at = room + lane * row;
+  if (mine)
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at),
+        "l"(pool + from), "r"(row), "r"(smem_u32(bar))
+        : "memory");
+  const bool ok = mbar_wait_park(bar, phase, nullptr, 40);
+  phase ^= 1u;
+  if (mine && ok) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(pool + to),
+                 "r"(at), "r"(row)
+                 : "memory");
+    bulk_commit();
+    bulk_wait_read<0>();  // before the next rows come into this place
+  }
+  __syncwarp();
+}
+
+// Every sequence's moves as one list, an equal share of it to every warp: a
+// batch has sequences with thousands of moves beside sequences with none. The
+// blocks are one round of what the SMs hold. BULK (rows of a multiple of 16
+// bytes, aligned, at most kBulkRow): rows go through shared memory by bulk
+// copies, a lane issuing a row's, which keeps 192 KB an SM in flight; else
+// through registers, V at a time.
+template <typename V, bool BULK>
+__global__ void __launch_bounds__(BULK ? 128 : 256) evict_move_kernel(const EvictParams p) {
+  constexpr int NW = BULK ? 4 : 8;
+  __shared__ int64_t s_end[kListed];  // moves up to and with each sequence
+  __shared__ int64_t s_warp[NW];
+  __shared__ __align__(8) uint64_t s_bar[NW];
+  extern __shared__ __align__(128) uint8_t s_rows[];  // BULK: [NW][kBulkRoom]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (BULK && tid < NW) {
+    mbar_init(&s_bar[tid], 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
   grid_dep_wait();
   grid_dep_launch();
-  const int b = blockIdx.x / p.move_blocks;
-  move_rows<V>(p, b, p.holes + (int64_t)b * p.max_moves, p.movers + (int64_t)b * p.max_moves,
-               p.counts[b], (int)(blockIdx.x - b * p.move_blocks) * 8 + (threadIdx.x >> 5),
-               p.move_blocks * 8);
+  uint32_t phase = 0;
+  const int slots = BULK ? (int)min((int64_t)32, (int64_t)kBulkRoom / (p.a.width * p.a.elem_bytes)) : 32;
+  for (int b0 = 0; b0 < p.a.B; b0 += kListed) {
+    const int n = min(kListed, p.a.B - b0);
+    // sums over the sequences: neighbouring ones a thread
+    constexpr int PER = kListed / (32 * NW);
+    int64_t own[PER], run = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = tid * PER + i;
+      run += k < n ? p.counts[b0 + k] : 0;
+      own[i] = run;
+    }
+    int64_t before = run;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
+    }
+    __syncthreads();  // (the sums of the sequences before these have been read; the barriers are set)
+    if (lane == 31) s_warp[warp] = before;
+    __syncthreads();
+    before -= run;
+    for (int v = 0; v < warp; ++v) before += s_warp[v];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (tid * PER + i < n) s_end[tid * PER + i] = before + own[i];
+    __syncthreads();
+    const int64_t total = s_end[n - 1];
+    const int64_t workers = (int64_t)gridDim.x * NW, w = (int64_t)blockIdx.x * NW + warp;
+    const int per = (int)max((int64_t)1, min((int64_t)slots, (total + workers - 1) / workers));
+    for (int64_t i0 = w * per; i0 < total; i0 += workers * per) {
+      const int cnt = (int)min((int64_t)per, total - i0);
+      int64_t from = -1, to = -1;
+      if (lane < cnt) {
+        int lo = 0, hi = n - 1;  // the first sequence that ends behind this move
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (s_end[mid] > i0 + lane) hi = mid; else lo = mid + 1;
+        }
+        const int64_t k = i0 + lane - (lo > 0 ? s_end[lo - 1] : 0);
+        const int64_t at = (int64_t)(b0 + lo) * p.max_moves + k;
+        start_move(p, b0 + lo, p.holes[at], p.movers[at], from, to);
+      }
+      if constexpr (BULK)
+        copy_rows_bulk(p, cnt, from, to, smem_u32(s_rows) + warp * kBulkRoom, &s_bar[warp], phase);
+      else
+        copy_rows_of<V>(p, cnt, from, to);
+    }
+  }
+  if (BULK) bulk_wait<0>();  // this lane's stores are done
 }
 
 struct EvictPlan {
@@ -511,22 +616,26 @@ int evict_by_weight(const ck_evict_args& a, void* ws, size_t ws_bytes, cudaStrea
                          (uintptr_t)(a.row_ld * a.elem_bytes) |
                          (uintptr_t)((int64_t)a.width * a.elem_bytes);
   p.vec_bytes = bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : 2);
-  // Blocks for the longest possible list, and no more than fill the card. A
-  // list of at most kFewMoves rows (sessions that stay at their budget) is
-  // moved by the selecting kernel, without a second launch.
-  const int64_t need = (p.max_moves + 7) / 8;
-  int64_t fill = (8 * (int64_t)num_sms() + a.B - 1) / a.B;
-  if (fill < 1) fill = 1;
+  // One round of blocks (two or three an SM), or fewer where the lists cannot be that
+  // long. A list of at most kFewMoves rows (sessions that stay at their budget)
+  // is moved by the selecting kernel, without a second launch.
+  const bool bulk = p.vec_bytes == 16 && (int64_t)a.width * a.elem_bytes <= kBulkRow;
+  const int64_t need = ((int64_t)a.B * p.max_moves + 3) / 4, fill = (bulk ? 2 : 3) * (int64_t)num_sms();
   p.move_blocks = p.max_moves <= kFewMoves ? 0 : (int32_t)(need < fill ? need : fill);
   rc = pl.cs == 1   ? launch_select<1>(p, st)
        : pl.cs == 4 ? launch_select<4>(p, st)
        : pl.cs == 8 ? launch_select<8>(p, st)
                     : launch_select<16>(p, st);
   if (rc != CK_OK || p.move_blocks == 0) return rc;
-  const dim3 grid((unsigned)((int64_t)a.B * p.move_blocks));
-  if (p.vec_bytes == 16) return launch_pdl(evict_move_kernel<uint4>, grid, dim3(256), 0, st, p);
-  if (p.vec_bytes == 4) return launch_pdl(evict_move_kernel<uint32_t>, grid, dim3(256), 0, st, p);
-  return launch_pdl(evict_move_kernel<uint16_t>, grid, dim3(256), 0, st, p);
+  const dim3 grid((unsigned)p.move_blocks);
+  if (bulk) {
+    auto kern = evict_move_kernel<uint4, true>;
+    if (!smem_attr_ready(reinterpret_cast<const void*>(kern), 4 * kBulkRoom)) return record_cuda_error();
+    return launch_pdl(kern, grid, dim3(128), 4 * kBulkRoom, st, p);
+  }
+  if (p.vec_bytes == 16) return launch_pdl(evict_move_kernel<uint4, false>, grid, dim3(256), 0, st, p);
+  if (p.vec_bytes == 4) return launch_pdl(evict_move_kernel<uint32_t, false>, grid, dim3(256), 0, st, p);
+  return launch_pdl(evict_move_kernel<uint16_t, false>, grid, dim3(256), 0, st, p);
 }
 
 }  // namespace ck

@@ -935,7 +935,7 @@ __device__ __forceinline__ int2 unit_of(const PagedParams& p, int h) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(JT) join_kernel(const PagedParams p, int out_blocks,
+__global__ void __launch_bounds__(JT, 6) join_kernel(const PagedParams p, int out_blocks,
                                                   int w_blocks, int chunked) {
   __shared__ float s_f[kMaxParts];
   __shared__ float s_red[JT];
