@@ -18,6 +18,8 @@
 // weights and positions, a warp a row.
 //
 // Bytes: weights and positions once (8 B a slot), 2 row reads / writes a mover.
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -159,13 +161,13 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
   const int kept_n = min(n, budget);
 
   // tables of the rows that stay where they are (move_kernel overwrites the
-  // holes'), and with fill the columns behind them
+  // holes'), and with fill the columns behind them (out_width may be INT32_MAX)
   auto copy_tables = [&]() {
     const int end = a.fill ? a.out_width : kept_n;
     if (a.w_out != a.w_in)
-      for (int j = rank * ST + tid; j < end; j += CS * ST) w_out[j] = j < kept_n ? w_in[j] : 0.f;
+      for (int64_t j = rank * ST + tid; j < end; j += CS * ST) w_out[j] = j < kept_n ? w_in[j] : 0.f;
     if (a.pos_out != a.pos_in)
-      for (int j = rank * ST + tid; j < end; j += CS * ST) pos_out[j] = j < kept_n ? pos_in[j] : -1;
+      for (int64_t j = rank * ST + tid; j < end; j += CS * ST) pos_out[j] = j < kept_n ? pos_in[j] : -1;
   };
   if (n <= budget) {  // (the whole cluster: n is the sequence's)
     copy_tables();
@@ -573,9 +575,17 @@ template <int CS>
 int launch_select(const EvictParams& p, cudaStream_t st) {
   auto kern = evict_select_kernel<CS>;
   if (!smem_attr_ready(reinterpret_cast<const void*>(kern), kKeyCap * 4)) return record_cuda_error();
-  if (CS > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
-                    cudaSuccess)
-    return record_cuda_error();
+  if (CS > 8) {  // more than the portable 8 CTAs: allowed once per device
+    static std::atomic<uint64_t> allowed{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return record_cuda_error();
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if ((allowed.load(std::memory_order_relaxed) & bit) == 0) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return record_cuda_error();
+      allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = CS;
