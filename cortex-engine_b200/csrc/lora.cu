@@ -589,6 +589,11 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
           tma_load_2d(sA + (s * C::SL + i) * C::A_BYTES, &tmA, &full[s], kb * 64,
                       s_list[slot0 + i] * a.rank + j0);
       }
+      if (*abort_flag != 0)  // a wait ran out: no copy may land after this CTA's exit
+        for (int s = 0; s < C::STAGES && s < it; ++s) {
+          const int last = it - 1 - ((it - 1 - s) % C::STAGES);
+          mbar_wait(&full[s], (uint32_t)((last / C::STAGES) & 1), nullptr, 33);
+        }
     } else if (warp == 1 && lane == 0) {
       constexpr uint32_t idesc = idesc_bf16(128, RP, 0u);
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
@@ -915,15 +920,30 @@ struct LoraPlan {
 
 bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 
-// Rows up to which lora_rows_kernel runs (tensor-core tiles above).
-constexpr int64_t kRowsMax = 64;
+// Whether lora_rows_kernel runs: its epilogue reads h and B_i once a row, where
+// the tiles multiply B_i once for all rows that name it but take a block for each
+// adapter of a tile. Measured (us, rows against tiles; adapters all different /
+// in runs of 64 rows): 4 x 512 x 1536, rank 32, 12.3 / 12.3 against 16.4 / 14.3;
+// 32 x 768 x 2304, rank 64, 22.5 / 20.5 against 28.7 / 16.4; 64 x 768 x 2304,
+// rank 32, 22.5 / 20.5 against 49.2 / 16.4, rank 64, 30.7 / 30.7 against 28.7 / 18.4.
+// More rows than one operand of 64, only while all of them are few CTAs: 128 x
+// 512 x 1536 (24 tiles of W by rows), rank 8, 16.4 / 16.4 against 26.6 / 18.4; 256
+// x 4096 x 1024 (32), rank 32, 32.8 / 30.8 against 75.8 / 34.8; 192 x 512 x 1536
+// (36), 8 adapters of rank 16, 26.6 against 22.5. 512 x 512 x 512, rank 32, 28.7 /
+// 28.7 against 55.3 / 20.4: more than 8192 values of h are left to the tiles.
+bool by_rows(const ck_lora_args& a) {
+  if (a.M <= 32) return true;
+  if (a.rank > 32) return false;
+  return a.M <= 64 || ((a.M + 63) / 64 * ((a.N + 127) / 128) <= 32 && a.M * a.rank <= 8192);
+}
 
 int make_plan(const ck_lora_args& a, LoraPlan& pl) {
   if (a.dtype != CK_F32 && a.dtype != CK_BF16) return CK_ERR_UNSUPPORTED;
   if (a.M < 0 || a.N < 0 || a.K <= 0 || a.rank < 1 || a.n_adapters < 0) return CK_ERR_INVALID_ARG;
-  if (a.M > INT32_MAX || a.N > INT32_MAX || a.K > INT32_MAX) return CK_ERR_UNSUPPORTED;
-  if (a.rank > 256) return CK_ERR_UNSUPPORTED;
-  if (a.M > (int64_t)1 << 28 || ((a.M + 31) / 32) * ((a.N + 63) / 64) > INT32_MAX || (a.M * a.rank + 7) / 8 > INT32_MAX)
+  // (indexes inside a tile that reaches past the end stay below 2^31)
+  if (a.M > (int64_t)1 << 28 || a.N > INT32_MAX - 256 || a.K > INT32_MAX - 256 || a.rank > 256)
+    return CK_ERR_UNSUPPORTED;
+  if (((a.M + 31) / 32) * ((a.N + 63) / 64) > INT32_MAX || (a.M * a.rank + 7) / 8 > INT32_MAX)
     return CK_ERR_UNSUPPORTED;
   pl.p.a = a;
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
@@ -931,7 +951,7 @@ int make_plan(const ck_lora_args& a, LoraPlan& pl) {
                    aligned16(a.x) && aligned16(a.w) && aligned16(a.a) && aligned16(a.b) &&
                    (int64_t)a.n_adapters * a.N <= INT32_MAX - 256 &&
                    (int64_t)a.n_adapters * a.rank <= INT32_MAX - 256;
-  pl.path = a.dtype == CK_F32 ? PATH_F32 : !tma ? PATH_SIMT : (a.M <= kRowsMax ? PATH_ROWS : PATH_TILES);
+  pl.path = a.dtype == CK_F32 ? PATH_F32 : !tma ? PATH_SIMT : by_rows(a) ? PATH_ROWS : PATH_TILES;
   if (pl.path != PATH_TILES) {
     pl.bytes = up((size_t)a.M * a.rank * 4);
     return CK_OK;
@@ -1148,8 +1168,7 @@ int lora_linear(const ck_lora_args& a, void* ws, size_t ws_bytes, cudaStream_t s
     if (rc != CK_OK) return rc;
     if (a.M <= 16) return launch_rows_k<16>(pl.p, st);
     if (a.M <= 32) return launch_rows_k<32>(pl.p, st);
-    if (a.M <= 64) return launch_rows_k<64>(pl.p, st);
-    return launch_rows_k<128>(pl.p, st);
+    return launch_rows_k<64>(pl.p, st);
   }
   if (pl.path == PATH_F32) {
     rc = shrink<float>(pl.p, 0, st);
