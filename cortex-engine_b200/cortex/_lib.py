@@ -233,6 +233,32 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+def memory_range(t: torch.Tensor) -> tuple[int, int]:
+    """[first, last) byte address that ``t``'s elements lie in."""
+    p = t.data_ptr()
+    if t.numel() == 0:
+        return p, p
+    span = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return p, p + (span + 1) * t.element_size()
+
+
+def check_output(what: str, name: str, out: torch.Tensor, *inputs: torch.Tensor | None) -> None:
+    """An output that a caller provides: its elements must not share memory with
+    each other or lie within the span of an input."""
+    dims = sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1)
+    reach = 0
+    for s, n in dims:
+        if s <= reach:
+            raise ValueError(f"{what}: elements of {name} share memory")
+        reach += s * (n - 1)
+    lo, hi = memory_range(out)
+    for t in inputs:
+        if t is not None:
+            a, b = memory_range(t)
+            if a < hi and lo < b:
+                raise ValueError(f"{what}: {name} overlaps an input")
+
+
 class DeviceStatusError(RuntimeError):
     pass
 

@@ -52,7 +52,7 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
         recent: rows whose position is among the newest ``recent`` (position >
             newest - recent) are kept before all others; 0 <= recent <= budget.
         out: optional (lengths, weights, positions) to write to, each of which may be
-            the input itself (in place; otherwise they must not overlap); slots
+            the input itself (in place) and is apart from all other inputs; slots
             behind the new lengths are left as they were. Without it new tensors:
             weights and positions (B, budget), 0 and -1 behind the new lengths.
 
@@ -103,14 +103,23 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
         new_w_ld, new_cols = _table("out weights", new_w, torch.float32, B, min(budget, cap))
         new_pos_ld, n = _table("out positions", new_pos, torch.int32, B, min(budget, cap))
         new_cols = min(new_cols, n)
+        for name, given, own in (("out lengths", new_len, lengths), ("out weights", new_w, weights),
+                                 ("out positions", new_pos, positions)):
+            L.check_output("evict_by_weight", name, given, pool, page_table,
+                           *(t for t in (lengths, weights, positions)
+                             if t is not own or given is not own))
+        L.check_output("evict_by_weight", "out positions", new_pos, new_w, new_len)
+        L.check_output("evict_by_weight", "out weights", new_w, new_len)
     if not rows_contiguous(page_table):
         page_table = page_table.contiguous()
     page_ld, row_ld, _ = pool.stride()
+    if row_ld < width or page_ld < page_size * row_ld:
+        L.check_output("evict_by_weight", "pool", pool)
     block = _pack(pool.element_size(), B, pool.data_ptr(), pages, page_ld, row_ld, page_size, width,
                   page_table.data_ptr(), page_table.stride()[0], table_width, budget, recent, fill,
                   lengths.data_ptr(), new_len.data_ptr(), weights.data_ptr(), new_w.data_ptr(),
                   positions.data_ptr(), new_pos.data_ptr(), w_ld, new_w_ld, pos_ld, new_pos_ld,
-                  min(w_cols, pos_cols), new_cols)
+                  min(w_cols, pos_cols, 2 ** 31 - 1), min(new_cols, 2 ** 31 - 1))
     lib = L.load()
     n = L.workspace_bytes(lib.ck_evict_workspace_bytes, ("evict", d, B, cap, budget), block)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None

@@ -40,7 +40,7 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
             row without an adapter.
         scaling: optional (n,) float32 factor of each adapter's part.
         bias: optional (N,), x's dtype.
-        out: optional output, (..., N); it must not overlap an input.
+        out: optional output, (..., N), outside the memory that the inputs span.
 
     Sums are fp32 and the result is rounded once. An id >= n is recorded in the
     device status (IndexError from ``_lib.check_device_status``) and its row gets
@@ -113,10 +113,9 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         y = out if out.dim() == 2 else out.view(M, N)
         if not rows_contiguous(y):
             raise ValueError("lora_linear: out rows must be contiguous")
+        L.check_output("lora_linear", "out", y, x, w, lora_a, lora_b, adapter_ids, scaling, bias)
         if M > 1:
             ldy = y.stride()[0]
-            if ldy < N:
-                raise ValueError("lora_linear: out rows must not share memory")
     x_ptr, w_ptr, y_ptr = x2.data_ptr(), w.data_ptr(), y.data_ptr()
     a_ptr, b_ptr = lora_a.data_ptr(), lora_b.data_ptr()
     block = _pack(L.dtype_code(dtype), n, rank, M, K, N, x_ptr, ldx, w_ptr, ldw, a_ptr, b_ptr,

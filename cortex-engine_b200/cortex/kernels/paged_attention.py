@@ -51,7 +51,7 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
     """softmax(scale q k^T) v of one query token per sequence.
 
     Args:
-        q: (B, H, Dh) queries, the pool's dtype; Dh <= 256.
+        q: (B, H, Dh) queries, the pool's dtype; Dh <= 256, H <= 4096.
         pool: (num_pages, page_size, 2 * Hkv * Dh) rows of K of every head, then V
             of every head; H must be a multiple of Hkv (grouped queries).
         page_table: (B, pages) int32; position j of sequence b is row
@@ -63,8 +63,10 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
             each position has received so far. The call then returns
             (out, weights_out) with weights_out[b, j] = weights[b, j] + the sum over
             heads of position j's probability (what ``evict_by_weight`` reads).
-        out, weights_out: optional outputs; ``weights_out`` may be ``weights``
-            itself (in place), otherwise the two must not overlap.
+        out, weights_out: optional outputs, outside the memory that the inputs
+            span; only ``weights_out`` may be ``weights`` itself (in place).
+
+    With weights the workspace holds every score, 4 bytes a head and slot.
 
     A page outside the pool (its rows count as absent) or a length outside
     [0, pages * page_size] (clamped) is recorded in the device status
@@ -105,6 +107,9 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
         out = torch.empty(B, H, Dh, dtype=dtype, device=dev)
     elif out.shape != q.shape or out.dtype != dtype or not rows_contiguous(out):
         raise ValueError("paged_attention: out must be like q with contiguous heads")
+    else:
+        L.check_output("paged_attention", "out", out, q, pool, page_table, lengths, weights,
+                       weights_out)
     table_width = page_table.shape[1]
     W = w_in = w_out = w_in_ld = w_out_ld = 0
     if weights is not None:
@@ -115,6 +120,11 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
             weights_out = torch.empty(weights.shape, dtype=torch.float32, device=dev)
         elif weights_out.shape != weights.shape or weights_out.dtype != torch.float32:
             raise ValueError("paged_attention: weights_out must be like weights")
+        elif weights_out is weights:
+            L.check_output("paged_attention", "weights_out", weights_out, q, pool, page_table, lengths)
+        else:
+            L.check_output("paged_attention", "weights_out", weights_out, q, pool, page_table,
+                           lengths, weights)
         if not rows_contiguous(weights) or not rows_contiguous(weights_out):
             raise ValueError("paged_attention: weights rows must be contiguous")
         W, w_in, w_out = weights.shape[1], weights.data_ptr(), weights_out.data_ptr()
@@ -133,7 +143,8 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
     if page_size == 1:
         pr = 0
     q_ptr, pool_ptr = q.data_ptr(), pool.data_ptr()
-    block = _pack(L.dtype_code(dtype), B, H, Hkv, Dh, q_ptr, qb, qh, pool_ptr, pages, pb, pr, page_size, table_width, page_table.data_ptr(), page_table.stride()[0],
+    block = _pack(L.dtype_code(dtype), B, H, Hkv, Dh, q_ptr, qb, qh, pool_ptr, pages, pb, pr,
+                  page_size, table_width, page_table.data_ptr(), page_table.stride()[0],
                   lengths.data_ptr(), out.data_ptr(), ob, oh, w_in, w_out, w_in_ld, w_out_ld, W,
                   Dh ** -0.5 if scale is None else scale)
     lib = L.load()

@@ -233,3 +233,48 @@ def test_refusals():
         evict_by_weight(pool.cpu(), table, lengths, w, pos, **ok)
     empty = evict_by_weight(pool, table[:0], lengths[:0], w[:0], pos[:0], **ok)
     assert empty[0].shape == (0,) and empty[1].shape == (0, 10)
+
+
+def test_outputs_apart_from_inputs():
+    pool, table, lengths, w, pos = make([30, 30], 16, 8, torch.float32)
+    ok = dict(budget=10, recent=2)
+    fresh = lambda: (lengths.clone(), w.clone(), pos.clone())  # noqa: E731
+    for i, bad in ((0, torch.zeros(1, dtype=torch.int32, device=DEV).expand(2)),
+                   (1, w[:, 1:12]), (1, pos.view(torch.float32)), (2, w.view(torch.int32)),
+                   (1, torch.zeros(1, 10, device=DEV).expand(2, 10))):
+        out = list(fresh())
+        out[i] = bad
+        with pytest.raises(ValueError):
+            evict_by_weight(pool, table, lengths, w, pos, out=tuple(out), **ok)
+    n1, w1, p1 = fresh()
+    with pytest.raises(ValueError):
+        evict_by_weight(pool, table, lengths, w, pos, out=(n1, p1.view(torch.float32), p1), **ok)
+    with pytest.raises(ValueError):
+        evict_by_weight(pool[:1].expand(4, 16, 8), table, lengths, w, pos, **ok)
+    state = make([30, 30], 16, 8, torch.float32)
+    assert same(pool, state[0])
+
+
+@pytest.mark.parametrize("dtype,width", [(torch.bfloat16, 1024), (torch.float32, 24),
+                                         (torch.bfloat16, 33)])
+def test_rows_past_four_gigabytes(dtype, width):
+    """Pages whose elements lie more than 2^31 elements from the pool's start."""
+    pool, table, lengths, w, pos = make([900, 333, 1], 16, width, dtype)
+    x = want(pool, table, lengths, w, pos, 100, 10)
+    first = 2 ** 31 // (16 * width) + 5
+    big = torch.empty(first + len(pool), 16, width, dtype=dtype, device=DEV)
+    big[first:] = pool
+    wide = torch.where(table < len(pool), table + first, table)
+    n, w1, p1 = evict_by_weight(big, wide, lengths, w, pos, budget=100, recent=10)
+    assert same(big[first:], x[0]) and n.tolist() == x[1]
+    for b, k in enumerate(x[1]):
+        assert same(w1[b, :k], torch.from_numpy(x[2][b, :k]))
+        assert p1[b, :k].tolist() == x[3][b, :k].tolist()
+
+
+def test_the_largest_budget():
+    """Tables of INT32_MAX columns: the columns behind the rows are filled to the end."""
+    pool, table, lengths, w, pos = make([7], 16, 8, torch.float32)
+    n, w1, p1 = evict_by_weight(pool, table, lengths, w, pos, budget=2 ** 31 - 1)
+    assert n.tolist() == [7] and same(w1[0, :7], w[0, :7]) and same(p1[0, :7], pos[0, :7])
+    assert not bool(w1[0, 7:].any()) and int(p1[0, 7:].max()) == int(p1[0, 7:].min()) == -1

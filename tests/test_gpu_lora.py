@@ -89,6 +89,10 @@ CASES = [
     (513, 264, 520, 200, 3, BF, "random"),
     (2000, 512, 1536, 16, 8, BF, "one"),
     (400, 72, 77, 5, 6, BF, "runs"),
+    (300, 256, 1600, 16, 200, BF, "random"),
+    (33, 512, 1000, 33, 40, BF, "random"),
+    (200, 520, 77, 12, 5, BF, "random"),
+    (512, 64, 512, 16, 3, BF, "runs"),
     (33, 70, 97, 3, 4, BF, "random"),
     (200, 70, 97, 16, 4, BF, "runs"),
     (1, 256, 768, 8, 5, F, "one"),
@@ -271,3 +275,38 @@ def test_expanded_and_single_rows(M):
     if M > 1:
         with pytest.raises(ValueError):
             lora_linear(x, w, a, b, ids, out=torch.empty(264, dtype=BF, device=DEV).expand(M, 264))
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_outputs_apart_from_inputs(M):
+    x, w, a, b, ids, s, bias = make(M, 256, 256, 16, 5, BF)
+    wide = torch.empty(M, 512, dtype=BF, device=DEV)
+    for out in (x, w[:M], torch.empty(1, 256, dtype=BF, device=DEV).expand(M, 256)):
+        with pytest.raises(ValueError):
+            lora_linear(x, w, a, b, ids, out=out)
+    wide[:, :256] = x
+    with pytest.raises(ValueError):  # columns beside x: inside the memory that x spans
+        lora_linear(wide[:, :256], w, a, b, ids, out=wide[:, 256:])
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_rows_past_four_gigabytes(dtype):
+    """x, then y, with more than 2^31 elements; the rows at both ends are checked."""
+    K, N = 2048, 16
+    M = 2 ** 31 // K + 700
+    small = make(900, K, N, 8, 5, dtype, pattern="runs")
+    x, w, a, b, ids, s, bias = small
+    big = torch.zeros(M, K, dtype=dtype, device=DEV)
+    big[:450], big[-450:] = x[:450], x[450:]
+    far = torch.full((M,), -1, dtype=torch.int32, device=DEV)
+    far[:450], far[-450:] = ids[:450], ids[450:]
+    y = lora_linear(big, w, a, b, far, scaling=s, bias=bias)
+    check(torch.cat([y[:450], y[-450:]]), small)
+    del big, y
+    K, N = 16, 2048
+    small = make(900, K, N, 8, 5, dtype, pattern="runs")
+    x, w, a, b, ids, s, bias = small
+    big = torch.zeros(M, K, dtype=dtype, device=DEV)
+    big[:450], big[-450:] = x[:450], x[450:]
+    y = lora_linear(big, w, a, b, far, scaling=s, bias=bias)
+    check(torch.cat([y[:450], y[-450:]]), small)

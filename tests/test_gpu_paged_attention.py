@@ -307,3 +307,36 @@ def test_refusals():
     with pytest.raises(NotImplementedError):
         big = torch.zeros(2, 1, 512, device=DEV)
         paged_attention(big, torch.zeros(2, 16, 1024, device=DEV), table, lengths)
+
+
+def test_outputs_apart_from_inputs():
+    q, pool, table, lengths = make([5, 6], 4, 4, 64, 16, torch.bfloat16)
+    w = torch.zeros(2, 40, device=DEV)
+    for out in (q, pool[0, 0].as_strided(q.shape, q.stride()),
+                torch.empty(1, 4, 64, dtype=q.dtype, device=DEV).expand(2, 4, 64)):
+        with pytest.raises(ValueError):
+            paged_attention(q, pool, table, lengths, out=out)
+    with pytest.raises(ValueError):  # shifted against the input
+        paged_attention(q, pool, table, lengths, weights=w[:, :20], weights_out=w[:, 1:21])
+    with pytest.raises(ValueError):
+        paged_attention(q, pool, table, lengths, weights=w[:1].expand(2, 40),
+                        weights_out=w[:1].expand(2, 40))
+    got = paged_attention(q, pool, table, lengths, weights=w, weights_out=w)
+    assert got[1] is w
+
+
+@pytest.mark.parametrize("dtype,H", [(torch.bfloat16, 8), (torch.float32, 8), (torch.bfloat16, 3)])
+def test_rows_past_four_gigabytes(dtype, H):
+    """Pages whose elements lie more than 2^31 elements from the pool's start."""
+    Dh, page = (64, 16) if H == 8 else (20, 16)
+    q, pool, table, lengths = make([700, 33, 1], H, H, Dh, page, dtype)
+    o, tol, w, wtol = want(q, pool, table, lengths)
+    width, n = pool.shape[2], len(pool)
+    first = 2 ** 31 // (page * width) + 5
+    big = torch.empty(first + n, page, width, dtype=dtype, device=DEV)
+    big[first:] = pool
+    live = table < n
+    got, gw = paged_attention(q, big, torch.where(live, table + first, table), lengths,
+                              weights=torch.zeros(w.shape, device=DEV))
+    check(got, o, tol)
+    check(gw, w, wtol)

@@ -43,6 +43,7 @@ def test_paged_attention_refusals():
     assert lib.ck_paged_attention(None, 0, 0, 0) == L.CK_ERR_INVALID_ARG
     assert rc(dtype=L.CK_I8) == L.CK_ERR_UNSUPPORTED
     assert rc(Dh=257) == L.CK_ERR_UNSUPPORTED
+    assert rc(H=4100) == L.CK_ERR_UNSUPPORTED
     for bad in (dict(B=-1), dict(H=0), dict(Hkv=0), dict(H=6), dict(Dh=0), dict(page_size=0),
                 dict(page_table_width=-1), dict(num_pages=-1), dict(scale=float("nan")),
                 dict(page_table_width=2 ** 28), dict(w_out=16), dict(w_out=16, w_in=16, w_width=63)):
@@ -109,7 +110,8 @@ def test_lora_refusals():
 
     assert lib.ck_lora_linear(None, 0, 0, 0) == L.CK_ERR_INVALID_ARG
     assert rc(dtype=L.CK_I8) == L.CK_ERR_UNSUPPORTED
-    assert rc(rank=257) == L.CK_ERR_UNSUPPORTED
+    for big in (dict(rank=257), dict(M=2 ** 28 + 1), dict(N=2 ** 31 - 100), dict(K=2 ** 31 - 100)):
+        assert rc(**big) == L.CK_ERR_UNSUPPORTED, big
     for bad in (dict(M=-1), dict(N=-1), dict(K=0), dict(rank=0), dict(n_adapters=-1)):
         assert rc(**bad) == L.CK_ERR_INVALID_ARG, bad
     for missing in ("x", "w", "a", "b", "ids", "y"):
@@ -135,3 +137,18 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         lora_linear(torch.zeros(2, 8), torch.zeros(4, 8), torch.zeros(1, 2, 8), torch.zeros(1, 4, 2),
                     torch.zeros(2, dtype=i32))
+
+
+def test_outputs_that_share_memory_are_refused():
+    buf = torch.zeros(4, 16)
+    x, y = buf[:2], buf[2:]
+    L.check_output("op", "out", y, x, None)
+    L.check_output("op", "out", torch.zeros(3, 1, 5)[:, :, ::2], x)  # strides, a dimension of one
+    L.check_output("op", "out", torch.zeros(6, 2).t(), x)
+    L.check_output("op", "out", torch.zeros(0, 4), x)
+    for out in (torch.zeros(4).expand(2, 4), torch.zeros(8).as_strided((3, 4), (2, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            L.check_output("op", "out", out, x)
+    for out in (x, buf[1:3], buf[:, 8:]):
+        with pytest.raises(ValueError, match="overlaps an input"):
+            L.check_output("op", "out", out, x)
