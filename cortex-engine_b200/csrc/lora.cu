@@ -10,7 +10,8 @@
 // Two launches: the first computes h[m] = s_i A_i x[m] (rank values a row), the
 // second the product with W, to whose fp32 accumulator it adds B_i h[m]:
 //   * few rows (bf16): lora_rows_kernel, W as the 128-row operand of tcgen05
-//     MMAs and the rows of x as its narrow one, K split over a cluster;
+//     MMAs and the rows of x as its narrow one, K split over a cluster (a row or
+//     two: h in the same launch);
 //   * many rows (bf16): gemm_tc.cu's tiles with the adapters as further K
 //     blocks (h rounded to bf16, rows of other adapters masked off);
 //   * fp32: lora_gemv_kernel (few rows) and lora_sgemm_kernel, on the CUDA cores;
@@ -692,6 +693,10 @@ __global__ void __launch_bounds__(256) lora_copy_kernel(const __nv_bfloat16* src
 // SMs; they exchange their fp32 partials through distributed shared memory,
 // each finishing NTOK / SK of the rows: sum over the ranks in order, adapter
 // and bias added, one rounding, a warp storing 32 neighbouring columns.
+//
+// ONE: no first launch. Each CTA computes its K part of every row's h = A_i x in
+// the two warps that have nothing else to do, and the parts meet as the others
+// do. Every tile of W does that again, so only a few values are left to it.
 
 template <int NTOK, int SK>
 struct RowsCfg {
@@ -705,7 +710,13 @@ struct RowsCfg {
   static constexpr uint32_t COLS = NTOK < 32 ? 32 : NTOK;
 };
 
-template <int NTOK, int SK>
+// Values of h (M rank) that lora_rows_kernel computes itself: as many as its two
+// warps hold at once. One launch against two, us a call in a captured sequence of
+// them: 1 x 512 x 1536, rank 16, 4.7 / 5.0; 1 x 4096 x 4096, rank 32, 11.8 / 12.4; 2 x
+// 1024 x 256, rank 16, 5.2 / 5.5; with 64 values 4 x 512 x 1536, rank 16, 5.9 / 5.4.
+constexpr int kOneH = 32;
+
+template <int NTOK, int SK, bool ONE>
 __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ CUtensorMap tmW,
                                                         const __grid_constant__ CUtensorMap tmX,
                                                         const LoraParams p, int n_tiles) {
@@ -722,6 +733,8 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_id = reinterpret_cast<int*>(smem + C::RING + 256);  // [NTOK] adapters of the rows
+  __shared__ float s_part[ONE ? kOneH : 1];  // h of this CTA's part of K
+  __shared__ __align__(16) float s_h[ONE ? kOneH : 1];  // h of the rows that it finishes
   const ck_lora_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = SK > 1 ? (int)cl_rank() : 0;
@@ -752,6 +765,10 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (ONE) {
+    grid_dep_wait();
+    grid_dep_launch();
+  }
 
   constexpr int PER = (NTOK + SK - 1) / SK;  // rows of x that this CTA finishes
   const int c0 = rank * PER;
@@ -759,7 +776,7 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
   bool ok = true;
   if (warp >= 2) {
     // the idle warps fetch the adapters' rows that the epilogue will read
-    for (int c = tid - 64; c < rows; c += 64) s_id[c] = adapter_of(a, m0 + c0 + c, false);
+    for (int c = tid - 64; c < rows; c += 64) s_id[c] = adapter_of(a, m0 + c0 + c, ONE && n0 == 0);
     asm volatile("bar.sync 1, 64;" ::: "memory");
     const int64_t line = (int64_t)min((int64_t)128, a.N - n0) * a.rank * 2;  // bytes of B_i's 128 rows
     for (int c = 0; c < rows; ++c)
@@ -769,6 +786,47 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
         for (int64_t o = (tid - 64) * 128; o < line; o += 64 * 128)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(src + o));
       }
+    if constexpr (ONE) {
+      // 8 lanes for VB values of h, 16 bytes of a K block each
+      constexpr int VB = kOneH / 8;
+      const int values = (int)a.M * a.rank, sub = lane & 7;
+      const __nv_bfloat16 *x[VB], *A[VB];
+      float d[VB];
+      bool in[VB];
+#pragma unroll
+      for (int i = 0; i < VB; ++i) {
+        const int v = (tid - 64) / 8 + 8 * i;
+        const int r = min(v, values - 1) / a.rank, j = min(v, values - 1) - r * a.rank;
+        const int id = v < values ? adapter_of(a, r, false) : -1;
+        in[i] = id >= 0;
+        x[i] = reinterpret_cast<const __nv_bfloat16*>(a.x) + r * a.ldx;
+        A[i] = reinterpret_cast<const __nv_bfloat16*>(a.a) + ((int64_t)max(id, 0) * a.rank + j) * a.K;
+        d[i] = 0.f;
+      }
+#pragma unroll 2
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int64_t k = kb * (int64_t)64 + sub * 8;
+        float xv[VB][8], av[VB][8];
+#pragma unroll
+        for (int i = 0; i < VB; ++i) {
+          const bool here = in[i] && k < a.K;
+          const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+          unpack8(here ? __ldg(reinterpret_cast<const uint4*>(x[i] + k)) : zero, xv[i]);
+          unpack8(here ? __ldg(reinterpret_cast<const uint4*>(A[i] + k)) : zero, av[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < VB; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[i] = fmaf(xv[i][e], av[i][e], d[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < VB; ++i) {
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) d[i] += __shfl_xor_sync(0xffffffffu, d[i], o);
+        const int v = (tid - 64) / 8 + 8 * i;
+        if (sub == 0 && v < values) s_part[v] = d[i];
+      }
+    }
   }
   if (warp == 0 && lane == 0) {
     int issued = 0;
@@ -821,13 +879,33 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
     }
   }
   tc_fence_before();
-  grid_dep_wait();  // h is there
-  grid_dep_launch();
+  if (!ONE) {
+    grid_dep_wait();  // h is there
+    grid_dep_launch();
+  }
   if (SK > 1) cl_sync(); else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::COLS);
   }
+  if constexpr (ONE) {
+    for (int i = tid; i < rows * a.rank; i += 128) {
+      const int id = s_id[i / a.rank];
+      float v = 0.f;
+#pragma unroll
+      for (int r = 0; r < SK; ++r) {
+        float f;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                     : "=f"(f)
+                     : "r"((SK > 1 ? cl_map(s_part, r) : smem_u32(s_part)) + (c0 * a.rank + i) * 4)
+                     : "memory");
+        v += f;
+      }
+      s_h[i] = id >= 0 && a.scaling != nullptr ? v * __ldg(a.scaling + id) : v;
+    }
+    __syncthreads();
+  }
+  const float* h_rows = ONE ? s_h : p.h + (m0 + c0) * a.rank;  // of the rows that it finishes
   const int n = n0 + tid;
   if (ok && n < a.N) {
     constexpr int UB = PER < 4 ? PER : 4;  // rows in flight
@@ -863,7 +941,7 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
           h0[u] = h1[u] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (id < 0) continue;
           const __nv_bfloat16* br = B + ((int64_t)id * a.N + n) * a.rank + j;
-          const float* h = p.h + (m0 + c0 + c + u) * a.rank + j;
+          const float* h = h_rows + (c + u) * a.rank + j;
           if (vec) {
             w[u] = __ldg(reinterpret_cast<const uint4*>(br));
             h0[u] = *reinterpret_cast<const float4*>(h);
@@ -912,6 +990,7 @@ enum Path { PATH_ROWS, PATH_TILES, PATH_F32, PATH_SIMT };
 struct LoraPlan {
   LoraParams p;
   Path path;
+  bool one;                       // PATH_ROWS: one launch, no workspace
   int ld_h, max_slots, tiles;     // PATH_TILES
   int64_t ld_b, ld_stage;         // packed B / staged y row strides, 0: used in place
   size_t off_h, off_cnt, off_slots, off_b, off_y;
@@ -952,8 +1031,9 @@ int make_plan(const ck_lora_args& a, LoraPlan& pl) {
                    (int64_t)a.n_adapters * a.N <= INT32_MAX - 256 &&
                    (int64_t)a.n_adapters * a.rank <= INT32_MAX - 256;
   pl.path = a.dtype == CK_F32 ? PATH_F32 : !tma ? PATH_SIMT : by_rows(a) ? PATH_ROWS : PATH_TILES;
+  pl.one = pl.path == PATH_ROWS && a.M <= 16 && a.M * a.rank <= kOneH;
   if (pl.path != PATH_TILES) {
-    pl.bytes = up((size_t)a.M * a.rank * 4);
+    pl.bytes = pl.one ? 0 : up((size_t)a.M * a.rank * 4);
     return CK_OK;
   }
   pl.ld_h = (a.rank + 7) / 8 * 8;
@@ -1014,7 +1094,7 @@ int run_f32(const LoraParams& p, cudaStream_t st) {
   return launch_sgemm<4, 2, 2, VEC>(p, st);
 }
 
-template <int NTOK, int SK>
+template <int NTOK, int SK, bool ONE>
 int launch_rows(const LoraParams& p, cudaStream_t st) {
   using C = RowsCfg<NTOK, SK>;
   const ck_lora_args& a = p.a;
@@ -1022,7 +1102,7 @@ int launch_rows(const LoraParams& p, cudaStream_t st) {
   if (!make_tmap_2d(&tw, a.w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.K, a.N, a.ldw, 64, 128, 128) ||
       !make_tmap_2d(&tx, a.x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.K, a.M, a.ldx, 64, NTOK, 128))
     return CK_ERR_INVALID_ARG;
-  auto kern = lora_rows_kernel<NTOK, SK>;
+  auto kern = lora_rows_kernel<NTOK, SK, ONE>;
   if (!smem_attr_ready(reinterpret_cast<const void*>(kern), C::SMEM)) return record_cuda_error();
   const int n_tiles = (int)((a.N + 127) / 128);
   cudaLaunchAttribute attr[2];
@@ -1042,7 +1122,7 @@ int launch_rows(const LoraParams& p, cudaStream_t st) {
   return launch_cfg(cfg, kern, tw, tx, p, n_tiles);
 }
 
-template <int NTOK>
+template <int NTOK, bool ONE = false>
 int launch_rows_k(const LoraParams& p, cudaStream_t st) {
   // K split until the tiles give every SM a CTA (or a CTA one K block)
   const int64_t units = (p.a.N + 127) / 128 * ((p.a.M + NTOK - 1) / NTOK);
@@ -1050,10 +1130,10 @@ int launch_rows_k(const LoraParams& p, cudaStream_t st) {
   const int sms = num_sms() > 0 ? num_sms() : 148;
   int sk = 1;
   while (sk < 8 && units * sk < sms && kb >= 2 * sk) sk *= 2;
-  if (sk == 8) return launch_rows<NTOK, 8>(p, st);
-  if (sk == 4) return launch_rows<NTOK, 4>(p, st);
-  if (sk == 2) return launch_rows<NTOK, 2>(p, st);
-  return launch_rows<NTOK, 1>(p, st);
+  if (sk == 8) return launch_rows<NTOK, 8, ONE>(p, st);
+  if (sk == 4) return launch_rows<NTOK, 4, ONE>(p, st);
+  if (sk == 2) return launch_rows<NTOK, 2, ONE>(p, st);
+  return launch_rows<NTOK, 1, ONE>(p, st);
 }
 
 template <int RP, int SK>
@@ -1160,10 +1240,11 @@ int lora_linear(const ck_lora_args& a, void* ws, size_t ws_bytes, cudaStream_t s
   if (a.M == 0 || a.N == 0) return CK_OK;
   if (!a.x || !a.w || !a.y || !a.ids || (a.n_adapters > 0 && (!a.a || !a.b)))
     return CK_ERR_INVALID_ARG;
-  if (ws == nullptr || ws_bytes < pl.bytes || !aligned16(ws)) return CK_ERR_WORKSPACE;
+  if (pl.bytes > 0 && (ws == nullptr || ws_bytes < pl.bytes || !aligned16(ws))) return CK_ERR_WORKSPACE;
   if (pl.path == PATH_TILES) return run_tiles(pl, reinterpret_cast<uint8_t*>(ws), st);
   pl.p.h = reinterpret_cast<float*>(ws);
   if (pl.path == PATH_ROWS) {
+    if (pl.one) return launch_rows_k<16, true>(pl.p, st);
     rc = shrink<__nv_bfloat16>(pl.p, 1, st);
     if (rc != CK_OK) return rc;
     if (a.M <= 16) return launch_rows_k<16>(pl.p, st);

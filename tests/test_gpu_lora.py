@@ -74,6 +74,14 @@ CASES = [
     (1, 512, 1536, 16, 4, BF, "one"),
     (1, 64, 8, 1, 1, BF, "one"),
     (2, 256, 100, 8, 3, BF, "random"),
+    (1, 4096, 1000, 8, 3, BF, "one"),
+    (3, 72, 40, 5, 4, BF, "random"),
+    (5, 520, 264, 3, 2, BF, "random"),
+    (16, 64, 2304, 16, 7, BF, "random"),
+    (16, 128, 77, 16, 7, BF, "runs"),
+    (1, 192, 256, 256, 2, BF, "one"),
+    (1, 200, 20000, 4, 2, BF, "one"),
+    (2, 8, 9, 1, 1, BF, "one"),
     (7, 512, 512, 16, 5, BF, "random"),
     (8, 4096, 256, 16, 8, BF, "random"),
     (17, 520, 264, 24, 9, BF, "random"),
@@ -112,7 +120,7 @@ def test_against_definition(M, K, N, rank, n, dtype, pattern):
     assert L.device_status()[0] == 0
 
 
-@pytest.mark.parametrize("M", [1, 20, 100, 700])
+@pytest.mark.parametrize("M", [1, 8, 20, 100, 700])
 def test_same_inputs_same_bits(M):
     x, w, a, b, ids, s, bias = make(M, 512, 768, 16, 6, BF)
     y = lora_linear(x, w, a, b, ids, scaling=s, bias=bias)
@@ -149,7 +157,7 @@ def test_strides_and_leading_shape(M, dtype):
     check(lora_linear(x, w.t().contiguous().t(), store[:, :16], b, ids, scaling=s, bias=bias), state)
 
 
-@pytest.mark.parametrize("M", [5, 64, 300, 2000])
+@pytest.mark.parametrize("M", [2, 5, 64, 300, 2000])
 def test_rows_do_not_mix(M):
     """NaN and infinities in one row, or in an adapter that no row names, stay there."""
     x, w, a, b, ids, s, bias = state = make(M, 512, 256, 16, 5, BF)
@@ -191,7 +199,7 @@ def test_bad_ids_are_recorded(M):
     assert L.device_status()[0] == 0
 
 
-@pytest.mark.parametrize("M", [4, 300, 1100])
+@pytest.mark.parametrize("M", [1, 4, 300, 1100])
 def test_capture_replay_and_streams(M):
     x, w, a, b, ids, s, bias = state = make(M, 512, 768, 16, 6, BF)
     lora_linear(x, w, a, b, ids, scaling=s, bias=bias)
@@ -310,3 +318,18 @@ def test_rows_past_four_gigabytes(dtype):
     big[:450], big[-450:] = x[:450], x[450:]
     y = lora_linear(big, w, a, b, far, scaling=s, bias=bias)
     check(torch.cat([y[:450], y[-450:]]), small)
+
+
+@pytest.mark.parametrize("M,rank", [(1, 16), (2, 16), (16, 2), (32, 1)])
+def test_bad_ids_of_few_rows(M, rank):
+    x, w, a, b, ids, s, bias = make(M, 512, 300, rank, 5, BF)
+    bad, none = ids.clone(), ids.clone()
+    bad[-1], none[-1] = 5, -1
+    got = lora_linear(x, w, a, b, bad, scaling=s, bias=bias)
+    with pytest.raises(IndexError):
+        L.check_device_status("lora_linear")
+    assert torch.equal(got, lora_linear(x, w, a, b, none, scaling=s, bias=bias))
+    none[:] = -1
+    y = lora_linear(x, w, a[:0], b[:0], none, bias=bias)
+    assert torch.equal(y, lora_linear(x, w, a, b, none, scaling=s, bias=bias))
+    assert L.device_status()[0] == 0

@@ -118,12 +118,14 @@ def test_lora_refusals():
         for M in (3, 300):
             assert rc(M=M, **{missing: None}) == L.CK_ERR_INVALID_ARG
     assert rc(M=0) == L.CK_OK and rc(N=0) == L.CK_OK
-    for M in (3, 300):
+    for M in (40, 300):
         for dtype in (L.CK_BF16, L.CK_F32):
             need = lib.ck_lora_workspace_bytes(_lora(M=M, dtype=dtype))
             assert need > 0
             assert rc(M=M, dtype=dtype, n=need - 1) == L.CK_ERR_WORKSPACE
             assert rc(M=M, dtype=dtype, ws=0) == L.CK_ERR_WORKSPACE
+    # a few rows in one launch: no workspace
+    assert lib.ck_lora_workspace_bytes(_lora(M=1)) == 0
     assert lib.ck_lora_workspace_bytes(None) == 0
 
 
