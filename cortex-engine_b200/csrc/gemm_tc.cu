@@ -271,6 +271,22 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
   // epilogue is done (measured on B200: the early signal made the Cortex
   // forward 1.5-2 % slower with the fused LayerNorm, 1 % faster without it).
   if (!C::LN) grid_dep_launch();
+  // FUSE_LORA: the adapters (.x) and the rows to leave alone of LOOK slots of a
+  // tile, read ahead. A stage holds h once and B_i of per_stage slots (their rows
+  // are as short as the rank).
+  constexpr int LOOK = 4;
+  const int per_stage = C::LORA ? 128 / p.lora_sw : 1;
+  auto slot_ids = [&](int mt, int s0, int (&ids)[LOOK]) {
+#pragma unroll
+    for (int u = 0; u < LOOK; ++u)
+      if (s0 + u < p.lora_max)
+        ids[u] = (int)p.lora_slots[2 * ((int64_t)mt * p.lora_max + s0 + u)].x;
+  };
+  auto slot_masks = [&](int mt, int s0, uint4 (&masks)[LOOK]) {
+#pragma unroll
+    for (int u = 0; u < LOOK; ++u)
+      if (s0 + u < p.lora_max) masks[u] = p.lora_slots[2 * ((int64_t)mt * p.lora_max + s0 + u) + 1];
+  };
 
   if (warp == 0) {
     // ── TMA producer ──
@@ -281,6 +297,13 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
       for (int tile = tile0; tile < num_tiles && !*abort_flag; tile += tstep) {
         int mt, nt, part;
         tile_mn(tile, mt, nt, part);
+        // adapters: fetched LOOK slots at a time, the next ones while these are
+        // issued, the first (from the second tile on) under the K blocks
+        int count = 0, next[LOOK];
+        if (C::LORA && tile != tile0) {
+          count = p.lora_cnt[mt];
+          slot_ids(mt, 0, next);
+        }
         for (int kb = 0; kb < p.num_k_blocks; ++kb) {
           if (!mbar_wait_park(&empty[stage], phase ^ 1, abort_flag, 1)) break;
           if (PAIR) {
@@ -322,20 +345,39 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
           }
         }
         if constexpr (C::LORA) {
-          grid_dep_wait();
-          const int blocks = p.lora_cnt[mt] * p.lora_blocks;
-          for (int i = 0; i < blocks; ++i) {
-            const int slot = i / p.lora_blocks, rb = i - slot * p.lora_blocks;
-            const int id = (int)p.lora_slots[2 * ((int64_t)mt * p.lora_max + slot)].x;
-            if (!mbar_wait_park(&empty[stage], phase ^ 1, abort_flag, 1)) break;
-            mbar_arrive_expect_tx(&full[stage], (uint32_t)((BM + BN) * p.lora_sw));
-            tma_load_2d(sA + stage * C::A_BYTES, &tmY2, &full[stage], rb * BK, mt * BM);
-            // (rows past the adapter's N are columns that the store drops)
-            tma_load_2d(sB + stage * C::B_BYTES, &tmR, &full[stage], rb * BK, id * p.N + nt * BN);
-            ++issued;
-            if (++stage == C::STAGES) {
-              stage = 0;
-              phase ^= 1;
+          if (tile == tile0) {
+            grid_dep_wait();
+            count = p.lora_cnt[mt];
+            slot_ids(mt, 0, next);
+          }
+          bool go = true;
+          for (int s0 = 0; s0 < count && go; s0 += LOOK) {
+            int ids[LOOK];
+#pragma unroll
+            for (int u = 0; u < LOOK; ++u) ids[u] = next[u];
+            slot_ids(mt, s0 + LOOK, next);
+#pragma unroll
+            for (int u = 0; u < LOOK; ++u) {
+              const int at = u & (per_stage - 1);
+              const int left = min(per_stage, count - s0 - u);  // (at == 0) slots of the stage
+              for (int rb = 0; rb < p.lora_blocks && left > 0 && go; ++rb) {
+                if (at == 0) {
+                  go = mbar_wait_park(&empty[stage], phase ^ 1, abort_flag, 1);
+                  if (!go) break;
+                  mbar_arrive_expect_tx(&full[stage], (uint32_t)((BM + left * BN) * p.lora_sw));
+                  tma_load_2d(sA + stage * C::A_BYTES, &tmY2, &full[stage], rb * BK, mt * BM);
+                  ++issued;
+                }
+                // (rows past the adapter's N are columns that the store drops)
+                tma_load_2d(sB + stage * C::B_BYTES + at * BN * p.lora_sw, &tmR, &full[stage],
+                            rb * BK, ids[u] * p.N + nt * BN);
+                if (at == per_stage - 1 || left == 1) {
+                  if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                  }
+                }
+              }
             }
           }
         }
@@ -360,6 +402,12 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
         int mt_, nt_, part;
         tile_mn(tile, mt_, nt_, part);
         const uint32_t idesc = PAIR ? C::IDESC_PAIR : (part >= 0 ? C::IDESC_HALF : C::IDESC);
+        int count = 0;
+        uint4 next[LOOK];
+        if (C::LORA && tile != tile0) {
+          count = p.lora_cnt[mt_];
+          slot_masks(mt_, 0, next);
+        }
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, 2)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
@@ -393,27 +441,41 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
           }
         }
         if constexpr (C::LORA) {
-          if (ok) grid_dep_wait();
-          const int blocks = ok ? p.lora_cnt[mt_] * p.lora_blocks : 0;
-          for (int i = 0; i < blocks; ++i) {
-            const uint4 off =
-                p.lora_slots[2 * ((int64_t)mt_ * p.lora_max + i / p.lora_blocks) + 1];
-            if (!mbar_wait(&full[stage], phase, abort_flag, 3)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t a_addr = smem_u32(sA + stage * C::A_BYTES);
-            const uint32_t b_addr = smem_u32(sB + stage * C::B_BYTES);
-            const int ranks = p.lora_rank - i % p.lora_blocks * BK;  // of this block and behind
-            const int steps = ranks >= BK ? BK / 16 : (ranks + 15) / 16;
-            for (int k = 0; k < steps; ++k)
-              tc_mma_ss_masked(d_tmem, sw_desc(a_addr + k * 32, (uint32_t)p.lora_sw),
-                               sw_desc(b_addr + k * 32, (uint32_t)p.lora_sw), idesc, 1u, off);
-            tc_commit(&empty[stage]);
-            if (++stage == C::STAGES) {
-              stage = 0;
-              phase ^= 1;
+          if (ok && tile == tile0) {
+            grid_dep_wait();
+            count = p.lora_cnt[mt_];
+            slot_masks(mt_, 0, next);
+          }
+          for (int s0 = 0; s0 < count && ok; s0 += LOOK) {
+            uint4 off[LOOK];
+#pragma unroll
+            for (int u = 0; u < LOOK; ++u) off[u] = next[u];
+            slot_masks(mt_, s0 + LOOK, next);
+#pragma unroll
+            for (int u = 0; u < LOOK; ++u) {
+              const int at = u & (per_stage - 1);
+              const int left = min(per_stage, count - s0 - u);
+              for (int rb = 0; rb < p.lora_blocks && left > 0 && ok; ++rb) {
+                if (at == 0) {
+                  ok = mbar_wait(&full[stage], phase, abort_flag, 3);
+                  if (!ok) break;
+                  tc_fence_after();
+                }
+                const uint32_t a_addr = smem_u32(sA + stage * C::A_BYTES);
+                const uint32_t b_addr = smem_u32(sB + stage * C::B_BYTES) + at * BN * p.lora_sw;
+                const int ranks = p.lora_rank - rb * BK;  // of this block and behind
+                const int steps = ranks >= BK ? BK / 16 : (ranks + 15) / 16;
+                for (int k = 0; k < steps; ++k)
+                  tc_mma_ss_masked(d_tmem, sw_desc(a_addr + k * 32, (uint32_t)p.lora_sw),
+                                   sw_desc(b_addr + k * 32, (uint32_t)p.lora_sw), idesc, 1u, off[u]);
+                if (at == per_stage - 1 || left == 1) {
+                  tc_commit(&empty[stage]);
+                  if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                  }
+                }
+              }
             }
           }
         }

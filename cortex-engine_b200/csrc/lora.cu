@@ -469,9 +469,9 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
 //
 // A cluster of SK CTAs per 128-row tile of x and SL adapters. It lists the
 // tile's adapters in the order of their first row (with, for each, the rows that
-// are not its own) and computes D_i[128 x RP] = x_tile A_i^T for its SL of them:
-// both operands by TMA into a ring of 64-wide K blocks, the accumulators side by
-// side in TMEM, each CTA an SK-th of K. A row then takes the columns of its own
+// are not its own) and computes D[128 x SL RP] = x_tile A^T for its SL of them,
+// one MMA's columns: both operands by TMA into a ring of 64-wide K blocks whose
+// depth is what the adapters' number leaves, each CTA an SK-th of K. A row then takes the columns of its own
 // adapter; the ranks' partials meet in distributed shared memory, each CTA
 // finishing RP / SK columns: sum in rank order, times s_i, rounded to bf16 for
 // the GEMM's operand. Bound by x, read once a cluster; clusters whose SL the tile
@@ -479,14 +479,14 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
 // unwritten: no block of the GEMM uses it.
 template <int RP, int SK>
 struct TilesCfg {
-  static constexpr int SL = RP == 16 ? 8 : 4;
+  static constexpr int SL = 256 / RP;  // one MMA's columns
   static constexpr int X_BYTES = 128 * 128;
   static constexpr int A_BYTES = RP * 128;
-  static constexpr int STAGE = X_BYTES + SL * A_BYTES;
-  static constexpr int STAGES = 96 * 1024 / STAGE;  // two CTAs an SM
-  static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
-  static constexpr uint32_t COLS = SL * RP;
-  static_assert(RP * 128 * 4 <= STAGES * STAGE, "the partials lie over the drained ring");
+  static constexpr int RING = 96 * 1024;  // two CTAs an SM
+  static constexpr int STAGES = RING / (X_BYTES + A_BYTES);  // (fewer with more adapters)
+  static constexpr int SMEM = 1024 + RING + 256;
+  static constexpr uint32_t COLS = 256;
+  static_assert(RP * 128 * 4 <= RING, "the partials lie over the drained ring");
 };
 
 template <int RP, int SK>
@@ -499,10 +499,8 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
   __shared__ uint32_t s_first[4];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* sX = smem;
-  uint8_t* sA = smem + C::STAGES * C::X_BYTES;
   float* part = reinterpret_cast<float*>(smem);  // [RP][128], once the ring is drained
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::RING);
   uint64_t* empty = full + C::STAGES;
   uint64_t* done = empty + C::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -577,39 +575,48 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
   // a pass per RP ranks (one, up to 64); none without adapters from slot0 on
   const int n_slots = min(C::SL, total - slot0);
   const int passes = n_slots > 0 ? (a.rank + RP - 1) / RP : 0;
-  int it = 0;  // K blocks so far, of the producing and of the multiplying thread
+  // a stage: 64 columns of x, then of the adapters' A one after the other
+  const int stage_bytes = C::X_BYTES + max(n_slots, 1) * C::A_BYTES;
+  const int stages = min(C::STAGES, C::RING / stage_bytes);
+  int stage = 0, issued = 0;  // of the producing and of the multiplying thread
+  uint32_t phase = 0;
   for (int pass = 0; pass < passes; ++pass) {
     const int j0 = pass * RP;
     if (warp == 0 && lane == 0) {
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % C::STAGES;
-        if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, 30)) break;
-        mbar_arrive_expect_tx(&full[s], C::X_BYTES + n_slots * C::A_BYTES);
-        tma_load_2d(sX + s * C::X_BYTES, &tmX, &full[s], kb * 64, tile * 128);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, 30)) break;
+        mbar_arrive_expect_tx(&full[stage], (uint32_t)stage_bytes);
+        uint8_t* to = smem + stage * stage_bytes;
+        tma_load_2d(to, &tmX, &full[stage], kb * 64, tile * 128);
         for (int i = 0; i < n_slots; ++i)  // (rows past the rank are columns that nobody takes)
-          tma_load_2d(sA + (s * C::SL + i) * C::A_BYTES, &tmA, &full[s], kb * 64,
+          tma_load_2d(to + C::X_BYTES + i * C::A_BYTES, &tmA, &full[stage], kb * 64,
                       s_list[slot0 + i] * a.rank + j0);
+        ++issued;
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
       if (*abort_flag != 0)  // a wait ran out: no copy may land after this CTA's exit
-        for (int s = 0; s < C::STAGES && s < it; ++s) {
-          const int last = it - 1 - ((it - 1 - s) % C::STAGES);
-          mbar_wait(&full[s], (uint32_t)((last / C::STAGES) & 1), nullptr, 33);
+        for (int s = 0; s < stages && s < issued; ++s) {
+          const int last = issued - 1 - ((issued - 1 - s) % stages);
+          mbar_wait(&full[s], (uint32_t)((last / stages) & 1), nullptr, 33);
         }
     } else if (warp == 1 && lane == 0) {
-      constexpr uint32_t idesc = idesc_bf16(128, RP, 0u);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % C::STAGES;
-        if (!mbar_wait(&full[s], (uint32_t)((it / C::STAGES) & 1), abort_flag, 31)) break;
+      const uint32_t idesc = idesc_bf16(128, (uint32_t)(n_slots * RP), 0u);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, 31)) break;
         tc_fence_after();
-        const uint32_t xa = smem_u32(sX + s * C::X_BYTES);
-        for (int i = 0; i < n_slots; ++i) {
-          const uint32_t aa = smem_u32(sA + (s * C::SL + i) * C::A_BYTES);
+        const uint32_t xa = smem_u32(smem + stage * stage_bytes), aa = xa + C::X_BYTES;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_ss(tmem + i * RP, sw128_desc(xa + k * 32, 16, 1024),
-                      sw128_desc(aa + k * 32, 16, 1024), idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+        for (int k = 0; k < 4; ++k)
+          tc_mma_ss(tmem, sw128_desc(xa + k * 32, 16, 1024), sw128_desc(aa + k * 32, 16, 1024),
+                    idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+        tc_commit(&empty[stage]);
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
         }
-        tc_commit(&empty[s]);
       }
       tc_commit(done);
       mbar_wait(done, (uint32_t)(pass & 1), nullptr, 32);
