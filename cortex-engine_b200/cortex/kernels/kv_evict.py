@@ -105,11 +105,11 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
         new_cols = min(new_cols, n)
         for name, given, own in (("out lengths", new_len, lengths), ("out weights", new_w, weights),
                                  ("out positions", new_pos, positions)):
-            L.check_output("evict_by_weight", name, given, pool, page_table,
-                           *(t for t in (lengths, weights, positions)
-                             if t is not own or given is not own))
-        L.check_output("evict_by_weight", "out positions", new_pos, new_w, new_len)
-        L.check_output("evict_by_weight", "out weights", new_w, new_len)
+            if given is not own:
+                L.check_output("evict_by_weight", name, given, pool, page_table, lengths, weights,
+                               positions, *(t for t in out if t is not given))
+            elif not given.is_contiguous():
+                L.check_output("evict_by_weight", name, given)
     if not rows_contiguous(page_table):
         page_table = page_table.contiguous()
     page_ld, row_ld, _ = pool.stride()

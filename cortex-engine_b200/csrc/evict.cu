@@ -31,9 +31,17 @@ constexpr int ST = 512;          // threads of a selecting CTA
 constexpr int SW = ST / 32;
 constexpr int kKeyCap = 49152;   // slots whose key a CTA keeps in shared memory
 constexpr int kBulkRoom = 24576; // shared memory of a warp that moves rows by bulk copies
-constexpr int kBulkRow = 8192;   // bytes of the longest row moved that way
+// Bytes of the longest row moved that way: against copies through registers, us a
+// call, 512 moves in each of 32 sequences of 2 KB rows 17.0 / 21.1, 500 in 16 of
+// 4 KB 16.9 / 17.3, of 8 KB 25.0 / 23.7.
+constexpr int kBulkRow = 4096;
 constexpr int kListed = 1024;    // sequences that the moving kernel lists at a time
-constexpr int kFewMoves = 128;   // rows that the selecting kernel moves itself
+// Rows, and bytes of them, that the selecting kernel moves itself at most. Against a
+// second launch, us a call: 32 sequences of 2 KB rows, 1 move 7.8 / 10.4, 128 moves
+// 14.0 / 15.5, 256 moves 17.8 / 14.2; 16 of 4 KB rows, 100 moves 16.2 / 14.3, of 8
+// KB 24.2 / 16.2. (The bound is on what the table allows, a step moves a row.)
+constexpr int kFewMoves = 128;
+constexpr int64_t kFewBytes = 512 * 1024;
 constexpr uint32_t kProtected = 0xFFFFFFFFu;
 
 struct EvictParams {
@@ -429,19 +437,20 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
   }
 }
 
-// The same through shared memory by bulk copies, a row a lane: `room` bytes of it
-// are the warp's, for at most `slots` rows at a time.
-__device__ __forceinline__ void copy_rows_bulk(const EvictParams& p, int cnt, int64_t from, int64_t to,
-                                               uint32_t room, uint64_t* bar, uint32_t& phase) {
+// The same through shared memory by bulk copies, a lane issuing its move's: the
+// moves of lanes [first, first + slots), whose rows fill the warp's `room`.
+__device__ __forceinline__ void copy_rows_bulk(const EvictParams& p, int first, int slots, int64_t from,
+                                               int64_t to, uint32_t room, uint64_t* bar,
+                                               uint32_t& phase) {
   const int lane = threadIdx.x & 31;
   const uint32_t row = (uint32_t)(p.a.width * p.a.elem_bytes);
   uint8_t* pool = reinterpret_cast<uint8_t*>(p.a.pool);
-  const bool mine = lane < cnt && from >= 0 && to >= 0;
+  const bool mine = lane >= first && lane < first + slots && from >= 0 && to >= 0;
   const uint32_t rows = __popc(__ballot_sync(0xffffffffu, mine));
   if (rows == 0u) return;
   if (lane == 0) mbar_arrive_expect_tx(bar, rows * row);
   __syncwarp();
-  const uint32_t at = room + lane * row;
+  const uint32_t at = room + (uint32_t)(lane - first) * row;
   if (mine)
     asm volatile(
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at),
@@ -481,7 +490,7 @@ __global__ void __launch_bounds__(BULK ? 128 : 256) evict_move_kernel(const Evic
   grid_dep_wait();
   grid_dep_launch();
   uint32_t phase = 0;
-  const int slots = BULK ? (int)min((int64_t)32, (int64_t)kBulkRoom / (p.a.width * p.a.elem_bytes)) : 32;
+  const int slots = BULK ? (int)min((int64_t)32, (int64_t)kBulkRoom / (p.a.width * p.a.elem_bytes)) : 32;  // rows at a time
   for (int b0 = 0; b0 < p.a.B; b0 += kListed) {
     const int n = min(kListed, p.a.B - b0);
     // sums over the sequences: neighbouring ones a thread
@@ -510,7 +519,7 @@ __global__ void __launch_bounds__(BULK ? 128 : 256) evict_move_kernel(const Evic
     __syncthreads();
     const int64_t total = s_end[n - 1];
     const int64_t workers = (int64_t)gridDim.x * NW, w = (int64_t)blockIdx.x * NW + warp;
-    const int per = (int)max((int64_t)1, min((int64_t)slots, (total + workers - 1) / workers));
+    const int per = (int)max((int64_t)1, min((int64_t)32, (total + workers - 1) / workers));
     for (int64_t i0 = w * per; i0 < total; i0 += workers * per) {
       const int cnt = (int)min((int64_t)per, total - i0);
       int64_t from = -1, to = -1;
@@ -524,10 +533,12 @@ __global__ void __launch_bounds__(BULK ? 128 : 256) evict_move_kernel(const Evic
         const int64_t at = (int64_t)(b0 + lo) * p.max_moves + k;
         start_move(p, b0 + lo, p.holes[at], p.movers[at], from, to);
       }
-      if constexpr (BULK)
-        copy_rows_bulk(p, cnt, from, to, smem_u32(s_rows) + warp * kBulkRoom, &s_bar[warp], phase);
-      else
+      if constexpr (BULK) {
+        for (int k = 0; k < cnt; k += slots)
+          copy_rows_bulk(p, k, slots, from, to, smem_u32(s_rows) + warp * kBulkRoom, &s_bar[warp], phase);
+      } else {
         copy_rows_of<V>(p, cnt, from, to);
+      }
     }
   }
   if (BULK) bulk_wait<0>();  // this lane's stores are done
@@ -536,6 +547,7 @@ __global__ void __launch_bounds__(BULK ? 128 : 256) evict_move_kernel(const Evic
 struct EvictPlan {
   EvictParams p;
   int cs;
+  bool few;  // one launch
   size_t off_holes, off_movers, bytes;
 };
 
@@ -567,7 +579,8 @@ int make_plan(const ck_evict_args& a, EvictPlan& pl) {
   pl.off_holes = up((size_t)a.B * 4);
   pl.off_movers = pl.off_holes + list;
   // (one CTA a sequence and few movers: they never leave shared memory)
-  pl.bytes = p.max_moves > 0 && !(pl.cs == 1 && p.max_moves <= kFewMoves) ? pl.off_movers + list : 0;
+  pl.few = p.max_moves <= kFewMoves && (int64_t)p.max_moves * a.width * a.elem_bytes <= kFewBytes;
+  pl.bytes = p.max_moves > 0 && !(pl.cs == 1 && pl.few) ? pl.off_movers + list : 0;
   return CK_OK;
 }
 
@@ -627,11 +640,11 @@ int evict_by_weight(const ck_evict_args& a, void* ws, size_t ws_bytes, cudaStrea
                          (uintptr_t)((int64_t)a.width * a.elem_bytes);
   p.vec_bytes = bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : 2);
   // One round of blocks (two or three an SM), or fewer where the lists cannot be that
-  // long. A list of at most kFewMoves rows (sessions that stay at their budget)
+  // long. A short list (sessions that stay at their budget)
   // is moved by the selecting kernel, without a second launch.
   const bool bulk = p.vec_bytes == 16 && (int64_t)a.width * a.elem_bytes <= kBulkRow;
   const int64_t need = ((int64_t)a.B * p.max_moves + 3) / 4, fill = (bulk ? 2 : 3) * (int64_t)num_sms();
-  p.move_blocks = p.max_moves <= kFewMoves ? 0 : (int32_t)(need < fill ? need : fill);
+  p.move_blocks = pl.few ? 0 : (int32_t)(need < fill ? need : fill);
   rc = pl.cs == 1   ? launch_select<1>(p, st)
        : pl.cs == 4 ? launch_select<4>(p, st)
        : pl.cs == 8 ? launch_select<8>(p, st)
