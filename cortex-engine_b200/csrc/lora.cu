@@ -217,9 +217,11 @@ __global__ void __launch_bounds__(256) lora_gemv_kernel(const LoraParams p) {
 // rows that name it alone (chosen, not multiplied by zero: an infinity of one
 // adapter stays with its rows). A slice is summed by itself, even and odd k in
 // the two halves of paired FMAs, and added to the total: K / 32 + 16 roundings
-// in a row instead of K.
-template <int MT, int WM, int WN, bool VEC>
-__global__ void __launch_bounds__(32 * WM * WN, MT == 8 ? 1 : 3)
+// in a row instead of K. Where the tiles leave SMs idle, the SK CTAs of a cluster
+// share one: each takes a part of K and every SK-th adapter, and finishes TM / SK
+// rows from the partial tiles in distributed shared memory, in rank order.
+template <int MT, int WM, int WN, int SK, bool VEC>
+__global__ void __launch_bounds__(32 * WM * WN, 3)
     lora_sgemm_kernel(const LoraParams p, int n_tiles) {
   constexpr int TM = 4 * MT * WM, TN = 32 * WN, TK = 32, LD = TK + 4, NS = 4;
   constexpr int THREADS = 32 * WM * WN;
@@ -233,12 +235,17 @@ __global__ void __launch_bounds__(32 * WM * WN, MT == 8 ? 1 : 3)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int lm = lane >> 3, ln = lane & 7;
   const int wm = warp / WN, wn = warp % WN;
-  const int64_t m0 = (int64_t)(blockIdx.x / n_tiles) * TM;
-  const int64_t n0 = (int64_t)(blockIdx.x % n_tiles) * TN;
+  const int rank = SK > 1 ? (int)cl_rank() : 0;
+  const int64_t m0 = (int64_t)(blockIdx.x / SK / n_tiles) * TM;
+  const int64_t n0 = (int64_t)(blockIdx.x / SK % n_tiles) * TN;
   const float* x = reinterpret_cast<const float*>(a.x);
   const float* w = reinterpret_cast<const float*>(a.w);
   const float* B = reinterpret_cast<const float*>(a.b);
-  const int slices = (int)((a.K + TK - 1) / TK);
+  // this CTA's slices of K: [k_first, k_first + slices)
+  const int all = (int)((a.K + TK - 1) / TK);
+  const int k_first = (int)((int64_t)all * rank / SK);
+  const int slices = (int)((int64_t)all * (rank + 1) / SK) - k_first;
+  const int64_t k_begin = (int64_t)k_first * TK;
   const int rank_slices = (a.rank + TK - 1) / TK;
   int total = slices;  // and those of the adapters, once they are listed
 
@@ -275,7 +282,7 @@ __global__ void __launch_bounds__(32 * WM * WN, MT == 8 ? 1 : 3)
       const int i = tid + q * THREADS, r = i / (TK / 4), c = i % (TK / 4) * 4;
       const int64_t row = r < TM ? m0 + r : n0 + r - TM;
       const bool in = row < (r < TM ? a.M : a.N);
-      src[q] = r < TM ? x + (in ? row : 0) * a.ldx + c : w + (in ? row : 0) * a.ldw + c;
+      src[q] = (r < TM ? x + (in ? row : 0) * a.ldx : w + (in ? row : 0) * a.ldw) + k_begin + c;
       there |= (uint32_t)in << q;
     }
   }
@@ -286,17 +293,19 @@ __global__ void __launch_bounds__(32 * WM * WN, MT == 8 ? 1 : 3)
 #pragma unroll
         for (int q = 0; q < PIECES; ++q) {
           const int i = tid + q * THREADS, r = i / (TK / 4), c = i % (TK / 4) * 4;
-          const bool in = ((there >> q) & 1u) && (s + 1 < slices || s * (int64_t)TK + c < a.K);
+          const bool in = ((there >> q) & 1u) && (s + 1 < slices || k_begin + s * (int64_t)TK + c < a.K);
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (r * LD + c) * 4),
                        "l"(in ? src[q] : x), "r"(in ? 16 : 0)
                        : "memory");
           src[q] += TK;
         }
       } else {
-        fetch(s, x + m0 * a.ldx, a.ldx, w + n0 * a.ldw, a.ldw, (int64_t)s * TK, a.K, false);
+        fetch(s, x + m0 * a.ldx, a.ldx, w + n0 * a.ldw, a.ldw, k_begin + (int64_t)s * TK, a.K,
+              false);
       }
     } else if (s < total) {
-      const int item = (s - slices) / rank_slices, c0 = (s - slices) % rank_slices * TK;
+      const int item = rank + SK * ((s - slices) / rank_slices);
+      const int c0 = (s - slices) % rank_slices * TK;
       fetch(s, p.h + m0 * a.rank, a.rank, B + ((int64_t)s_list[item] * a.N + n0) * a.rank, a.rank, c0,
             a.rank, a.rank % 4 == 0 && (reinterpret_cast<uintptr_t>(B) & 15u) == 0);
     }
@@ -325,7 +334,7 @@ __global__ void __launch_bounds__(32 * WM * WN, MT == 8 ? 1 : 3)
     }
     if (first) s_list[before] = id;
     __syncthreads();
-    total = slices + count * rank_slices;
+    total = slices + (count > rank ? (count - rank + SK - 1) / SK : 0) * rank_slices;
   }
   if (slices < NS - 1)
     for (int s = 0; s < NS - 1; ++s) fetch_slice(s);
@@ -364,7 +373,7 @@ __global__ void __launch_bounds__(32 * WM * WN, MT == 8 ? 1 : 3)
         }
       }
     }
-    const int only = s < slices ? -2 : s_list[(s - slices) / rank_slices];
+    const int only = s < slices ? -2 : s_list[rank + SK * ((s - slices) / rank_slices)];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -377,15 +386,44 @@ __global__ void __launch_bounds__(32 * WM * WN, MT == 8 ? 1 : 3)
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   const float* bias = reinterpret_cast<const float*>(a.bias);
   float* y = reinterpret_cast<float*>(a.y);
+  if constexpr (SK > 1) {
+    __syncthreads();  // the ring is drained: the partial tile takes its place
+    float* part = sm;  // [TM][TN]
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t n = n0 + wn * 32 + ln + 8 * j;
-    if (n >= a.N) continue;
-    const float bj = bias != nullptr ? __ldg(bias + n) : 0.f;
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int64_t m = m0 + wm * 4 * MT + lm + 4 * i;
-      if (m < a.M) y[m * a.ldy + n] = acc[i][j] + bj;
+      for (int j = 0; j < 4; ++j)
+        part[(wm * 4 * MT + lm + 4 * i) * TN + wn * 32 + ln + 8 * j] = acc[i][j];
+    cl_sync();
+    constexpr int ROWS = TM / SK;
+    static_assert(TM % SK == 0, "whole rows per CTA");
+    for (int i = tid; i < ROWS * TN; i += THREADS) {
+      const int r = rank * ROWS + i / TN, c = i % TN;
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < SK; ++k) {
+        float f;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                     : "=f"(f)
+                     : "r"(cl_map(part + r * TN + c, k))
+                     : "memory");
+        v += f;
+      }
+      if (m0 + r < a.M && n0 + c < a.N)
+        y[(m0 + r) * a.ldy + n0 + c] = v + (bias != nullptr ? __ldg(bias + n0 + c) : 0.f);
+    }
+    cl_sync();  // no CTA leaves while another reads its partials
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t n = n0 + wn * 32 + ln + 8 * j;
+      if (n >= a.N) continue;
+      const float bj = bias != nullptr ? __ldg(bias + n) : 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int64_t m = m0 + wm * 4 * MT + lm + 4 * i;
+        if (m < a.M) y[m * a.ldy + n] = acc[i][j] + bj;
+      }
     }
   }
 }
@@ -990,10 +1028,6 @@ __global__ void __launch_bounds__(128) lora_rows_kernel(const __grid_constant__ 
   if (SK > 1) cl_sync();  // no CTA leaves while another reads its partials
 }
 
-// Rows up to which lora_gemv_kernel runs, lora_sgemm_kernel above (us): 16 x 512 x
-// 1536 10.4 / 20.9, 24 14.7 / 21.2, 48 24.4 / 21.3; 24 x 4096 x 4096 121 / 118, 32 146 / 114.
-constexpr int64_t kGemvMax = 24;
-
 enum Path { PATH_ROWS, PATH_TILES, PATH_F32, PATH_SIMT };
 
 struct LoraPlan {
@@ -1080,15 +1114,30 @@ int shrink(const LoraParams& p, int early, cudaStream_t st) {
              : launch_pdl(lora_shrink_kernel<T, 1, false>, grid, dim3(256), 0, st, p, jblocks, early);
 }
 
-template <int MT, int WM, int WN, bool VEC>
+// Tiles of 32 x 64 (128 x 64 took 87 us where they take 65 at 1024 x 512 x 1536, and
+// 1234 against 1189 at 1266 x 4096 x 4096).
+template <int SK, bool VEC>
 int launch_sgemm(const LoraParams& p, cudaStream_t st) {
-  constexpr int TM = 4 * MT * WM, TN = 32 * WN;
+  constexpr int MT = 4, WM = 2, WN = 2, TM = 4 * MT * WM, TN = 32 * WN;
   constexpr int smem = 4 * (TM + TN) * 36 * 4;
-  auto kern = lora_sgemm_kernel<MT, WM, WN, VEC>;
+  auto kern = lora_sgemm_kernel<MT, WM, WN, SK, VEC>;
   if (!smem_attr_ready(reinterpret_cast<const void*>(kern), smem)) return record_cuda_error();
   const int n_tiles = (int)((p.a.N + TN - 1) / TN);
-  return launch_pdl(kern, dim3((unsigned)((p.a.M + TM - 1) / TM * n_tiles)), dim3(32 * WM * WN), smem,
-                    st, p, n_tiles);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = SK;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.a.M + TM - 1) / TM * n_tiles * SK));
+  cfg.blockDim = dim3(32 * WM * WN);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return launch_cfg(cfg, kern, p, n_tiles);
 }
 
 template <bool VEC>
@@ -1096,11 +1145,21 @@ int run_f32(const LoraParams& p, cudaStream_t st) {
   const ck_lora_args& a = p.a;
   const unsigned gx = (unsigned)((a.N + 7) / 8);
   if (a.M == 1) return launch_pdl(lora_gemv_kernel<1, VEC>, dim3(gx), dim3(256), 0, st, p);
-  if (a.M <= kGemvMax)
+  // W once for 8 rows, against tiles whose K is split (us): 8 x 4096 x 4096 44 / 49, 16 67
+  // / 51; 8 x 512 x 1536 7.2 / 9.5, 24 12.1 / 9.6; 24 x 2048 x 512 12.7 / 13.5, 24 x 256 x
+  // 256 5.5 / 9.2.
+  if (a.M <= 8 || (a.M <= 24 && a.N <= 1024))
     return launch_pdl(lora_gemv_kernel<8, VEC>, dim3(gx, (unsigned)((a.M + 7) / 8)), dim3(256), 0, st, p);
-  // 128 x 64 tiles once they give every SM one, else 32 x 64
-  if ((a.M + 127) / 128 * ((a.N + 63) / 64) >= num_sms()) return launch_sgemm<8, 4, 2, VEC>(p, st);
-  return launch_sgemm<4, 2, 2, VEC>(p, st);
+  // K split while the SMs (three CTAs each) have room and a CTA keeps two slices:
+  // 32 x 4096 x 4096 51 us against 114 unsplit, 64 x 512 x 1536 12.4 against 21.4
+  const int64_t tiles = (a.M + 31) / 32 * ((a.N + 63) / 64), slices = (a.K + 31) / 32;
+  const int sms = num_sms() > 0 ? num_sms() : 148;
+  int sk = 1;
+  while (sk < 8 && 2 * tiles * sk <= 3 * sms && slices >= 4 * sk) sk *= 2;
+  if (sk == 8) return launch_sgemm<8, VEC>(p, st);
+  if (sk == 4) return launch_sgemm<4, VEC>(p, st);
+  if (sk == 2) return launch_sgemm<2, VEC>(p, st);
+  return launch_sgemm<1, VEC>(p, st);
 }
 
 template <int NTOK, int SK, bool ONE>

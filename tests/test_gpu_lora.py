@@ -105,6 +105,9 @@ CASES = [
     (200, 70, 97, 16, 4, BF, "runs"),
     (1, 256, 768, 8, 5, F, "one"),
     (301, 256, 768, 8, 5, F, "runs"),
+    (100, 1024, 264, 40, 9, F, "random"),
+    (45, 520, 77, 3, 1, F, "one"),
+    (64, 2050, 129, 7, 30, F, "random"),
     (130, 70, 97, 3, 4, F, "random"),
     (1500, 512, 264, 64, 9, F, "random"),
     (40, 1024, 64, 256, 2, F, "random"),
