@@ -74,7 +74,9 @@ __device__ __forceinline__ int adapter_of(const ck_lora_args& a, int64_t m, bool
 }
 
 // h: a warp per row and JB ranks, its lanes over K; the JB sums are reduced
-// together (a lane gives half of its sums away at each step).
+// together (a lane gives half of its sums away at each step). Bound by latency: x
+// and A come from L2 (48 rows, K 4096, rank 16: about 5 us, most of them beside the
+// product).
 template <typename T, int JB, bool VEC>
 __global__ void __launch_bounds__(256) lora_shrink_kernel(const LoraParams p, int jblocks, int early) {
   grid_dep_wait();
@@ -154,7 +156,8 @@ __device__ __forceinline__ float adapter_part(const LoraParams& p, int id, int64
   return d;
 }
 
-// Up to MR rows of x at a time: a warp a row of W, read once for them; bound by W.
+// Up to MR rows of x at a time: a warp a row of W, read once for them; bound by W
+// (2 x 4096 x 4096 36 us a call, 67 MB at 1.9 TB/s; 1 x 512 x 1536 6 us).
 template <int MR, bool VEC>
 __global__ void __launch_bounds__(256) lora_gemv_kernel(const LoraParams p) {
   grid_dep_wait();
@@ -219,7 +222,8 @@ __global__ void __launch_bounds__(256) lora_gemv_kernel(const LoraParams p) {
 // the two halves of paired FMAs, and added to the total: K / 32 + 16 roundings
 // in a row instead of K. Where the tiles leave SMs idle, the SK CTAs of a cluster
 // share one: each takes a part of K and every SK-th adapter, and finishes TM / SK
-// rows from the partial tiles in distributed shared memory, in rank order.
+// rows from the partial tiles in distributed shared memory, in rank order. Bound
+// by the FMA pipe: 1266 x 4096 x 4096 1188 us, 36 TF/s; 301 x 256 x 768 13 us a call.
 template <int MT, int WM, int WN, int SK, bool VEC>
 __global__ void __launch_bounds__(32 * WM * WN, 3)
     lora_sgemm_kernel(const LoraParams p, int n_tiles) {
@@ -429,7 +433,8 @@ __global__ void __launch_bounds__(32 * WM * WN, 3)
 }
 
 // bf16 whose strides break TMA's 16-byte rules: 64 x 64 tiles, 4 x 4 a thread,
-// the next K slice in registers while this one is multiplied.
+// the next K slice in registers while this one is multiplied. Not made for speed:
+// 2000 x 510 x 1536 248 us, where 2000 x 512 x 1536 takes 15 by the tiles.
 __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int n_tiles) {
   using T = __nv_bfloat16;
   constexpr int TM = 64, TN = 64, TK = 16;
@@ -514,7 +519,9 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
 // finishing RP / SK columns: sum in rank order, times s_i, rounded to bf16 for
 // the GEMM's operand. Bound by x, read once a cluster; clusters whose SL the tile
 // has no adapters for leave after the list. h of rows without an adapter stays
-// unwritten: no block of the GEMM uses it.
+// unwritten: no block of the GEMM uses it. 8192 x 512, 8 adapters of rank 16: 11 us
+// from cold caches, of which the chain ids, list, first operands, partials, sum is
+// all; its bytes would take 1.5.
 template <int RP, int SK>
 struct TilesCfg {
   static constexpr int SL = 256 / RP;  // one MMA's columns
@@ -716,7 +723,8 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
 }
 
 // Row copies with a change of stride: B rows padded to 16-byte rows (rank not
-// a multiple of 8), and y out of the padded staging rows (N or ldy not one).
+// a multiple of 8; 2000 x 512 x 1536 of rank 12 19 us against 15 of rank 16), and y
+// out of the padded staging rows (N or ldy not one; 27 us at N 1535).
 __global__ void __launch_bounds__(256) lora_copy_kernel(const __nv_bfloat16* src, int64_t ld_src,
                                                         __nv_bfloat16* dst, int64_t ld_dst,
                                                         int64_t rows, int64_t cols) {
@@ -737,7 +745,8 @@ __global__ void __launch_bounds__(256) lora_copy_kernel(const __nv_bfloat16* src
 // cluster share a tile, each an SK-th of K, so that a small W still fills the
 // SMs; they exchange their fp32 partials through distributed shared memory,
 // each finishing NTOK / SK of the rows: sum over the ranks in order, adapter
-// and bias added, one rounding, a warp storing 32 neighbouring columns.
+// and bias added, one rounding, a warp storing 32 neighbouring columns. 48 rows,
+// K = N = 4096: 18 us a call, W at 1.9 TB/s.
 //
 // ONE: no first launch. Each CTA computes its K part of every row's h = A_i x in
 // the two warps that have nothing else to do, and the parts meet as the others

@@ -26,6 +26,10 @@
 // input.
 //
 // All statistics are fp32 in the log2 domain (s log2(e), 2^x).
+//
+// Measured: 16 sequences of 3000 to 32768 positions, 32 heads over 8 of 128, 840 MB,
+// 141 us a call (6.0 TB/s); 32 sequences of 32 to 4096, 12 heads of 64, with weights
+// 30 us (25 for the stream, 2.8 TB/s); 300 positions, 8 heads of 64, 4.6 us.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -759,7 +763,8 @@ __global__ void __launch_bounds__(NW * 32) paged_stream_kernel(const PagedParams
 // together: at each of the first three butterfly steps a lane gives half of
 // its sums away and keeps the other half, so 9 shuffles serve 8 rows instead
 // of 40, and lane L ends with the score of row L / 4. The exponentials are then
-// one per lane for all 8 rows.
+// one per lane for all 8 rows. Bound by its instructions: 16 sequences of 3000 to
+// 32768 positions, 32 heads over 8 of 96, 963 us.
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float* f) {
@@ -923,7 +928,9 @@ __global__ void __launch_bounds__(NW * 32) paged_simt_kernel(const PagedParams p
 // ── parts put together; weights ─────────────────────────────────────────────
 //
 // Blocks [0, out_blocks) write one (b, h) output each; the rest write the
-// weights of 256 positions of one sequence each.
+// weights of 256 positions of one sequence each. Bound by loads that depend on one
+// another, so six blocks share an SM (40 registers): 10.9 us against 14.6 with two
+// (32 sequences of 32 to 4096, 12 heads).
 
 constexpr int JT = 256;
 
