@@ -108,6 +108,9 @@ CASES = [
     ([9000, 8999], 24, 264, torch.bfloat16, 8000, 4000, "few"),
     ([33000], 128, 8, torch.float32, 5, 2, "equal"),
     ([20000, 6], 100, 8, torch.float32, 19999, 0, "wild"),
+    ([300, 290, 151], 16, 2056, torch.bfloat16, 150, 9, "spread"),
+    ([290, 151, 10], 16, 2050, torch.bfloat16, 150, 9, "few"),
+    ([140, 100], 16, 4000, torch.bfloat16, 70, 9, "spread"),
 ]
 
 
@@ -118,6 +121,15 @@ def test_against_definition(lens, page, width, dtype, budget, recent, weights):
 
 def test_more_slots_than_shared_memory_holds():
     run_case(make([450001] + [100] * 9, 512, 2, torch.float32, weights="few"), 77777, 50)
+
+
+def test_many_moves_of_long_rows():
+    run_case(make([32768, 20], 128, 1024, torch.float32), 16384, 100)
+
+
+def test_more_sequences_than_a_list_holds():
+    rng = np.random.default_rng(5)
+    run_case(make(rng.integers(0, 300, 1100).tolist(), 60, 8, torch.bfloat16), 150, 7)
 
 
 def test_budget_beyond_the_table():

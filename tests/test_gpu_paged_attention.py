@@ -99,6 +99,9 @@ CASES = [
     ([70, 9], 3, 3, 20, 5, torch.bfloat16),
     ([70, 9], 2, 1, 256, 16, torch.bfloat16),
     ([77], 2, 2, 33, 1, torch.bfloat16),
+    ([1000, 3, 0, 513], 8, 8, 64, 64, torch.bfloat16),
+    ([1000], 4, 2, 32, 128, torch.bfloat16),
+    ([500, 9], 4, 4, 64, 16, torch.float32),
     ([0, 1, 7, 8, 9, 24, 25, 1025], 4, 4, 64, 24, torch.float32),
     ([200, 600], 8, 2, 128, 64, torch.float32),
     ([50, 3], 5, 1, 32, 16, torch.float32),
