@@ -98,6 +98,9 @@ CASES = [
     (2000, 512, 1536, 16, 8, BF, "one"),
     (400, 72, 77, 5, 6, BF, "runs"),
     (300, 256, 1600, 16, 200, BF, "random"),
+    (300, 256, 1600, 32, 50, BF, "random"),
+    (300, 128, 1600, 64, 50, BF, "random"),
+    (300, 256, 1600, 100, 9, BF, "random"),
     (33, 512, 1000, 33, 40, BF, "random"),
     (200, 520, 77, 12, 5, BF, "random"),
     (512, 64, 512, 16, 3, BF, "runs"),
