@@ -74,21 +74,19 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
         with torch.cuda.device(d):
             return evict_by_weight(pool, page_table, lengths, weights, positions, budget=budget,
                                    recent=recent, out=out)
-    check_pages("evict_by_weight", pool, page_table, lengths)
+    B, table_width, pages, page_size, width = check_pages("evict_by_weight", pool, page_table, lengths)
     if pool.dtype is not torch.bfloat16 and pool.dtype is not torch.float32:
         raise NotImplementedError(f"evict_by_weight: rows of {pool.dtype}")
     if not 1 <= budget < 2 ** 31 or not 0 <= recent <= budget:
         raise ValueError(f"evict_by_weight: needs 1 <= budget and 0 <= recent <= budget, "
                          f"got {budget} and {recent}")
-    B, table_width = page_table.shape
-    pages, page_size, width = pool.shape
     cap = table_width * page_size
     w_ld, w_cols = _table("weights", weights, torch.float32, B, cap)
     pos_ld, pos_cols = _table("positions", positions, torch.int32, B, cap)
     dev = pool.device
     fill = out is None
     if fill:
-        new_len = torch.empty(B, dtype=torch.int32, device=dev)
+        new_len = torch.empty_like(lengths, memory_format=torch.contiguous_format)
         new_w = torch.empty(B, budget, dtype=torch.float32, device=dev)
         new_pos = torch.empty(B, budget, dtype=torch.int32, device=dev)
         new_w_ld = new_pos_ld = new_cols = budget

@@ -19,13 +19,6 @@ from cortex.kernels.paged_attention import rows_contiguous
 _pack = L.LORA_ARGS.pack
 
 
-def _three(what: str, t: torch.Tensor) -> tuple[int, int, int]:
-    shape = tuple(t.shape)
-    if len(shape) != 3:
-        raise ValueError(f"lora_linear: {what} must have 3 dimensions, got {shape}")
-    return shape
-
-
 def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                 adapter_ids: torch.Tensor, *, scaling: torch.Tensor | None = None,
                 bias: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -55,15 +48,16 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     if d != L.current_device():
         with torch.cuda.device(d):
             return lora_linear(x, w, lora_a, lora_b, adapter_ids, scaling=scaling, bias=bias, out=out)
-    dtype, xs, ws, (n, rank, a_k) = x.dtype, x.shape, w.shape, _three("lora_a", lora_a)
+    dtype, xs, ws, a_shape = x.dtype, x.shape, w.shape, lora_a.shape
     K = xs[-1] if len(xs) > 0 else -1
     lead = xs[:-1]
     if len(ws) != 2 or ws[1] != K or K < 1:
         raise ValueError(f"lora_linear: w must be (N, K) with K = {K}, got {tuple(ws)}")
     N = ws[0]
-    if a_k != K or rank < 1:
-        raise ValueError(f"lora_linear: lora_a must be (n, rank, {K}), got {tuple(lora_a.shape)}")
-    if _three("lora_b", lora_b) != (n, N, rank):
+    if len(a_shape) != 3 or a_shape[2] != K or a_shape[1] < 1:
+        raise ValueError(f"lora_linear: lora_a must be (n, rank, {K}), got {tuple(a_shape)}")
+    n, rank, _ = a_shape
+    if lora_b.shape != (n, N, rank):
         raise ValueError(f"lora_linear: lora_b must be {(n, N, rank)}, got {tuple(lora_b.shape)}")
     if dtype is not w.dtype or dtype is not lora_a.dtype or dtype is not lora_b.dtype:
         raise TypeError(f"lora_linear: x, w, lora_a and lora_b differ in dtype ({dtype}, "
@@ -76,7 +70,7 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     ids, x2 = adapter_ids, x
     if len(lead) != 1:
         ids, x2 = ids.reshape(-1), x.reshape(-1, K)
-    M, ldx, ldw = len(x2), x2.stride()[0], w.stride()[0]
+    M, ldx, ldw = x2.shape[0], x2.stride()[0], w.stride()[0]
     if not rows_contiguous(x2) or (ldx < K and M > 1):  # (rows that share memory: expanded)
         x2, ldx = x2.contiguous(), K
     if not rows_contiguous(w) or (ldw < K and N > 1):

@@ -21,22 +21,25 @@ _pack = L.PAGED_ATTENTION_ARGS.pack
 
 
 def check_pages(what: str, pool: torch.Tensor, page_table: torch.Tensor,
-                lengths: torch.Tensor) -> None:
-    """Checks shared by the operators over a paged pool."""
-    if pool.dim() != 3:
+                lengths: torch.Tensor) -> tuple[int, int, int, int, int]:
+    """Checks shared by the operators over a paged pool: (sequences, pages of a
+    table row, pages, page size, row width)."""
+    shape, table, count = pool.shape, page_table.shape, lengths.shape
+    if len(shape) != 3:
         raise ValueError(f"{what}: pool must be (num_pages, page_size, width), "
-                         f"got {tuple(pool.shape)}")
+                         f"got {tuple(shape)}")
     if page_table.dtype is not torch.int32 or lengths.dtype is not torch.int32:
         raise TypeError(f"{what}: page_table and lengths must be int32, got "
                         f"{page_table.dtype} and {lengths.dtype}")
-    if page_table.dim() != 2 or lengths.dim() != 1 or len(page_table) != len(lengths):
+    if len(table) != 2 or len(count) != 1 or table[0] != count[0]:
         raise ValueError(f"{what}: page_table must be (B, pages) beside lengths (B,), got "
-                         f"{tuple(page_table.shape)} and {tuple(lengths.shape)}")
-    _, page_size, width = pool.shape
+                         f"{tuple(table)} and {tuple(count)}")
+    pages, page_size, width = shape
     if page_size < 1 or width < 1:
         raise ValueError(f"{what}: pages must hold at least one row of one element")
     if pool.stride()[2] != 1 and width > 1:
         raise ValueError(f"{what}: pool rows must be contiguous")
+    return table[0], table[1], pages, page_size, width
 
 
 def rows_contiguous(t: torch.Tensor) -> bool:
@@ -82,15 +85,14 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
         with torch.cuda.device(d):
             return paged_attention(q, pool, page_table, lengths, scale=scale, weights=weights,
                                    out=out, weights_out=weights_out)
-    check_pages("paged_attention", pool, page_table, lengths)
+    B, table_width, pages, page_size, width = check_pages("paged_attention", pool, page_table, lengths)
     dtype = q.dtype
     if dtype is not pool.dtype:
         raise TypeError(f"paged_attention: q is {dtype}, the pool {pool.dtype}")
-    B = len(lengths)
-    pages, page_size, width = pool.shape
-    if q.dim() != 3 or len(q) != B:
-        raise ValueError(f"paged_attention: q must be (B, H, Dh) with B = {B}, got {tuple(q.shape)}")
-    _, H, Dh = q.shape
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != B:
+        raise ValueError(f"paged_attention: q must be (B, H, Dh) with B = {B}, got {tuple(shape)}")
+    _, H, Dh = shape
     if Dh == 0 or width % (2 * Dh) != 0:
         raise ValueError(f"paged_attention: rows of {width} are not K | V of heads of {Dh}")
     Hkv = width // (2 * Dh)
@@ -104,20 +106,19 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
         lengths = lengths.contiguous()
     dev = q.device
     if out is None:
-        out = torch.empty(B, H, Dh, dtype=dtype, device=dev)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(B, H, Dh, dtype=dtype, device=dev)
     elif out.shape != q.shape or out.dtype != dtype or not rows_contiguous(out):
         raise ValueError("paged_attention: out must be like q with contiguous heads")
     else:
         L.check_output("paged_attention", "out", out, q, pool, page_table, lengths, weights,
                        weights_out)
-    table_width = page_table.shape[1]
     W = w_in = w_out = w_in_ld = w_out_ld = 0
     if weights is not None:
         if weights.dtype != torch.float32 or weights.dim() != 2 or weights.shape[0] != B or \
                 weights.shape[1] < table_width * page_size:
             raise ValueError("paged_attention: weights must be float32 (B, >= pages * page_size)")
         if weights_out is None:
-            weights_out = torch.empty(weights.shape, dtype=torch.float32, device=dev)
+            weights_out = torch.empty_like(weights, memory_format=torch.contiguous_format)
         elif weights_out.shape != weights.shape or weights_out.dtype != torch.float32:
             raise ValueError("paged_attention: weights_out must be like weights")
         elif weights_out is weights:
