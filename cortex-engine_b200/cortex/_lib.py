@@ -332,14 +332,23 @@ def stream_of(device: torch.device) -> int:
 _ws_bytes: dict = {}
 
 
-def workspace_bytes(query, key: tuple, block: bytes) -> int:
-    """``query(block)``, remembered per ``key`` (the call's sizes)."""
+def launch(what: str, call, query, key: tuple, block: bytes, dev: torch.device, stream: int) -> None:
+    """``call(block, workspace, bytes, stream)`` with a workspace on ``dev`` of the
+    size that ``query(block)`` gives. The size is remembered per ``key`` (the
+    call's sizes) once a call with it has been accepted: a refused argument
+    block has no size."""
     n = _ws_bytes.get(key)
-    if n is None:
+    known = n is not None
+    if not known:
+        n = query(block)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    rc = call(block, ws.data_ptr() if n else 0, n, stream)
+    if rc != CK_OK:
+        check(rc, what)
+    if not known:
         if len(_ws_bytes) > 4096:
             _ws_bytes.clear()
-        n = _ws_bytes[key] = query(block)
-    return n
+        _ws_bytes[key] = n
 
 
 _get_device = getattr(torch._C, "_cuda_getDevice", None)

@@ -119,12 +119,8 @@ def evict_by_weight(pool: torch.Tensor, page_table: torch.Tensor, lengths: torch
                   positions.data_ptr(), new_pos.data_ptr(), w_ld, new_w_ld, pos_ld, new_pos_ld,
                   min(w_cols, pos_cols, 2 ** 31 - 1), min(new_cols, 2 ** 31 - 1))
     lib = L.load()
-    n = L.workspace_bytes(lib.ck_evict_workspace_bytes, ("evict", d, B, cap, budget, width, pool.dtype),
-                          block)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    rc = lib.ck_evict_by_weight(block, ws.data_ptr() if n else 0, n, L.raw_stream(d))
-    if rc != L.CK_OK:
-        L.check(rc, "ck_evict_by_weight")
+    L.launch("ck_evict_by_weight", lib.ck_evict_by_weight, lib.ck_evict_workspace_bytes,
+             ("evict", d, B, cap, budget, width, pool.dtype), block, dev, L.raw_stream(d))
     return new_len, new_w, new_pos
 
 

@@ -118,11 +118,8 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     # everything the size depends on, alignment included
     key = ("lora", d, dtype, M, K, N, rank, n, (ldx | ldw) & 7, ldy & 7,
            (x_ptr | w_ptr | a_ptr | b_ptr) & 15, y_ptr & 15)
-    nb = L.workspace_bytes(lib.ck_lora_workspace_bytes, key, block)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    rc = lib.ck_lora_linear(block, ws.data_ptr() if nb else 0, nb, L.raw_stream(d))
-    if rc != L.CK_OK:
-        L.check(rc, "ck_lora_linear")
+    L.launch("ck_lora_linear", lib.ck_lora_linear, lib.ck_lora_workspace_bytes, key, block, dev,
+             L.raw_stream(d))
     if out is not None:
         return out
     return y if len(lead) == 1 else y.reshape(*lead, N)

@@ -152,11 +152,8 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
     # everything the size depends on, alignment included
     key = ("attention", d, dtype, B, H, Hkv, Dh, page_size, table_width, W, (pb | pr | qb | qh) & 7,
            (q_ptr | pool_ptr) & 15)
-    n = L.workspace_bytes(lib.ck_paged_attention_workspace_bytes, key, block)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    rc = lib.ck_paged_attention(block, ws.data_ptr() if n else 0, n, L.raw_stream(d))
-    if rc != L.CK_OK:
-        L.check(rc, "ck_paged_attention")
+    L.launch("ck_paged_attention", lib.ck_paged_attention, lib.ck_paged_attention_workspace_bytes, key,
+             block, dev, L.raw_stream(d))
     return out if weights is None else (out, weights_out)
 
 

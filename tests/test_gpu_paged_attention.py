@@ -343,3 +343,16 @@ def test_rows_past_four_gigabytes(dtype, H):
                               weights=torch.zeros(w.shape, device=DEV))
     check(got, o, tol)
     check(gw, w, wtol)
+
+
+def test_a_valid_call_after_a_refused_one():
+    """A scale of NaN is refused; the same shapes with a valid one are not."""
+    q, pool, table, lengths = make([30, 77], 2, 2, 64, 16, torch.bfloat16, seed=8)
+    w = torch.zeros(2, table.shape[1] * 16, device=DEV)
+    with pytest.raises(ValueError):
+        paged_attention(q, pool, table, lengths, weights=w, scale=float("nan"))
+    o, tol, ws, wtol = want(q, pool, table, lengths)
+    out, got = paged_attention(q, pool, table, lengths, weights=w)
+    check(out, o, tol)
+    check(got, ws, wtol + U * ws)
+    assert L.device_status()[0] == 0

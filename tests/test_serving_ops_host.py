@@ -154,3 +154,23 @@ def test_outputs_that_share_memory_are_refused():
     for out in (x, buf[1:3], buf[:, 8:]):
         with pytest.raises(ValueError, match="overlaps an input"):
             L.check_output("op", "out", out, x)
+
+
+def test_a_refused_call_leaves_no_workspace_size():
+    """The size query answers 0 for a block that the call refuses: the next call of
+    the same key asks again."""
+    sizes, seen = [0, 512], []
+
+    def query(block):
+        return sizes[len(seen)]
+
+    def call(block, ws, n, stream):
+        seen.append(n)
+        return L.CK_OK if n == 512 else L.CK_ERR_INVALID_ARG
+
+    key, cpu = ("a key of this test",), torch.device("cpu")
+    with pytest.raises(ValueError):
+        L.launch("op", call, query, key, b"", cpu, 0)
+    L.launch("op", call, query, key, b"", cpu, 0)
+    L.launch("op", call, lambda block: 1 / 0, key, b"", cpu, 0)  # remembered: not asked again
+    assert seen == [0, 512, 512]
