@@ -194,6 +194,14 @@ class StreamingKVCache:
         spare = len(self._free) + sum(len(m.pages) for e, m in self._meta.items() if e not in listed)
         if sum(need) > spare:
             raise RuntimeError(f"append_rows: {sum(need)} pages needed, {spare} can be had")
+        # what may fail comes before the entries change
+        src = rows.contiguous()
+        if src.data_ptr() % 16 != 0:
+            src = src.clone()
+        n_segs = sum(-(-(m.n_events + n) // self.page_size) - m.n_events // self.page_size
+                     for m in metas)
+        host = torch.empty(n_segs, 3, dtype=torch.int32, pin_memory=True)
+        seg = torch.empty(n_segs, 3, dtype=torch.int32, device=self.device)
         for m in metas:  # most recent: never the ones that make room below
             self._lru.move_to_end(m.page_id)
         segs = []
@@ -208,13 +216,12 @@ class StreamingKVCache:
             m.n_events = end
             m.edited = True
             m.last_used_at = time.monotonic()
-        src = rows.contiguous()
+        host.copy_(torch.tensor(segs, dtype=torch.int32))
         with torch.cuda.device(self.device):
-            seg = torch.tensor(segs, dtype=torch.int32).pin_memory().to(self.device,
-                                                                       non_blocking=True)
+            seg.copy_(host, non_blocking=True)
             rc = L.load().ck_copy_rows(src.data_ptr(), len(metas) * n, self.rows.data_ptr(),
                                        self.num_pages * self.page_size, row_bytes, seg.data_ptr(),
-                                       len(segs), L.stream_of(self.device))
+                                       n_segs, L.stream_of(self.device))
         L.check(rc, "ck_copy_rows")
 
     def evict_rows(self, metas: Sequence[PageMeta], weights: torch.Tensor,

@@ -227,3 +227,17 @@ def test_an_edited_entry_is_not_a_windows_rows():
         again = model.forward_streaming(win, cache)["behavior"]
         hit = model.forward_streaming(win, cache)["behavior"]
     assert torch.equal(fresh, again) and torch.equal(fresh, hit)
+
+
+def test_rows_to_append_at_any_address():
+    """Rows that begin off a 16-byte boundary arrive like others, over page ends too."""
+    cache = StreamingKVCache(8, 4, 8, torch.float32, DEV)
+    a, b = cache.write_rows("a", 0, 3), cache.write_rows("b", 0, 4)
+    flat = torch.arange(2 * 6 * 8 + 1, dtype=torch.float32, device=DEV)
+    rows = flat[1:].reshape(2, 6, 8)
+    assert rows.data_ptr() % 16 != 0
+    cache.append_rows([a, b], rows)
+    for m, first, r in ((a, 3, rows[0]), (b, 4, rows[1])):
+        assert (m.n_events, len(m.pages)) == (first + 6, 3)
+        assert torch.equal(cache.pool[m.pages].reshape(-1, 8)[first:first + 6], r)
+    assert L.device_status()[0] == 0
