@@ -196,8 +196,10 @@ class StreamingKVCache:
             raise RuntimeError(f"append_rows: {sum(need)} pages needed, {spare} can be had")
         # what may fail comes before the entries change
         src = rows.contiguous()
-        if src.data_ptr() % 16 != 0:
-            src = src.clone()
+        lo, hi = L.memory_range(src)
+        pool_lo, pool_hi = L.memory_range(self._pool)
+        if lo % 16 != 0 or (lo < pool_hi and pool_lo < hi):
+            src = src.clone()  # (a pool page that is read below may be written as well)
         n_segs = sum(-(-(m.n_events + n) // self.page_size) - m.n_events // self.page_size
                      for m in metas)
         host = torch.empty(n_segs, 3, dtype=torch.int32, pin_memory=True)

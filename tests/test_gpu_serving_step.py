@@ -241,3 +241,17 @@ def test_rows_to_append_at_any_address():
         assert (m.n_events, len(m.pages)) == (first + 6, 3)
         assert torch.equal(cache.pool[m.pages].reshape(-1, 8)[first:first + 6], r)
     assert L.device_status()[0] == 0
+
+
+def test_rows_to_append_that_lie_in_the_pool():
+    """Rows read from pages that the same call writes: they arrive as they were."""
+    cache = StreamingKVCache(5, 4, 4096, torch.float32, DEV)
+    a, b = cache.write_rows("a", 0, 4), cache.write_rows("b", 0, 12)
+    cache.rows.copy_(torch.arange(20, device=DEV)[:, None].expand(20, 4096))
+    assert (a.pages, b.pages) == ([4], [3, 2, 1])
+    cache.append_rows([a], cache.rows[2:14][None])  # "b" makes room: its pages 1, 2 and 3
+    assert a.pages == [4, 1, 2, 3] and not cache.is_live(b)
+    got = cache.pool[a.pages].reshape(-1, 4096)
+    assert got[:, 0].tolist() == [16, 17, 18, 19] + list(range(2, 14))
+    assert torch.equal(got, got[:, :1].expand(16, 4096))
+    assert L.device_status()[0] == 0
