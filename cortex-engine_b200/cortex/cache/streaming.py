@@ -270,7 +270,9 @@ class StreamingKVCache:
     def _entry_for(self, session_id: str, bin_start: int, n_pages: int) -> PageMeta:
         key = (session_id, bin_start)
         eid = self._table.get(key)
-        if eid is not None and len(self._meta[eid].pages) != n_pages:
+        # (an edited entry's rows are its holder's: what replaces them is a new entry,
+        # and the old PageMeta is no longer live)
+        if eid is not None and (len(self._meta[eid].pages) != n_pages or self._meta[eid].edited):
             self._free_entry(eid)
             eid = None
         if eid is None:
@@ -280,7 +282,6 @@ class StreamingKVCache:
             self._meta[eid] = PageMeta(eid, session_id, bin_start, 0, time.monotonic(), pages)
             self._lru[eid] = None
         self._lru.move_to_end(eid)
-        self._meta[eid].edited = False
         return self._meta[eid]
 
     def _allocate(self, n_pages: int) -> list[int]:

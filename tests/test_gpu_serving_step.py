@@ -255,3 +255,24 @@ def test_rows_to_append_that_lie_in_the_pool():
     assert got[:, 0].tolist() == [16, 17, 18, 19] + list(range(2, 14))
     assert torch.equal(got, got[:, :1].expand(16, 4096))
     assert L.device_status()[0] == 0
+
+
+def test_a_rewritten_key_is_another_entry():
+    """Rows written under the key of an entry that grew or shrank replace it: its
+    PageMeta does not stand for the new rows, however many pages they take."""
+    for n in (2, 4, 5):
+        for rewrite in ("write_rows", "write"):
+            cache = StreamingKVCache(8, 4, 16, torch.float32, DEV)
+            a = cache.write_rows("a", 0, 3)
+            cache.append_rows([a], torch.ones(1, 1, 16, device=DEV))
+            if rewrite == "write_rows":
+                new = cache.write_rows("a", 0, n)
+            else:
+                cache.write("a", 0, torch.zeros(n, 16, device=DEV))
+                new = cache.lookup("a", 0)
+            assert new is not a and not cache.is_live(a) and cache.is_live(new)
+            assert not new.edited and new.n_events == (min(n, 4) if rewrite == "write" else n)
+            with pytest.raises(ValueError):
+                cache.page_table([a])
+            assert cache.page_table([new])[1].tolist() == [new.n_events]
+            assert sorted(cache._free + new.pages) == list(range(8))
