@@ -2,13 +2,14 @@
 
 For a batch of windows, each keyed by (session_id, bin_start):
 
-1. windows found in the cache (same key, same event count) are hits; the
-   others are misses;
+1. windows found in the cache (same key, same event count, entry not edited)
+   are hits; the others are misses;
 2. ``ck_forward_kv`` runs packing, tokenizer + norm_kv and kv_proj for the
    missed windows only (one packed int32 batch, one host-to-device copy);
 3. ``ck_copy_rows`` assembles the batch's packed K|V rows: hits from their
    pool pages, misses from step 2, and writes the missed windows' rows into
-   newly reserved pages;
+   newly reserved pages (not where an edited entry has the window's key, or
+   where edited entries leave no room);
 4. ``ck_forward_from_kv`` runs the rest of the forward (latent queries, cross
    attention, the self-attention stack, the head).
 
@@ -101,6 +102,8 @@ def forward_with_kv_cache(model, windows: list[dict], cache) -> torch.Tensor:
     for j, b in enumerate(miss):
         seg_miss.append((int(miss_off[j]), int(off_all[b]), int(counts[b])))
         w = windows[b]
+        if metas[b] is not None and metas[b].edited:
+            continue  # its holder's rows stay
         meta = cache.write_rows(w["session_id"], int(w["bin_start"]), int(counts[b]))
         if meta is not None:
             written.append((meta, int(miss_off[j])))

@@ -20,6 +20,10 @@ are (they depend only on the window's own events), so the key is the window
 identity (session, first bin). Rows of the same spike in an overlapping window
 are NOT the same: time bins are window-relative (a max_time_bins vocabulary),
 so a shifted window shifts every time embedding.
+
+An entry that grew or shrank (``append_rows``, ``evict_rows``) is no such
+function: its rows are nowhere else. It makes room for nothing and stays until
+``evict_session`` frees it or its key is written again.
 """
 
 from __future__ import annotations
@@ -70,7 +74,9 @@ class StreamingKVCache:
         self._table: dict[tuple[str, int], int] = {}      # key -> entry id (its first page)
         self._meta: dict[int, PageMeta] = {}              # entry id -> metadata
         self._free: list[int] = list(range(num_pages))
-        self._lru: OrderedDict[int, None] = OrderedDict()  # entry ids, most recent last
+        # entry ids: those that may make room, most recent last, and the edited ones
+        self._lru: OrderedDict[int, None] = OrderedDict()
+        self._held: set[int] = set()
         self._hits = 0
         self._misses = 0
 
@@ -88,8 +94,11 @@ class StreamingKVCache:
 
     def write(self, session_id: str, bin_start: int, embeddings: torch.Tensor) -> None:
         """Cache the first ``page_size`` rows of ``embeddings`` in one page,
-        reusing the key's page if present (cortex/cache/streaming.py:150-184)."""
+        reusing the key's page if present (cortex/cache/streaming.py:150-184).
+        Raises ``RuntimeError`` when edited entries hold every page."""
         n = min(int(embeddings.shape[0]), self.page_size)
+        if self._pages_but(self._held - {self._table.get((session_id, bin_start))}) < 1:
+            raise RuntimeError("write: edited entries hold every page")
         meta = self._entry_for(session_id, bin_start, n_pages=1)
         self._pool[meta.pages[0], :n, :] = embeddings[:n].detach().to(
             dtype=self._pool.dtype, device=self.device)
@@ -121,7 +130,7 @@ class StreamingKVCache:
         if eid is None:
             self._misses += 1
             return None
-        self._lru.move_to_end(eid)
+        self._touch(eid)
         meta = self._meta[eid]
         meta.last_used_at = time.monotonic()
         self._hits += 1
@@ -129,10 +138,10 @@ class StreamingKVCache:
 
     def write_rows(self, session_id: str, bin_start: int, n_rows: int) -> PageMeta | None:
         """Reserve pages for ``n_rows`` rows of the key (replacing an older
-        entry); None when they cannot fit in the pool. The caller copies the
-        rows in (``segments(meta, ..., into_pool=True)`` + ``ck_copy_rows``)."""
+        entry); None when they cannot fit beside the edited entries. The caller
+        copies the rows in (``segments(meta, ..., into_pool=True)`` + ``ck_copy_rows``)."""
         n_pages = max(1, -(-n_rows // self.page_size))
-        if n_pages > self.num_pages:
+        if n_pages > self._pages_but(self._held - {self._table.get((session_id, bin_start))}):
             return None
         meta = self._entry_for(session_id, bin_start, n_pages)
         meta.n_events = n_rows
@@ -167,14 +176,14 @@ class StreamingKVCache:
         for b, m in enumerate(metas):
             host[b, 0] = m.n_events
             host[b, 1:1 + len(m.pages)] = torch.tensor(m.pages, dtype=torch.int32)
-            self._lru.move_to_end(m.page_id)
+            self._touch(m.page_id)
         dev = host.pin_memory().to(self.device, non_blocking=True)
         return dev[:, 1:], dev[:, 0].contiguous()
 
     def append_rows(self, metas: Sequence[PageMeta], rows: torch.Tensor) -> None:
         """Add ``rows[b]`` ((B, n, hidden_dim), the pool's dtype) behind the rows
         of every entry (all different), in pages taken from the pool; least
-        recently used entries that are not listed make room. Raises
+        recently used entries that are neither listed nor edited make room. Raises
         ``RuntimeError``, changing nothing, when the pool cannot hold them."""
         self._check_live(metas, distinct=True)
         dev = L.require_cuda(rows, what="append_rows")
@@ -190,8 +199,7 @@ class StreamingKVCache:
         if row_bytes % 16 != 0:
             raise NotImplementedError("append_rows: rows must be a multiple of 16 bytes")
         need = [max(0, -(-(m.n_events + n) // self.page_size) - len(m.pages)) for m in metas]
-        listed = {m.page_id for m in metas}
-        spare = len(self._free) + sum(len(m.pages) for e, m in self._meta.items() if e not in listed)
+        spare = self._pages_but(self._held | {m.page_id for m in metas})
         if sum(need) > spare:
             raise RuntimeError(f"append_rows: {sum(need)} pages needed, {spare} can be had")
         # what may fail comes before the entries change
@@ -204,8 +212,8 @@ class StreamingKVCache:
                      for m in metas)
         host = torch.empty(n_segs, 3, dtype=torch.int32, pin_memory=True)
         seg = torch.empty(n_segs, 3, dtype=torch.int32, device=self.device)
-        for m in metas:  # most recent: never the ones that make room below
-            self._lru.move_to_end(m.page_id)
+        for m in metas:  # none of them makes room below
+            self._hold(m)
         segs = []
         for b, (m, k) in enumerate(zip(metas, need)):
             m.pages.extend(self._allocate(k))
@@ -216,7 +224,6 @@ class StreamingKVCache:
                 segs.append((b * n + at - m.n_events, m.pages[page] * self.page_size + off, take))
                 at += take
             m.n_events = end
-            m.edited = True
             m.last_used_at = time.monotonic()
         host.copy_(torch.tensor(segs, dtype=torch.int32))
         with torch.cuda.device(self.device):
@@ -246,7 +253,7 @@ class StreamingKVCache:
                 self._free.extend(m.pages[keep:])
                 del m.pages[keep:]
                 m.n_events = budget
-                m.edited = True
+                self._hold(m)
             m.last_used_at = time.monotonic()
 
     def _check_live(self, metas: Sequence[PageMeta], distinct: bool) -> None:
@@ -266,6 +273,21 @@ class StreamingKVCache:
         return self._pool.view(self.num_pages * self.page_size, self.hidden_dim)
 
     # ── internals ────────────────────────────────────────────────────────────
+
+    def _touch(self, eid: int) -> None:
+        if eid in self._lru:
+            self._lru.move_to_end(eid)
+
+    def _hold(self, meta: PageMeta) -> None:
+        """The entry's rows are no longer its window's: they cannot be computed again."""
+        meta.edited = True
+        self._lru.pop(meta.page_id, None)
+        self._held.add(meta.page_id)
+
+    def _pages_but(self, entries: set[int]) -> int:
+        """Pages that do not belong to these entries: free, or to be had by eviction
+        if all edited entries are among them."""
+        return self.num_pages - sum(len(self._meta[e].pages) for e in entries)
 
     def _entry_for(self, session_id: str, bin_start: int, n_pages: int) -> PageMeta:
         key = (session_id, bin_start)
@@ -297,6 +319,7 @@ class StreamingKVCache:
             self._table.pop((meta.session_id, meta.bin_start), None)
             self._free.extend(meta.pages)
         self._lru.pop(eid, None)
+        self._held.discard(eid)
 
 
 __all__ = ["PageMeta", "StreamingKVCache"]

@@ -276,3 +276,58 @@ def test_a_rewritten_key_is_another_entry():
                 cache.page_table([a])
             assert cache.page_table([new])[1].tolist() == [new.n_events]
             assert sorted(cache._free + new.pages) == list(range(8))
+
+
+def test_grown_rows_stay():
+    """Rows that were appended exist nowhere else: nothing that makes room takes them."""
+    cache = StreamingKVCache(6, 4, 16, torch.float32, DEV)
+    a, b = cache.write_rows("a", 0, 4), cache.write_rows("b", 0, 4)
+    rows = torch.arange(32, dtype=torch.float32, device=DEV).reshape(1, 2, 16)
+    cache.append_rows([a], rows)
+    kept = a.pages[1]
+    assert cache.write_rows("c", 0, 16) is not None  # "b" makes room, "a" does not
+    assert cache.is_live(a) and not cache.is_live(b) and cache.pages_used == 6
+    assert cache.write_rows("d", 0, 17) is None and cache.pages_used == 6
+    d = cache.write_rows("d", 0, 12)
+    assert not cache.lookup("c", 0) and cache.is_live(a) and a.n_events == 6
+    with pytest.raises(RuntimeError):  # 5 pages needed, 3 can be had: nothing changes
+        cache.append_rows([a], torch.zeros(1, 20, 16, device=DEV))
+    assert a.n_events == 6 and len(a.pages) == 2 and cache.is_live(d)
+    cache.append_rows([a], torch.zeros(1, 18, 16, device=DEV))
+    assert len(a.pages) == 6 and not cache.is_live(d)
+    assert torch.equal(cache.pool[kept, :2], rows[0])
+    assert cache.write_rows("d", 0, 1) is None  # "a" holds every page
+    with pytest.raises(RuntimeError):
+        cache.write("d", 0, torch.zeros(1, 16, device=DEV))
+    cache.write("a", 0, torch.zeros(1, 16, device=DEV))  # its own key: replaced
+    assert not cache.is_live(a) and cache.pages_used == 1
+    e = cache.write_rows("e", 0, 9)
+    pos = torch.arange(12, dtype=torch.int32, device=DEV)[None].clone()
+    cache.evict_rows([e], torch.rand(1, 12, device=DEV), pos, budget=8)
+    assert cache.write_rows("f", 0, 17) is None and cache.is_live(e)
+    assert cache.evict_session("e") == 1 and cache.write_rows("f", 0, 17) is not None
+
+
+def test_forward_streaming_leaves_edited_entries():
+    from cortex.workloads import WORKLOADS, build_model, make_events
+
+    wl = WORKLOADS["cfg1"]
+    model = build_model(wl, DEV)
+    wins = []
+    for i in range(3):
+        ev = make_events(np.array([200 + i]), seed=7 + i)
+        wins.append({"session_id": f"s{i}", "bin_start": 0, "neuron_ids": ev["neuron_ids"],
+                     "time_bins": ev["time_bins"], "values": ev["values"]})
+    cache = StreamingKVCache(10, 64, 2 * wl.config.latent_dim, torch.bfloat16, DEV)
+    with torch.no_grad():
+        fresh = model.forward_streaming(wins, StreamingKVCache(64, 64, cache.hidden_dim,
+                                                               torch.bfloat16, DEV))["behavior"]
+        model.forward_streaming(wins[:1], cache)
+        meta = cache.lookup("s0", 0)
+        cache.append_rows([meta], torch.randn(1, 9, cache.hidden_dim, device=DEV).bfloat16())
+        held = cache.pool[meta.pages].clone()
+        for _ in range(2):  # 10 pages: "s0" and one of the others
+            assert torch.equal(model.forward_streaming(wins, cache)["behavior"], fresh)
+            assert cache.is_live(meta) and meta.n_events == 209
+            assert torch.equal(cache.pool[meta.pages], held)
+    assert L.device_status()[0] == 0
