@@ -52,6 +52,11 @@ class PageMeta:
     edited: bool = False  # rows appended or evicted since the entry was written
 
 
+def _check_not_capturing(what: str) -> None:
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: the cache's host state cannot be captured into a CUDA graph")
+
+
 class StreamingKVCache:
     """Paged row cache in device memory.
 
@@ -160,6 +165,10 @@ class StreamingKVCache:
         return out
 
     # ── entries that grow and shrink ─────────────────────────────────────────
+    #
+    # The pages and lengths of entries are host metadata, copied to the device by
+    # each call: a captured call would change them once and copy the same ones in
+    # every replay, so these methods refuse to be captured.
 
     @property
     def pool(self) -> torch.Tensor:
@@ -170,6 +179,7 @@ class StreamingKVCache:
         """(page_table (B, pages) int32, lengths (B,) int32) of entries on the
         device, as ``paged_attention`` takes them. The copy is queued on the
         current stream. Entries may be listed more than once."""
+        _check_not_capturing("page_table")
         self._check_live(metas, distinct=False)
         width = max((len(m.pages) for m in metas), default=0)
         host = torch.zeros(len(metas), width + 1, dtype=torch.int32)
@@ -185,6 +195,7 @@ class StreamingKVCache:
         of every entry (all different), in pages taken from the pool; least
         recently used entries that are neither listed nor edited make room. Raises
         ``RuntimeError``, changing nothing, when the pool cannot hold them."""
+        _check_not_capturing("append_rows")
         self._check_live(metas, distinct=True)
         dev = L.require_cuda(rows, what="append_rows")
         if rows.dim() != 3 or rows.shape[0] != len(metas) or rows.shape[2] != self.hidden_dim:
@@ -241,6 +252,7 @@ class StreamingKVCache:
         and the pages behind the budget go back to the pool."""
         from cortex.kernels.kv_evict import evict_by_weight
 
+        _check_not_capturing("evict_rows")
         self._check_live(metas, distinct=True)
         if not metas:
             return

@@ -331,3 +331,26 @@ def test_forward_streaming_leaves_edited_entries():
             assert cache.is_live(meta) and meta.n_events == 209
             assert torch.equal(cache.pool[meta.pages], held)
     assert L.device_status()[0] == 0
+
+
+def test_cache_methods_are_not_captured():
+    """They refuse, nothing changes, and the capture around them goes on."""
+    cache = StreamingKVCache(8, 4, 16, torch.float32, DEV)
+    a = cache.write_rows("a", 0, 3)
+    rows, one = torch.ones(1, 2, 16, device=DEV), torch.ones(1, device=DEV)
+    w, pos = torch.rand(1, 4, device=DEV), torch.zeros(1, 4, dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            for call in (lambda: cache.page_table([a]), lambda: cache.append_rows([a], rows),
+                         lambda: cache.evict_rows([a], w, pos, budget=1)):
+                with pytest.raises(RuntimeError, match="captured"):
+                    call()
+            one.add_(1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert one.tolist() == [2] and a.n_events == 3 and not a.edited and cache.pages_used == 1
+    cache.append_rows([a], rows)
+    assert cache.page_table([a])[1].tolist() == [5]

@@ -174,3 +174,16 @@ def test_a_refused_call_leaves_no_workspace_size():
     L.launch("op", call, query, key, b"", cpu, 0)
     L.launch("op", call, lambda block: 1 / 0, key, b"", cpu, 0)  # remembered: not asked again
     assert seen == [0, 512, 512]
+
+
+def test_cache_methods_refuse_capture(monkeypatch):
+    from cortex.cache import StreamingKVCache
+
+    cache = object.__new__(StreamingKVCache)  # the refusal comes before any of its state
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        cache.page_table([])
+    with pytest.raises(RuntimeError, match="captured"):
+        cache.append_rows([], torch.zeros(0, 1, 8))
+    with pytest.raises(RuntimeError, match="captured"):
+        cache.evict_rows([], torch.zeros(0, 8), torch.zeros(0, 8, dtype=torch.int32), budget=1)
