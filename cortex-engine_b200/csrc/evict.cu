@@ -629,7 +629,9 @@ int evict_by_weight(const ck_evict_args& a, void* ws, size_t ws_bytes, cudaStrea
   if (a.B == 0) return CK_OK;
   EvictParams& p = pl.p;
   if (a.fill && (a.w_out == a.w_in || a.pos_out == a.pos_in)) return CK_ERR_INVALID_ARG;
-  if (!a.lengths || !a.lengths_out || !a.w_in || !a.w_out || !a.pos_in || !a.pos_out)
+  // (tables without a column have no address)
+  if (!a.lengths || !a.lengths_out || (p.cap > 0 && (!a.w_in || !a.pos_in)) ||
+      ((p.cap > 0 || a.fill) && (!a.w_out || !a.pos_out)))
     return CK_ERR_INVALID_ARG;
   if (p.cap > 0 && ((a.num_pages > 0 && !a.pool) || !a.page_table)) return CK_ERR_INVALID_ARG;
   if (pl.bytes > 0 && (ws == nullptr || ws_bytes < pl.bytes ||

@@ -290,3 +290,21 @@ def test_the_largest_budget():
     n, w1, p1 = evict_by_weight(pool, table, lengths, w, pos, budget=2 ** 31 - 1)
     assert n.tolist() == [7] and same(w1[0, :7], w[0, :7]) and same(p1[0, :7], pos[0, :7])
     assert not bool(w1[0, 7:].any()) and int(p1[0, 7:].max()) == int(p1[0, 7:].min()) == -1
+
+
+def test_tables_without_columns():
+    """Sequences without a page: nothing to evict, and lengths other than 0 are bad."""
+    pool, table, lengths, w, pos = make([30, 5], 16, 8, torch.float32)
+    none = (pool, table[:, :0], torch.zeros_like(lengths), w[:, :0], pos[:, :0])
+    before = pool.clone()
+    n, w1, p1 = evict_by_weight(*none, budget=3, recent=1)
+    assert n.tolist() == [0, 0] and w1.tolist() == [[0] * 3] * 2 and p1.tolist() == [[-1] * 3] * 2
+    got = evict_by_weight(*none, budget=3, out=(none[2], none[3], none[4]))
+    assert got[0].tolist() == [0, 0] and got[1].shape == (2, 0)
+    fresh = evict_by_weight(*none, budget=3, out=(torch.ones_like(lengths), w.clone(), pos.clone()))
+    assert fresh[0].tolist() == [0, 0] and same(fresh[1], w) and same(fresh[2], pos)
+    assert L.device_status()[0] == 0
+    n, _, _ = evict_by_weight(pool, table[:, :0], lengths, w[:, :0], pos[:, :0], budget=3)
+    with pytest.raises(IndexError):
+        L.check_device_status("evict_by_weight")
+    assert n.tolist() == lengths.tolist() and same(pool, before)

@@ -187,3 +187,16 @@ def test_cache_methods_refuse_capture(monkeypatch):
         cache.append_rows([], torch.zeros(0, 1, 8))
     with pytest.raises(RuntimeError, match="captured"):
         cache.evict_rows([], torch.zeros(0, 8), torch.zeros(0, 8, dtype=torch.int32), budget=1)
+
+
+def test_evict_tables_without_columns():
+    """No slots: the inputs may be NULL, outputs that are filled may not."""
+    lib = L.load()
+
+    def rc(**kw):
+        none = dict(page_table_width=0, page_table=None, w_in=None, pos_in=None, in_width=0)
+        return lib.ck_evict_by_weight(_evict(**{**none, **kw}), 0, 0, 0)
+
+    assert rc(B=0) == L.CK_OK
+    for missing in ("w_out", "pos_out", "lengths", "lengths_out"):
+        assert rc(**{missing: None}) == L.CK_ERR_INVALID_ARG
