@@ -442,8 +442,9 @@ __global__ void __launch_bounds__(ST, 2) evict_select_kernel(const EvictParams p
 }
 
 // The same through shared memory by bulk copies, a lane issuing its move's: the
-// moves of lanes [first, first + slots), whose rows fill the warp's `room`.
-__device__ __forceinline__ void copy_rows_bulk(const EvictParams& p, int first, int slots, int64_t from,
+// moves of lanes [first, first + slots), whose rows fill the warp's `room`. False
+// when the copies did not come in time (recorded): the barrier is not used again.
+__device__ __forceinline__ bool copy_rows_bulk(const EvictParams& p, int first, int slots, int64_t from,
                                                int64_t to, uint32_t room, uint64_t* bar,
                                                uint32_t& phase) {
   const int lane = threadIdx.x & 31;
@@ -451,7 +452,7 @@ __device__ __forceinline__ void copy_rows_bulk(const EvictParams& p, int first, 
   uint8_t* pool = reinterpret_cast<uint8_t*>(p.a.pool);
   const bool mine = lane >= first && lane < first + slots && from >= 0 && to >= 0;
   const uint32_t rows = __popc(__ballot_sync(0xffffffffu, mine));
-  if (rows == 0u) return;
+  if (rows == 0u) return true;
   if (lane == 0) mbar_arrive_expect_tx(bar, rows * row);
   __syncwarp();
   const uint32_t at = room + (uint32_t)(lane - first) * row;
@@ -460,9 +461,13 @@ __device__ __forceinline__ void copy_rows_bulk(const EvictParams& p, int first, 
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at),
         "l"(pool + from), "r"(row), "r"(smem_u32(bar))
         : "memory");
-  const bool ok = mbar_wait_park(bar, phase, nullptr, 40);
+  const bool ok = __all_sync(0xffffffffu, mbar_wait_park(bar, phase, nullptr, 40));
   phase ^= 1u;
-  if (mine && ok) {
+  if (!ok) {  // no copy may land after this block's exit: the same time for them again
+    mbar_wait_park(bar, phase ^ 1u, nullptr, 41);
+    return false;
+  }
+  if (mine) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(pool + to),
                  "r"(at), "r"(row)
                  : "memory");
@@ -470,6 +475,7 @@ __device__ __forceinline__ void copy_rows_bulk(const EvictParams& p, int first, 
     bulk_wait_read<0>();  // before the next rows come into this place
   }
   __syncwarp();
+  return true;
 }
 
 // Every sequence's moves as one list, an equal share of it to every warp: a
@@ -494,6 +500,7 @@ __global__ void __launch_bounds__(BULK ? 128 : 256) evict_move_kernel(const Evic
   grid_dep_wait();
   grid_dep_launch();
   uint32_t phase = 0;
+  bool ok = true;  // of the warp
   const int slots = BULK ? (int)min((int64_t)32, (int64_t)kBulkRoom / (p.a.width * p.a.elem_bytes)) : 32;  // rows at a time
   for (int b0 = 0; b0 < p.a.B; b0 += kListed) {
     const int n = min(kListed, p.a.B - b0);
@@ -538,8 +545,9 @@ __global__ void __launch_bounds__(BULK ? 128 : 256) evict_move_kernel(const Evic
         start_move(p, b0 + lo, p.holes[at], p.movers[at], from, to);
       }
       if constexpr (BULK) {
-        for (int k = 0; k < cnt; k += slots)
-          copy_rows_bulk(p, k, slots, from, to, smem_u32(s_rows) + warp * kBulkRoom, &s_bar[warp], phase);
+        for (int k = 0; k < cnt && ok; k += slots)
+          ok = copy_rows_bulk(p, k, slots, from, to, smem_u32(s_rows) + warp * kBulkRoom, &s_bar[warp],
+                              phase);
       } else {
         copy_rows_of<V>(p, cnt, from, to);
       }
