@@ -21,6 +21,8 @@
 // The second may therefore read x and W, and write y, before its own wait for
 // the first: only the adapters' part comes after it, so the first launch runs
 // beside the product.
+#include <math_constants.h>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -522,6 +524,12 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
 // unwritten: no block of the GEMM uses it. 8192 x 512, 8 adapters of rank 16: 11 us
 // from cold caches, of which the chain ids, list, first operands, partials, sum is
 // all; its bytes would take 1.5.
+// v for a rounding to bf16 that takes no finite number to infinity
+__device__ __forceinline__ float in_bf16_range(float v) {
+  constexpr float kMax = 3.3895313892515355e38f;  // (2 - 2^-7) 2^127
+  return fabsf(v) < CUDART_INF_F ? fminf(fmaxf(v, -kMax), kMax) : v;
+}
+
 template <int RP, int SK>
 struct TilesCfg {
   static constexpr int SL = 256 / RP;  // one MMA's columns
@@ -711,7 +719,8 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
           v[e] = j0 + c0 + c + e < a.rank ? v[e] * scale : 0.f;
         }
         if (j0 + c0 + c < p.ld_h)
-          *reinterpret_cast<uint32_t*>(p.h + m * p.ld_h + j0 + c0 + c) = cvt_bf16x2(v[0], v[1]);
+          *reinterpret_cast<uint32_t*>(p.h + m * p.ld_h + j0 + c0 + c) =
+              cvt_bf16x2(in_bf16_range(v[0]), in_bf16_range(v[1]));
       }
     }
     // the partials (for the next pass's copies) and the accumulators are free again

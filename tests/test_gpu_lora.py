@@ -339,3 +339,20 @@ def test_bad_ids_of_few_rows(M, rank):
     y = lora_linear(x, w, a[:0], b[:0], none, bias=bias)
     assert torch.equal(y, lora_linear(x, w, a, b, none, scaling=s, bias=bias))
     assert L.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("M", [5, 40, 700])
+def test_adapters_past_the_types_range(M):
+    """h near the end of fp32's range, beyond bf16's largest number, and infinite. Off by
+    2^-8 where h is rounded to bf16 (in the tiles) and 2^-8 in the result."""
+    x, w, a, b, ids, s, bias = make(M, 512, 256, 16, 5, BF)
+    ids[:] = torch.arange(M, device=DEV) % 3
+    x[:, 1:], w[:], a[:, :, 0] = 0, 0, 1.0
+    x[:, 0] = 3.3895e38  # bf16's largest
+    b[:] = 2.0 ** -10
+    s[:3] = torch.tensor([1.0, 1.003, 4.0])  # in range; beyond bf16's, in fp32's; infinite
+    y = lora_linear(x, w, a, b, ids, scaling=s).float().cpu()
+    big = float(x[0, 0]) * 16 * 2.0 ** -10
+    assert bool(((y[0::3] / big - 1).abs() <= 2.0 ** -7).all())
+    assert bool(((y[1::3] / (1.003 * big) - 1).abs() <= 2.0 ** -7).all())
+    assert bool(torch.isposinf(y[2::3]).all())
