@@ -519,7 +519,9 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
 // depth is what the adapters' number leaves, each CTA an SK-th of K. A row then takes the columns of its own
 // adapter; the ranks' partials meet in distributed shared memory, each CTA
 // finishing RP / SK columns: sum in rank order, times s_i, rounded to bf16 for
-// the GEMM's operand. Bound by x, read once a cluster; clusters whose SL the tile
+// the GEMM's operand (2^-8 |B||h| beside the result's own 2^-8 |y|; what the rounding
+// takes as a second operand took 24.1 us against 22.6 at 8192 x 512 x 1536 in runs,
+// 56.5 against 50.1 at 12001 x 768 x 2304, 149 against 119 with 64 adapters by rows). Bound by x, read once a cluster; clusters whose SL the tile
 // has no adapters for leave after the list. h of rows without an adapter stays
 // unwritten: no block of the GEMM uses it. 8192 x 512, 8 adapters of rank 16: 11 us
 // from cold caches, of which the chain ids, list, first operands, partials, sum is

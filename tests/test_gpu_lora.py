@@ -356,3 +356,32 @@ def test_adapters_past_the_types_range(M):
     assert bool(((y[0::3] / big - 1).abs() <= 2.0 ** -7).all())
     assert bool(((y[1::3] / (1.003 * big) - 1).abs() <= 2.0 ** -7).all())
     assert bool(torch.isposinf(y[2::3]).all())
+
+
+@pytest.mark.parametrize("M,K,N,rank,n,pattern,tiles", [
+    (1, 512, 256, 16, 3, "one", False),  # one launch
+    (2, 256, 100, 8, 3, "random", False),
+    (20, 512, 256, 24, 5, "random", False),  # rows, h in a launch before
+    (48, 768, 2304, 16, 64, "random", False),
+    (129, 512, 256, 16, 5, "random", False),
+    (300, 256, 1600, 8, 200, "random", True),  # tiles, rank within 16, 32, 64, beyond
+    (2000, 512, 1536, 16, 8, "runs", True),
+    (300, 256, 768, 32, 50, "random", True),
+    (700, 256, 1600, 20, 3, "runs", True),
+    (777, 768, 1000, 48, 24, "runs", True),
+    (300, 128, 1600, 64, 50, "random", True),
+    (1025, 512, 2048, 128, 7, "runs", True),
+    (513, 264, 520, 200, 3, "random", True),
+    (400, 72, 77, 5, 6, "runs", False),
+    (200, 70, 97, 16, 4, "runs", False),  # rows that TMA does not take
+])
+def test_adapters_are_rounded_in_the_tiles_alone(M, K, N, rank, n, pattern, tiles):
+    """The adapters alone (w = 0, so that nothing hides them): beside the fp32 sums and
+    the result's rounding, an error of 2^-8 |B||h| where the rows go through the
+    tiles, and of nothing elsewhere."""
+    x, w, a, b, ids, s, _ = make(M, K, N, rank, n, BF, seed=4, pattern=pattern)
+    w = torch.zeros_like(w)
+    y, tol, H = want(x, w, a, b, ids, s, None)
+    tol = tol + 2.0 ** -8 * y.abs() + (2.0 ** -8 * H if tiles else 0)
+    err = (lora_linear(x, w, a, b, ids, scaling=s).double().cpu() - y).abs()
+    assert bool((err <= tol).all()), float((err / tol.clamp(min=1e-30)).max())
