@@ -356,3 +356,31 @@ def test_a_valid_call_after_a_refused_one():
     check(out, o, tol)
     check(got, ws, wtol + U * ws)
     assert L.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("lens,H,Hkv,Dh", [
+    ([300], 8, 8, 64), ([900, 17, 0, 256], 4, 4, 64), ([700, 64], 8, 2, 128),
+    ([1000, 5], 3, 3, 32), ([800, 40], 16, 1, 64), ([500], 24, 2, 128), ([400, 33], 4, 2, 96),
+])
+def test_probabilities_keep_sixteen_bits(lens, H, Hkv, Dh):
+    """bf16, flat probabilities, values of both signs: the output is far smaller than
+    A = sum p |v|, so that its own rounding hides nothing. p = p1 + p2 in bf16 is off by
+    2^-8 of p2 at most, which is at most 2^-8 of p: 2^-16 A. Layouts outside the
+    streaming kernel keep p in fp32."""
+    q, pool, table, lengths = make(lens, H, Hkv, Dh, 16, torch.bfloat16, seed=12)
+    q = q * 0.125
+    o, tol, _, _ = want(q, pool, table, lengths)
+    A = want_magnitudes(q, pool, table, lengths)
+    check(paged_attention(q, pool, table, lengths), o, tol - (2.0 ** -8 - 2.0 ** -16) * A)
+    w = torch.zeros(len(lens), table.shape[1] * 16, device=DEV)
+    check(paged_attention(q, pool, table, lengths, weights=w)[0], o,
+          tol - (2.0 ** -8 - 2.0 ** -16) * A)
+
+
+def want_magnitudes(q, pool, table, lengths):
+    """sum_j p_j |v_j| in float64: the output of the same scores over |V|."""
+    Dh = q.shape[2]
+    Hkv = pool.shape[2] // (2 * Dh)
+    mag = pool.clone()
+    mag[:, :, Hkv * Dh:] = mag[:, :, Hkv * Dh:].abs()
+    return want(q, mag, table, lengths)[0]
