@@ -36,10 +36,8 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         out: optional output, (..., N), outside the memory that the inputs span.
 
     Sums are fp32 and the result is rounded once. bf16 calls of many rows (from 33 on,
-    by rows, rank and N; sizes and addresses that TMA takes) also round
-    h = scaling[i] A_i x to bf16 for the product with B_i, an error of at most
-    2^-8 |B_i||h|; float32 calls and bf16 calls of few rows keep it in fp32, so that a
-    bf16 row may differ by that much with the number of rows beside it. An id >= n is recorded in the
+    by rows, rank and N) carry h = scaling[i] A_i x as the sum of two bf16 numbers to the
+    product with B_i, an error of at most 2^-15 |B_i||h|. An id >= n is recorded in the
     device status (IndexError from ``_lib.check_device_status``) and its row gets
     no adapter.
     """

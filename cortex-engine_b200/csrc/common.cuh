@@ -499,6 +499,25 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
+// a and b as sums of two bf16 numbers each, packed: `high` cut off towards 0 (so that no
+// finite number becomes infinite), `low` the rest, off by 2^-15 of the number at most.
+// Both parts of a number have its sign and neither is 0 (but of numbers below 2^-103):
+// 2^-23 of it is added to the rest, so that an infinity times the two parts stays one.
+__device__ __forceinline__ void two_bf16x2(float a, float b, uint32_t& high, uint32_t& low) {
+  high = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+  constexpr float kOneUp = 1.0f + 1.1920928955078125e-7f;  // 1 + 2^-23
+  low = cvt_bf16x2(fmaf(a, kOneUp, -bf16_lo(high)), fmaf(b, kOneUp, -bf16_hi(high)));
+}
+
+// `bytes` contiguous bytes (a multiple of 16, both addresses 16-byte aligned)
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar,
                                             int c0, int c1) {
   asm volatile(

@@ -35,11 +35,14 @@ struct GemmArgs {
   // multiplies each row by 1 / sqrt(sum / K + norm_eps).
   const __nv_bfloat16* rms_gamma;
   // Low-rank adapters (FUSE_LORA): after its K blocks a row tile takes one
-  // block per 64 ranks of every adapter its rows name: A operand h (tmY2), B
+  // block per 64 ranks of every adapter its rows name: A operand h (lora_h), B
   // operand the adapter's (N, rank) matrix (tmR), the other rows' accumulator
   // lanes masked off. lora_cnt[row tile] slots of lora_slots[row tile * lora_max].
   // The blocks' rows are lora_sw = 32, 64 or 128 bytes wide, the least that holds
   // the rank: a tile of mixed rows takes many blocks, and they cost what they hold.
+  // h lies as the operand's shared-memory image (a contiguous copy), for each block the
+  // bf16 value and behind it what the rounding took.
+  const uint8_t* lora_h;
   const int* lora_cnt;
   const uint4* lora_slots;  // two uint4 a slot: (adapter, 0, 0, 0), masked-off lanes
   int lora_max, lora_blocks, lora_sw, lora_rank;

@@ -38,6 +38,7 @@
 
 #include <cstdlib>
 #include <cstring>
+#include <type_traits>
 #include <cudaTypedefs.h>
 
 #include "common.cuh"
@@ -191,10 +192,7 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
     prefetch_tmap(&tmY);
-    if (C::LORA) {
-      prefetch_tmap(&tmY2);
-      prefetch_tmap(&tmR);
-    }
+    if (C::LORA) prefetch_tmap(&tmR);
     if (C::LN) {
       prefetch_tmap(&tmY2);
       if (p.res_tma) prefetch_tmap(&tmR);
@@ -272,10 +270,10 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
   // forward 1.5-2 % slower with the fused LayerNorm, 1 % faster without it).
   if (!C::LN) grid_dep_launch();
   // FUSE_LORA: the adapters (.x) and the rows to leave alone of LOOK slots of a
-  // tile, read ahead. A stage holds h once and B_i of per_stage slots (their rows
-  // are as short as the rank).
+  // tile, read ahead. h comes in two bf16 parts, both of which multiply B_i: 16 bits of
+  // its mantissa. A stage holds both and B_i of 128 / lora_sw slots (their rows are as
+  // short as the rank); at 128 bytes a row two stages hold a part and a slot each.
   constexpr int LOOK = 4;
-  const int per_stage = C::LORA ? 128 / p.lora_sw : 1;
   auto slot_ids = [&](int mt, int s0, int (&ids)[LOOK]) {
 #pragma unroll
     for (int u = 0; u < LOOK; ++u)
@@ -351,35 +349,61 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
             slot_ids(mt, 0, next);
           }
           bool go = true;
-          for (int s0 = 0; s0 < count && go; s0 += LOOK) {
-            int ids[LOOK];
+          // (a loop for each width: these two threads pace the tile)
+          auto load_slots = [&](auto width) {
+            constexpr int SW = decltype(width)::value, PER = SW == 32 ? 4 : 2;
+            constexpr uint32_t PART = BM * SW, H = SW < 128 ? 2 * PART : PART;  // bytes; of a stage's h
+            const uint8_t* h = p.lora_h + (int64_t)mt * p.lora_blocks * 2 * PART;
+            auto open_stage = [&](const uint8_t* from, int slots) {
+              go = mbar_wait_park(&empty[stage], phase ^ 1, abort_flag, 1);
+              if (!go) return false;
+              mbar_arrive_expect_tx(&full[stage], H + (uint32_t)(slots * BN * SW));
+              bulk_load(sA + stage * C::A_BYTES, from, H, &full[stage]);
+              ++issued;
+              return true;
+            };
+            // (rows past the adapter's N are columns that the store drops)
+            auto load_b = [&](int at, int id, int rb) {
+              tma_load_2d(sB + stage * C::B_BYTES + at * BN * SW, &tmR, &full[stage], rb * BK,
+                          id * p.N + nt * BN);
+            };
+            auto next_stage = [&]() {
+              if (++stage == C::STAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
+            };
+            for (int s0 = 0; s0 < count && go; s0 += LOOK) {
+              int ids[LOOK];
 #pragma unroll
-            for (int u = 0; u < LOOK; ++u) ids[u] = next[u];
-            slot_ids(mt, s0 + LOOK, next);
+              for (int u = 0; u < LOOK; ++u) ids[u] = next[u];
+              slot_ids(mt, s0 + LOOK, next);
 #pragma unroll
-            for (int u = 0; u < LOOK; ++u) {
-              const int at = u & (per_stage - 1);
-              const int left = min(per_stage, count - s0 - u);  // (at == 0) slots of the stage
-              for (int rb = 0; rb < p.lora_blocks && left > 0 && go; ++rb) {
-                if (at == 0) {
-                  go = mbar_wait_park(&empty[stage], phase ^ 1, abort_flag, 1);
-                  if (!go) break;
-                  mbar_arrive_expect_tx(&full[stage], (uint32_t)((BM + left * BN) * p.lora_sw));
-                  tma_load_2d(sA + stage * C::A_BYTES, &tmY2, &full[stage], rb * BK, mt * BM);
-                  ++issued;
-                }
-                // (rows past the adapter's N are columns that the store drops)
-                tma_load_2d(sB + stage * C::B_BYTES + at * BN * p.lora_sw, &tmR, &full[stage],
-                            rb * BK, ids[u] * p.N + nt * BN);
-                if (at == per_stage - 1 || left == 1) {
-                  if (++stage == C::STAGES) {
-                    stage = 0;
-                    phase ^= 1;
+              for (int u = 0; u < LOOK; u += PER) {
+                const int left = min(PER, count - s0 - u);
+                if constexpr (SW < 128) {
+                  if (left <= 0 || !open_stage(h, left)) break;
+#pragma unroll
+                  for (int at = 0; at < PER; ++at)
+                    if (at < left) load_b(at, ids[u + at], 0);
+                  next_stage();
+                } else {
+                  for (int rb = 0; rb < p.lora_blocks && left > 0; ++rb) {
+                    if (!open_stage(h + rb * 2 * PART, 1)) break;
+                    load_b(0, ids[u], rb);
+                    next_stage();
+                    if (!open_stage(h + rb * 2 * PART + PART, left - 1)) break;
+                    if (left > 1) load_b(0, ids[u + 1], rb);
+                    next_stage();
                   }
+                  if (!go) break;
                 }
               }
             }
-          }
+          };
+          if (p.lora_sw == 32) load_slots(std::integral_constant<int, 32>{});
+          else if (p.lora_sw == 64) load_slots(std::integral_constant<int, 64>{});
+          else load_slots(std::integral_constant<int, 128>{});
         }
       }
       // Drain: make sure every issued copy has landed before the CTA can exit
@@ -446,38 +470,58 @@ __global__ void __launch_bounds__(GemmCfg<BN, WMODE, FUSE, EPI, PAIR>::NUM_THREA
             count = p.lora_cnt[mt_];
             slot_masks(mt_, 0, next);
           }
-          for (int s0 = 0; s0 < count && ok; s0 += LOOK) {
-            uint4 off[LOOK];
+          auto multiply_slots = [&](auto width) {
+            constexpr int SW = decltype(width)::value, PER = SW == 32 ? 4 : 2;
+            const uint64_t desc0 = sw_desc(0u, SW);
+            auto next_stage = [&]() {
+              tc_commit(&empty[stage]);
+              if (++stage == C::STAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
+            };
+            for (int s0 = 0; s0 < count && ok; s0 += LOOK) {
+              uint4 off[LOOK];
 #pragma unroll
-            for (int u = 0; u < LOOK; ++u) off[u] = next[u];
-            slot_masks(mt_, s0 + LOOK, next);
+              for (int u = 0; u < LOOK; ++u) off[u] = next[u];
+              slot_masks(mt_, s0 + LOOK, next);
 #pragma unroll
-            for (int u = 0; u < LOOK; ++u) {
-              const int at = u & (per_stage - 1);
-              const int left = min(per_stage, count - s0 - u);
-              for (int rb = 0; rb < p.lora_blocks && left > 0 && ok; ++rb) {
-                if (at == 0) {
+              for (int u = 0; u < LOOK; u += PER) {
+                const int left = min(PER, count - s0 - u);
+                for (int rb = 0; rb < (SW < 128 ? 1 : p.lora_blocks) && left > 0 && ok; ++rb) {
+                  const int behind = stage + 1 == C::STAGES ? 0 : stage + 1;
                   ok = mbar_wait(&full[stage], phase, abort_flag, 3);
+                  if (ok && SW == 128)
+                    ok = mbar_wait(&full[behind], behind == 0 ? phase ^ 1 : phase, abort_flag, 3);
                   if (!ok) break;
                   tc_fence_after();
-                }
-                const uint32_t a_addr = smem_u32(sA + stage * C::A_BYTES);
-                const uint32_t b_addr = smem_u32(sB + stage * C::B_BYTES) + at * BN * p.lora_sw;
-                const int ranks = p.lora_rank - rb * BK;  // of this block and behind
-                const int steps = ranks >= BK ? BK / 16 : (ranks + 15) / 16;
-                for (int k = 0; k < steps; ++k)
-                  tc_mma_ss_masked(d_tmem, sw_desc(a_addr + k * 32, (uint32_t)p.lora_sw),
-                                   sw_desc(b_addr + k * 32, (uint32_t)p.lora_sw), idesc, 1u, off[u]);
-                if (at == per_stage - 1 || left == 1) {
-                  tc_commit(&empty[stage]);
-                  if (++stage == C::STAGES) {
-                    stage = 0;
-                    phase ^= 1;
-                  }
+                  // 16 ranks a step (32 bytes: 2 in a descriptor), for both parts of h
+                  const uint64_t high = desc0 | (smem_u32(sA + stage * C::A_BYTES) >> 4);
+                  const uint64_t low =
+                      SW < 128 ? high + BM * SW / 16 : desc0 | (smem_u32(sA + behind * C::A_BYTES) >> 4);
+                  const uint64_t b0 = desc0 | (smem_u32(sB + stage * C::B_BYTES) >> 4);
+                  const uint64_t b1 = SW < 128 ? 0 : desc0 | (smem_u32(sB + behind * C::B_BYTES) >> 4);
+                  const int steps = SW < 128 ? SW / 32 : (p.lora_rank - rb * BK + 15) / 16;
+#pragma unroll
+                  for (int at = 0; at < PER; ++at)
+                    if (at < left) {
+                      const uint64_t b_desc = SW < 128 ? b0 + at * BN * SW / 16 : (at == 0 ? b0 : b1);
+#pragma unroll
+                      for (int k = 0; k < SW / 32; ++k)
+                        if (SW < 128 || k < steps) {
+                          tc_mma_ss_masked(d_tmem, high + 2 * k, b_desc + 2 * k, idesc, 1u, off[u + at]);
+                          tc_mma_ss_masked(d_tmem, low + 2 * k, b_desc + 2 * k, idesc, 1u, off[u + at]);
+                        }
+                    }
+                  next_stage();
+                  if (SW == 128) next_stage();
                 }
               }
             }
-          }
+          };
+          if (p.lora_sw == 32) multiply_slots(std::integral_constant<int, 32>{});
+          else if (p.lora_sw == 64) multiply_slots(std::integral_constant<int, 64>{});
+          else multiply_slots(std::integral_constant<int, 128>{});
         }
         if (!ok) break;
         if (PAIR)
@@ -1122,6 +1166,7 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
   a.ln_beta = nullptr;
   a.res_tma = 0;
   a.pre_b = (fz != nullptr && fz->w_static) ? 1 : 0;
+  a.lora_h = nullptr;
   a.lora_cnt = nullptr;
   a.lora_slots = nullptr;
   a.lora_max = a.lora_blocks = a.lora_sw = a.lora_rank = 0;
@@ -1135,6 +1180,7 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
     a.lora_blocks = (fz->lora_rank + BK - 1) / BK;
     a.lora_rank = fz->lora_rank;
     a.lora_sw = fz->lora_rank <= 16 ? 32 : (fz->lora_rank <= 32 ? 64 : 128);
+    a.lora_h = reinterpret_cast<const uint8_t*>(fz->lora_h);
     fuse = gemm::FUSE_LORA;
   } else if (fz != nullptr && fz->ln_out != nullptr) {
     // LayerNorm of the residual output as a second output: whole rows of
@@ -1194,10 +1240,6 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
   if (ln) {
     if (!make_tmap_2d(&ty2, fz->ln_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, N, M, fz->ln_ld, 64,
                       32, 128))
-      return CK_ERR_INVALID_ARG;
-  } else if (lora) {
-    if (!make_tmap_2d(&ty2, fz->lora_h, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, fz->lora_h_ld, M,
-                      fz->lora_h_ld, a.lora_sw / 2, BM, a.lora_sw))
       return CK_ERR_INVALID_ARG;
   } else {
     ty2 = ty;

@@ -80,13 +80,15 @@ struct GemmFusion {
   // aligned, store or bias epilogue): y = epi((x * gamma) W^T / sqrt(mean_k(x^2) + eps))
   const void* rms_gamma = nullptr;
   // Low-rank adapters (lora.cu): y += B_i h for the adapter i of each row. h
-  // (M, lora_h_ld) bf16, lora_h_ld = rank rounded up to 8, zero behind rank;
+  // bf16, zero behind the rank: for each 128-row tile and 64 ranks 128 rows of 16, 32 or 64
+  // columns (the least that holds the rank), their 16-byte pieces permuted as the
+  // swizzle of that width does, then as many rows with what the rounding took from these;
   // lora_b (n * N, rank) with row stride lora_b_ld (a multiple of 8); per 128-row tile lora_cnt slots of
   // two uint4 (adapter; rows that are not its own). Store or bias epilogue, one
   // rounding.
   const void* lora_h = nullptr;
   const void* lora_b = nullptr;
-  int64_t lora_b_ld = 0, lora_h_ld = 0;
+  int64_t lora_b_ld = 0;
   int32_t lora_n = 0, lora_rank = 0, lora_max = 0;
   const int32_t* lora_cnt = nullptr;
   const void* lora_slots = nullptr;

@@ -13,7 +13,7 @@
 //     MMAs and the rows of x as its narrow one, K split over a cluster (a row or
 //     two: h in the same launch);
 //   * many rows (bf16): gemm_tc.cu's tiles with the adapters as further K
-//     blocks (h rounded to bf16, rows of other adapters masked off);
+//     blocks (h as the sum of two bf16 parts, rows of other adapters masked off);
 //   * fp32: lora_gemv_kernel (few rows) and lora_sgemm_kernel, on the CUDA cores;
 //   * bf16 layouts that TMA does not take: lora_simt_kernel.
 // Order of the launches: a kernel of the first kind waits for all earlier work
@@ -35,11 +35,10 @@ struct LoraParams {
   float* h;  // [M][rank]
 };
 
-// tensor-core path: h as bf16 rows and the adapters of every 128-row tile
+// tensor-core path: h as the GEMM's operand and the adapters of every 128-row tile
 struct TileParams {
   ck_lora_args a;
-  __nv_bfloat16* h;   // [M][ld_h], ld_h = rank rounded up to 8, zero behind rank
-  int32_t ld_h;
+  uint8_t* h;         // [tiles][blocks of 64 ranks][parts][128 rows] (kernels.h)
   int32_t max_slots;  // per tile
   int32_t tiles;
   int32_t* cnt;       // [tiles]
@@ -518,18 +517,21 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
 // one MMA's columns: both operands by TMA into a ring of 64-wide K blocks whose
 // depth is what the adapters' number leaves, each CTA an SK-th of K. A row then takes the columns of its own
 // adapter; the ranks' partials meet in distributed shared memory, each CTA
-// finishing RP / SK columns: sum in rank order, times s_i, rounded to bf16 for
-// the GEMM's operand (2^-8 |B||h| beside the result's own 2^-8 |y|; what the rounding
-// takes as a second operand took 24.1 us against 22.6 at 8192 x 512 x 1536 in runs,
-// 56.5 against 50.1 at 12001 x 768 x 2304, 149 against 119 with 64 adapters by rows). Bound by x, read once a cluster; clusters whose SL the tile
-// has no adapters for leave after the list. h of rows without an adapter stays
+// finishing RP / SK columns: sum in rank order, times s_i, as two bf16 parts, each
+// written as the GEMM's operand lies in shared memory. (The first alone leaves 2^-8
+// |B||h|, as large as the result's own rounding; captured, us, with and without the
+// second: 8192 x 512 x 1536 in runs 22.0 / 21.6, 12001 x 768 x 2304 49.0 / 47.9, 64
+// adapters by rows 80.7 / 78.8.) Bound by x, read once a cluster; clusters whose SL the
+// tile has no adapters for leave after the list. h of rows without an adapter stays
 // unwritten: no block of the GEMM uses it. 8192 x 512, 8 adapters of rank 16: 11 us
 // from cold caches, of which the chain ids, list, first operands, partials, sum is
 // all; its bytes would take 1.5.
-// v for a rounding to bf16 that takes no finite number to infinity
-__device__ __forceinline__ float in_bf16_range(float v) {
-  constexpr float kMax = 3.3895313892515355e38f;  // (2 - 2^-7) 2^127
-  return fabsf(v) < CUDART_INF_F ? fminf(fmaxf(v, -kMax), kMax) : v;
+// N words (1, 2 or 4), aligned as one
+template <int N>
+__device__ __forceinline__ void store_words(void* to, const uint32_t* w) {
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(to) = w[0];
 }
 
 template <int RP, int SK>
@@ -703,26 +705,37 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
       uint32_t src[SK];
 #pragma unroll
       for (int r = 0; r < SK; ++r) src[r] = SK > 1 ? cl_map(part + tid, r) : smem_u32(part + tid);
+      constexpr int W = PER < 8 ? PER : 8;  // columns a store (16 bytes where there are 8)
+      constexpr int ROW = 2 * RP;
+      auto swizzled = [](int at) { return at ^ (((at >> 7) & (ROW / 16 - 1)) << 4); };
+      uint8_t* to = p.h + ((int64_t)tile * ((a.rank + 63) / 64) + pass) * 2 * 128 * ROW;
 #pragma unroll
-      for (int c = 0; c < PER; c += 2) {
-        float v[2];
+      for (int c = 0; c < PER; c += W) {
+        uint32_t high[W / 2], low[W / 2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          v[e] = 0.f;
+        for (int e = 0; e < W; e += 2) {
+          float v[2];
 #pragma unroll
-          for (int r = 0; r < SK; ++r) {
-            float f;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                         : "=f"(f)
-                         : "r"(src[r] + (c0 + c + e) * 512)
-                         : "memory");
-            v[e] += f;
+          for (int i = 0; i < 2; ++i) {
+            v[i] = 0.f;
+#pragma unroll
+            for (int r = 0; r < SK; ++r) {
+              float f;
+              asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                           : "=f"(f)
+                           : "r"(src[r] + (c0 + c + e + i) * 512)
+                           : "memory");
+              v[i] += f;
+            }
+            v[i] = j0 + c0 + c + e + i < a.rank ? v[i] * scale : 0.f;
           }
-          v[e] = j0 + c0 + c + e < a.rank ? v[e] * scale : 0.f;
+          two_bf16x2(v[0], v[1], high[e / 2], low[e / 2]);
+          if (fabsf(v[0]) == CUDART_INF_F) low[e / 2] = (low[e / 2] & 0xffff0000u) | (high[e / 2] & 0xffffu);
+          if (fabsf(v[1]) == CUDART_INF_F) low[e / 2] = (low[e / 2] & 0xffffu) | (high[e / 2] & 0xffff0000u);
         }
-        if (j0 + c0 + c < p.ld_h)
-          *reinterpret_cast<uint32_t*>(p.h + m * p.ld_h + j0 + c0 + c) =
-              cvt_bf16x2(in_bf16_range(v[0]), in_bf16_range(v[1]));
+        const int at = tid * ROW + (c0 + c) * 2;
+        store_words<W / 2>(to + swizzled(at), high);
+        store_words<W / 2>(to + 128 * ROW + swizzled(at), low);
       }
     }
     // the partials (for the next pass's copies) and the accumulators are free again
@@ -1054,7 +1067,7 @@ struct LoraPlan {
   LoraParams p;
   Path path;
   bool one;                       // PATH_ROWS: one launch, no workspace
-  int ld_h, max_slots, tiles;     // PATH_TILES
+  int max_slots, tiles;           // PATH_TILES
   int64_t ld_b, ld_stage;         // packed B / staged y row strides, 0: used in place
   size_t off_h, off_cnt, off_slots, off_b, off_y;
   size_t bytes;
@@ -1099,13 +1112,13 @@ int make_plan(const ck_lora_args& a, LoraPlan& pl) {
     pl.bytes = pl.one ? 0 : up((size_t)a.M * a.rank * 4);
     return CK_OK;
   }
-  pl.ld_h = (a.rank + 7) / 8 * 8;
   pl.tiles = (int)((a.M + 127) / 128);
   pl.max_slots = a.n_adapters < 1 ? 1 : (a.n_adapters < 128 ? a.n_adapters : 128);
   pl.ld_b = a.rank % 8 == 0 ? 0 : (a.rank + 7) / 8 * 8;
   pl.ld_stage = a.ldy % 8 == 0 && aligned16(a.y) ? 0 : (a.N + 7) / 8 * 8;
   pl.off_h = 0;
-  pl.off_cnt = up((size_t)a.M * pl.ld_h * 2);
+  // h: a tile's 128 rows of 16, 32 or 64 columns a block, twice
+  pl.off_cnt = (size_t)pl.tiles * ((a.rank + 63) / 64) * 2 * 128 * (a.rank <= 16 ? 32 : a.rank <= 32 ? 64 : 128);
   pl.off_slots = pl.off_cnt + up((size_t)pl.tiles * 4);
   pl.off_b = pl.off_slots + up((size_t)pl.tiles * pl.max_slots * 32);
   pl.off_y = pl.off_b + up((size_t)a.n_adapters * a.N * pl.ld_b * 2);
@@ -1290,8 +1303,7 @@ int run_tiles(const LoraPlan& pl, uint8_t* ws, cudaStream_t st) {
   }
   TileParams t;
   t.a = a;
-  t.h = reinterpret_cast<__nv_bfloat16*>(ws + pl.off_h);
-  t.ld_h = pl.ld_h;
+  t.h = ws + pl.off_h;
   t.max_slots = pl.max_slots;
   t.tiles = pl.tiles;
   t.cnt = reinterpret_cast<int32_t*>(ws + pl.off_cnt);
@@ -1307,7 +1319,6 @@ int run_tiles(const LoraPlan& pl, uint8_t* ws, cudaStream_t st) {
   fz.lora_n = a.n_adapters > 0 ? a.n_adapters : 1;
   fz.lora_b_ld = pl.ld_b > 0 ? pl.ld_b : a.rank;
   fz.lora_rank = a.rank;
-  fz.lora_h_ld = t.ld_h;
   fz.lora_max = pl.max_slots;
   fz.lora_cnt = t.cnt;
   fz.lora_slots = t.slots;

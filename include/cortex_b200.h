@@ -472,9 +472,8 @@ int ck_evict_by_weight(const ck_evict_args* args, void* workspace, size_t worksp
  *   y[m] = W x[m] + scaling[i] B_i (A_i x[m]) + bias,  i = ids[m], none for ids[m] < 0
  * x (M, K), w (N, K), a (n_adapters, rank, K) and b (n_adapters, N, rank) without
  * gaps, y (M, N); fp32 or bf16, scaling fp32 or NULL (1), bias (N,) of dtype or
- * NULL. Sums in fp32, one rounding of y; bf16 calls of many rows also round
- * h = s A x to bf16 for the product with B (2^-8 |B||h| at most), fp32 calls and
- * bf16 calls of few rows do not. An id >= n_adapters records CK_ERR_INDEX and
+ * NULL. Sums in fp32, one rounding of y; bf16 calls of many rows carry h = s A x as
+ * two bf16 parts to the product with B (2^-15 |B||h| at most). An id >= n_adapters records CK_ERR_INDEX and
  * counts as none. rank <= 256. y may not overlap an input. */
 typedef struct ck_lora_args {
   int dtype;
