@@ -204,7 +204,8 @@ struct Heads;
 // bf16: 16 positions at a time are the M side of mma.m16n8k16, the heads (8 NT) its
 // N side: S^T[16 x 8] = K[16 x Dh] Q^T, O^T[Dh x 8] += V^T[Dh x 16] P^T[16 x 8].
 // P goes from S^T's accumulator layout to the B operand by an 8 x 8 transpose
-// (movmatrix) as the sum of two bf16 numbers, the second what the first lost: one
+// (movmatrix) as the sum of two bf16 numbers of the same sign, so that an infinite value
+// stays one, the second what the first lost: one
 // alone leaves an error of 2^-8 sum p |v|, as large as the result's own rounding. The
 // tensor pipe has the room (captured, us, with and without the second: 8 sequences of 8000
 // to 32000 positions, 12 heads of 64, 78.5 / 79.1; 32 of 32 to 4096 with weights 29.9 /
@@ -330,11 +331,14 @@ struct Heads<__nv_bfloat16, DH, GT> {
         const float p2 = ex2(s[u][nt][2] - ref0), p3 = ex2(s[u][nt][3] - ref1);
         l[nt][0] += p0 + p2;
         l[nt][1] += p1 + p3;
-        const uint32_t h0 = cvt_bf16x2(p0, p1), h1 = cvt_bf16x2(p2, p3);
-        ph[u][nt][0] = transpose8x8(h0);
-        ph[u][nt][1] = transpose8x8(h1);
-        pl[u][nt][0] = transpose8x8(cvt_bf16x2(p0 - bf16_lo(h0), p1 - bf16_hi(h0)));
-        pl[u][nt][1] = transpose8x8(cvt_bf16x2(p2 - bf16_lo(h1), p3 - bf16_hi(h1)));
+        uint32_t high[2], low[2];
+        two_bf16x2(p0, p1, high[0], low[0]);
+        two_bf16x2(p2, p3, high[1], low[1]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          ph[u][nt][r] = transpose8x8(high[r]);
+          pl[u][nt][r] = transpose8x8(low[r]);
+        }
       }
     }
     // V^T tiles: matrices of positions 0-7 in pieces 2i, 2i + 1, then 8-15

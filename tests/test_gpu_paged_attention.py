@@ -364,17 +364,17 @@ def test_a_valid_call_after_a_refused_one():
 ])
 def test_probabilities_keep_sixteen_bits(lens, H, Hkv, Dh):
     """bf16, flat probabilities, values of both signs: the output is far smaller than
-    A = sum p |v|, so that its own rounding hides nothing. p = p1 + p2 in bf16 is off by
-    2^-8 of p2 at most, which is at most 2^-8 of p: 2^-16 A. Layouts outside the
-    streaming kernel keep p in fp32."""
+    A = sum p |v|, so that its own rounding hides nothing. p = p1 + p2 in bf16, p1 cut off
+    after 8 bits: off by 2^-8 of p2 < 2^-7 p, and 2^-23 p added, (2^-15 + 2^-23) A. Layouts
+    outside the streaming kernel keep p in fp32."""
     q, pool, table, lengths = make(lens, H, Hkv, Dh, 16, torch.bfloat16, seed=12)
     q = q * 0.125
     o, tol, _, _ = want(q, pool, table, lengths)
     A = want_magnitudes(q, pool, table, lengths)
-    check(paged_attention(q, pool, table, lengths), o, tol - (2.0 ** -8 - 2.0 ** -16) * A)
+    check(paged_attention(q, pool, table, lengths), o, tol - (2.0 ** -8 - 2.0 ** -15 - 2.0 ** -23) * A)
     w = torch.zeros(len(lens), table.shape[1] * 16, device=DEV)
     check(paged_attention(q, pool, table, lengths, weights=w)[0], o,
-          tol - (2.0 ** -8 - 2.0 ** -16) * A)
+          tol - (2.0 ** -8 - 2.0 ** -15 - 2.0 ** -23) * A)
 
 
 def want_magnitudes(q, pool, table, lengths):
@@ -384,3 +384,18 @@ def want_magnitudes(q, pool, table, lengths):
     mag = pool.clone()
     mag[:, :, Hkv * Dh:] = mag[:, :, Hkv * Dh:].abs()
     return want(q, mag, table, lengths)[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("Dh,H,Hkv", [(32, 3, 3), (64, 16, 1), (128, 4, 2), (96, 2, 2)])
+def test_infinite_values_that_are_alive(dtype, Dh, H, Hkv):
+    """An infinite element of V makes its column infinite, not NaN, at any probability."""
+    q, pool, table, lengths = make([300, 40, 7], H, Hkv, Dh, 16, dtype, seed=5, nan=False)
+    q = q * 0.25  # (no probability vanishes)
+    for b, j, d, value in ((0, 0, 1, float("inf")), (0, 131, Dh - 1, -float("inf")),
+                           (1, 39, 0, -float("inf")), (2, 3, 5, float("inf"))):
+        pool[table[b, j // 16], j % 16, Hkv * Dh + d] = value  # head 0 of the K|V heads
+        got = paged_attention(q, pool, table, lengths)[b, :H // Hkv]
+        assert bool((got[:, d] == value).all())
+    got = paged_attention(q, pool, table, lengths)
+    assert int((~torch.isfinite(got)).sum()) == 4 * (H // Hkv) and not bool(torch.isnan(got).any())
