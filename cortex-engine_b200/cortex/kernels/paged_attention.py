@@ -69,7 +69,8 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
         out, weights_out: optional outputs, outside the memory that the inputs
             span; only ``weights_out`` may be ``weights`` itself (in place).
 
-    With weights the workspace holds every score, 4 bytes a head and slot.
+    With weights the workspace holds every score, 4 bytes a head and slot of the table,
+    whatever the lengths (268 MB at 64 sequences of 32 heads and 32768 slots).
 
     A page outside the pool (its rows count as absent) or a length outside
     [0, pages * page_size] (clamped) is recorded in the device status

@@ -18,9 +18,9 @@
 // weights and positions, a warp a row.
 //
 // Bytes: weights and positions once (8 B a slot), a row read and written a mover.
-// Measured: 32 sequences, one row too many each, 8.3 us a call; 24 sequences of 700
+// Measured (captured): 32 sequences, one row too many each, 8.1 us a call; 24 sequences of 700
 // to 16384 slots down to 1000, rows of 3 KB, 34 us, of which 18 select and the rest
-// moves 88 MB; one sequence of 131072 slots 38 us (26 select). The selection is bound
+// moves 88 MB; one sequence of 131072 slots 39 us (26 select). The selection is bound
 // by its barriers, the moves by the chain of index, page and row.
 #include <atomic>
 

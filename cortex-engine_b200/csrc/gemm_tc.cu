@@ -1141,9 +1141,9 @@ int gemm_tc(const void* A, int64_t M, int64_t K, int64_t lda, const void* W, int
             const GemmFusion* fz) {
   const bool lora = fz != nullptr && fz->lora_h != nullptr;
   int BN = gemm_tc_block_n(N);
-  // adapters: 128-wide tiles while 256-wide ones are few. 128 / 256, us a call: 1024
-  // x 512 x 1536 (48 wide tiles) 11.5 / 11.9, 4096 x 512 x 512 (64) 14.2 / 12.6, 2000 x
-  // 768 x 2304 (144) 20.8 / 16.7
+  // adapters: 128-wide tiles while 256-wide ones are few. 128 / 256, us a call
+  // (captured): 1024 x 512 x 1536 (48 wide tiles) 10.4 / 11.1, 4096 x 512 x 512 (64) 13.8 /
+  // 12.2, 2000 x 768 x 2304 (144) 19.9 / 16.1
   if (lora && ((M + BM - 1) / BM) * ((N + 255) / 256) <= 48) BN = 128;
   GemmArgs a;
   a.M = (int)M;

@@ -158,7 +158,7 @@ __device__ __forceinline__ float adapter_part(const LoraParams& p, int id, int64
 }
 
 // Up to MR rows of x at a time: a warp a row of W, read once for them; bound by W
-// (2 x 4096 x 4096 36 us a call, 67 MB at 1.9 TB/s; 1 x 512 x 1536 6 us).
+// (2 x 4096 x 4096 36 us a call, captured, 67 MB at 1.9 TB/s; 1 x 512 x 1536 4.1 us).
 template <int MR, bool VEC>
 __global__ void __launch_bounds__(256) lora_gemv_kernel(const LoraParams p) {
   grid_dep_wait();
@@ -224,7 +224,8 @@ __global__ void __launch_bounds__(256) lora_gemv_kernel(const LoraParams p) {
 // in a row instead of K. Where the tiles leave SMs idle, the SK CTAs of a cluster
 // share one: each takes a part of K and every SK-th adapter, and finishes TM / SK
 // rows from the partial tiles in distributed shared memory, in rank order. Bound
-// by the FMA pipe: 1266 x 4096 x 4096 1188 us, 36 TF/s; 301 x 256 x 768 13 us a call.
+// by the FMA pipe: 1266 x 4096 x 4096 1207 us, 35 TF/s; 301 x 256 x 768 12.7 us a call
+// (captured).
 template <int MT, int WM, int WN, int SK, bool VEC>
 __global__ void __launch_bounds__(32 * WM * WN, 3)
     lora_sgemm_kernel(const LoraParams p, int n_tiles) {
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(32 * WM * WN, 3)
 
 // bf16 whose strides break TMA's 16-byte rules: 64 x 64 tiles, 4 x 4 a thread,
 // the next K slice in registers while this one is multiplied. Not made for speed:
-// 2000 x 510 x 1536 248 us, where 2000 x 512 x 1536 takes 15 by the tiles.
+// 2000 x 510 x 1536 229 us, where 2000 x 512 x 1536 takes 12 by the tiles (captured).
 __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int n_tiles) {
   using T = __nv_bfloat16;
   constexpr int TM = 64, TN = 64, TK = 16;
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(256) lora_simt_kernel(const LoraParams p, int 
 // second: 8192 x 512 x 1536 in runs 22.0 / 21.6, 12001 x 768 x 2304 49.0 / 47.9, 64
 // adapters by rows 80.7 / 78.8.) Bound by x, read once a cluster; clusters whose SL the
 // tile has no adapters for leave after the list. h of rows without an adapter stays
-// unwritten: no block of the GEMM uses it. 8192 x 512, 8 adapters of rank 16: 11 us
+// unwritten: no block of the GEMM uses it. 8192 x 512, 8 adapters of rank 16: 10.2 us
 // from cold caches, of which the chain ids, list, first operands, partials, sum is
 // all; its bytes would take 1.5.
 // N words (1, 2 or 4), aligned as one
@@ -747,8 +748,8 @@ __global__ void __launch_bounds__(128) lora_tiles_kernel(const __grid_constant__
 }
 
 // Row copies with a change of stride: B rows padded to 16-byte rows (rank not
-// a multiple of 8; 2000 x 512 x 1536 of rank 12 19 us against 15 of rank 16), and y
-// out of the padded staging rows (N or ldy not one; 27 us at N 1535).
+// a multiple of 8; 2000 x 512 x 1536 of rank 12 16 us against 12 of rank 16), and y
+// out of the padded staging rows (N or ldy not one; 24 us at N 1535).
 __global__ void __launch_bounds__(256) lora_copy_kernel(const __nv_bfloat16* src, int64_t ld_src,
                                                         __nv_bfloat16* dst, int64_t ld_dst,
                                                         int64_t rows, int64_t cols) {
@@ -770,7 +771,7 @@ __global__ void __launch_bounds__(256) lora_copy_kernel(const __nv_bfloat16* src
 // SMs; they exchange their fp32 partials through distributed shared memory,
 // each finishing NTOK / SK of the rows: sum over the ranks in order, adapter
 // and bias added, one rounding, a warp storing 32 neighbouring columns. 48 rows,
-// K = N = 4096: 18 us a call, W at 1.9 TB/s.
+// K = N = 4096: 18 us a call (captured), W at 1.9 TB/s.
 //
 // ONE: no first launch. Each CTA computes its K part of every row's h = A_i x in
 // the two warps that have nothing else to do, and the parts meet as the others
@@ -789,9 +790,9 @@ struct RowsCfg {
 };
 
 // Values of h (M rank) that lora_rows_kernel computes itself: as many as its two
-// warps hold at once. One launch against two, us a call in a captured sequence of
-// them: 1 x 512 x 1536, rank 16, 4.7 / 5.0; 1 x 4096 x 4096, rank 32, 11.8 / 12.4; 2 x
-// 1024 x 256, rank 16, 5.2 / 5.5; with 64 values 4 x 512 x 1536, rank 16, 5.9 / 5.4.
+// warps hold at once. One launch against two, us a call: 1 x 512 x 1536, rank 16, eager
+// 13.1 / 17.6, captured 4.65 / 4.83; captured 1 x 4096 x 4096, rank 32, 10.5 / 10.1; with 64
+// values 4 x 512 x 1536, rank 16, 5.7 / 5.2.
 constexpr int kOneH = 32;
 
 template <int NTOK, int SK, bool ONE>
@@ -1077,15 +1078,15 @@ bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) ==
 
 // Whether lora_rows_kernel runs: its epilogue reads h and B_i once a row, where
 // the tiles multiply B_i once for all rows that name it but take a block for each
-// adapter of a tile. Measured (us, rows against tiles; adapters all different /
-// in runs of 64 rows): 4 x 512 x 1536, rank 32, 12.3 / 12.3 against 16.4 / 14.3;
-// 32 x 768 x 2304, rank 64, 22.5 / 20.5 against 28.7 / 16.4; 64 x 768 x 2304,
-// rank 32, 22.5 / 20.5 against 49.2 / 16.4, rank 64, 30.7 / 30.7 against 28.7 / 18.4.
-// More rows than one operand of 64, only while all of them are few CTAs: 128 x
-// 512 x 1536 (24 tiles of W by rows), rank 8, 16.4 / 16.4 against 26.6 / 18.4; 256
-// x 4096 x 1024 (32), rank 32, 32.8 / 30.8 against 75.8 / 34.8; 192 x 512 x 1536
-// (36), 8 adapters of rank 16, 26.6 against 22.5. 512 x 512 x 512, rank 32, 28.7 /
-// 28.7 against 55.3 / 20.4: more than 8192 values of h are left to the tiles.
+// adapter of a tile. Measured (captured, us, rows against tiles; adapters all
+// different, then in runs of 64 rows): 4 x 512 x 1536, rank 32, 6.0 against 9.2; 32 x
+// 768 x 2304, rank 64, 13.2 against 27.2, in runs 13.5 against 9.1; 64 x 768 x 2304, rank
+// 32, 13.8 against 29.6, in runs 13.7 against 8.6, rank 64, 25.8 against 46.7, in runs 23.9
+// against 9.5. More rows than one operand of 64, only while all of them are few CTAs:
+// 128 x 512 x 1536 (24 tiles of W by rows), rank 8, 16 adapters, 8.9 against 15.6; 256 x
+// 4096 x 1024 (32), rank 32, 25.0 against 40.9; 192 x 512 x 1536 (36), 8 adapters of rank
+// 16, 18.9 against 11.2. 512 x 512 x 512, rank 32, 20.2 against 33.0, in runs 20.8 against
+// 10.6: more than 8192 values of h are left to the tiles.
 bool by_rows(const ck_lora_args& a) {
   if (a.M <= 32) return true;
   if (a.rank > 32) return false;
@@ -1127,9 +1128,9 @@ int make_plan(const ck_lora_args& a, LoraPlan& pl) {
 }
 
 // early: its successor may start beside it. That pays where the successor streams
-// W with a CTA or two an SM (48 rows x 4096 x 4096: 24.6 against 28.7 us); the
+// W with a CTA or two an SM (captured, 48 rows x 4096 x 4096: 17.8 against 21.0 us); the
 // fp32 tiles would crowd on the SMs that this kernel leaves free (301 x 256 x 768
-// 16.5 against 13.1 us, 128 x 4096 x 4096 220 against 161).
+// 15.8 against 12.7 us, 128 x 4096 x 4096 214 against 156).
 template <typename T>
 int shrink(const LoraParams& p, int early, cudaStream_t st) {
   const ck_lora_args& a = p.a;

@@ -7,8 +7,10 @@
 // (kv_proj's layout, the rows of StreamingKVCache). Position j of sequence b is
 // row j % page_size of page page_table[b, j / page_size].
 //
-// The call reads every live row once and does 2 G flop per byte (bf16, G query
-// heads to a K|V head), so HBM bounds it. The positions of all sequences make one
+// The call does 2 G flop per byte (bf16, G query heads to a K|V head), so HBM bounds
+// it. Every live row is read once where the G query heads make one unit (up to 16 in
+// bf16, 4 in fp32), else once a unit, side by side and so mostly from L2 (16 sequences
+// of 3000 to 16384 positions, fp32, 32 heads over 4 of 64: 111 us for 258 MB). The positions of all sequences make one
 // list of tiles of 16 or 32, cut into equal runs however ragged the lengths are;
 // a warp takes one run for one unit (the query heads of one K|V head, at most GT
 // of them), the warps of one run side by side, so that the pieces of a row are
@@ -27,9 +29,11 @@
 //
 // All statistics are fp32 in the log2 domain (s log2(e), 2^x).
 //
-// Measured: 16 sequences of 3000 to 32768 positions, 32 heads over 8 of 128, 840 MB,
-// 141 us a call (6.0 TB/s); 32 sequences of 32 to 4096, 12 heads of 64, with weights
-// 30 us (25 for the stream, 2.8 TB/s); 300 positions, 8 heads of 64, 4.6 us.
+// Measured (captured, a call): 16 sequences of 3000 to 32768 positions, 32 heads over 8 of
+// 128, 840 MB, 138 us (6.1 TB/s); 32 sequences of 32 to 4096, 12 heads of 64, 86 MB, with
+// weights 30 us (2.9 TB/s), without 27; 300 positions, 8 heads of 64, 4.3 us. Short rows
+// are bound by their instructions too: more than 500 a tile of 8 KB, and with one query
+// head to a K|V head six of the eight columns of every product and softmax are empty.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -206,14 +210,19 @@ struct Heads;
 // P goes from S^T's accumulator layout to the B operand by an 8 x 8 transpose
 // (movmatrix) as the sum of two bf16 numbers of the same sign, so that an infinite value
 // stays one, the second what the first lost: one
-// alone leaves an error of 2^-8 sum p |v|, as large as the result's own rounding. The
-// tensor pipe has the room (captured, us, with and without the second: 8 sequences of 8000
-// to 32000 positions, 12 heads of 64, 78.5 / 79.1; 32 of 32 to 4096 with weights 29.9 /
-// 29.6; 16 of 3000 to 32768, 32 heads over 2 of 128, 60.3 / 57.4). l sums the fp32 values.
+// alone leaves an error of 2^-8 sum p |v|, as large as the result's own rounding
+// (captured, us, with and without the second: 8 sequences of 8000 to 32000 positions, 12
+// heads of 64, 78.5 / 79.0; 32 of 32 to 4096 with weights 29.8 / 29.6; one of 1000, 8 heads
+// of 64, 7.0 / 6.7; 16 of 3000 to 32768, 32 heads over 2 of 128, 60.3 / 57.5). l sums the
+// fp32 values.
+// Up to four heads stand in the eight columns twice, so that one product takes both
+// parts, columns 0-3 the first ones, columns 4-7 the second (two products: 30.05 for the
+// 29.8 above).
 template <int DH, int GT>
 struct Heads<__nv_bfloat16, DH, GT> {
   using R = Ring<__nv_bfloat16, DH>;
-  static constexpr int NT = GT / 8;
+  static constexpr bool TWICE = GT == 4;
+  static constexpr int NT = TWICE ? 1 : GT / 8;
   static constexpr int KS = DH / 16;
   static constexpr int Q_FLOATS = 0;
   uint32_t q[NT][KS][2];
@@ -225,7 +234,7 @@ struct Heads<__nv_bfloat16, DH, GT> {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       // lane (g, t) holds head g's elements 2t, 2t + 1 of every 8
-      const int h = nt * 8 + g;
+      const int h = TWICE ? g & 3 : nt * 8 + g;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(
           reinterpret_cast<const __nv_bfloat16*>(p.a.q) + (int64_t)b * p.a.q_ld_b +
           (int64_t)(h0 + h) * p.a.q_ld_h + 2 * t);
@@ -336,8 +345,12 @@ struct Heads<__nv_bfloat16, DH, GT> {
         two_bf16x2(p2, p3, high[1], low[1]);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          ph[u][nt][r] = transpose8x8(high[r]);
-          pl[u][nt][r] = transpose8x8(low[r]);
+          if (TWICE) {
+            ph[u][nt][r] = transpose8x8(t < 2 ? high[r] : low[r]);
+          } else {
+            ph[u][nt][r] = transpose8x8(high[r]);
+            pl[u][nt][r] = transpose8x8(low[r]);
+          }
         }
       }
     }
@@ -351,7 +364,7 @@ struct Heads<__nv_bfloat16, DH, GT> {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           mma16816(o[nt][i], a.x, a.y, a.z, a.w, ph[u][nt][0], ph[u][nt][1]);
-          mma16816(o[nt][i], a.x, a.y, a.z, a.w, pl[u][nt][0], pl[u][nt][1]);
+          if (!TWICE) mma16816(o[nt][i], a.x, a.y, a.z, a.w, pl[u][nt][0], pl[u][nt][1]);
         }
       }
   }
@@ -374,13 +387,21 @@ struct Heads<__nv_bfloat16, DH, GT> {
         float ls;
         total(nt, e, ls);
         const int h = nt * 8 + 2 * t + e;
+        float sum[KS][2];  // both parts
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            sum[i][r] = o[nt][i][2 * r + e];
+            if (TWICE) sum[i][r] += __shfl_xor_sync(0xffffffffu, sum[i][r], 2);
+          }
         if (h < nh) {
           if (g == 0) put_ml(h, m[nt][e], ls);
           const float f = !normalise ? 1.f : (ls == 0.f ? 0.f : 1.f / ls);
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
-            put(h, 16 * i + g, f == 0.f && normalise ? 0.f : o[nt][i][e] * f);
-            put(h, 16 * i + g + 8, f == 0.f && normalise ? 0.f : o[nt][i][2 + e] * f);
+            put(h, 16 * i + g, f == 0.f && normalise ? 0.f : sum[i][0] * f);
+            put(h, 16 * i + g + 8, f == 0.f && normalise ? 0.f : sum[i][1] * f);
           }
         }
       }
@@ -777,7 +798,8 @@ __global__ void __launch_bounds__(NW * 32) paged_stream_kernel(const PagedParams
 // its sums away and keeps the other half, so 9 shuffles serve 8 rows instead
 // of 40, and lane L ends with the score of row L / 4. The exponentials are then
 // one per lane for all 8 rows. Bound by its instructions: 16 sequences of 3000 to
-// 32768 positions, 32 heads over 8 of 96, 963 us.
+// 32768 positions, 32 heads over 8 of 96, 965 us, a tenth of the copy rate: rows of
+// 192 bytes that are aligned could go through a ring as well.
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float* f) {
@@ -1094,7 +1116,7 @@ int make_plan(const ck_paged_attention_args& a, Plan& pl) {
             (a.page_ld * es) % 16 == 0 && (a.row_ld * es) % 16 == 0 && (a.q_ld_b * es) % 16 == 0 &&
             (a.q_ld_h * es) % 16 == 0;
   if (pl.ring && a.dtype == CK_BF16) {
-    p.gt = p.G <= 8 ? 8 : 16;
+    p.gt = p.G <= 4 ? 4 : (p.G <= 8 ? 8 : 16);
   } else {
     p.gt = p.G == 1 ? 1 : 4;
     const bool v4 = aligned16(a.pool) && a.page_ld % 4 == 0 && a.row_ld % 4 == 0 && a.Dh % 4 == 0;
@@ -1108,9 +1130,9 @@ int make_plan(const ck_paged_attention_args& a, Plan& pl) {
   p.n_chunks = 1;
   if (pl.ring) {
     // One block a unit and no parts (one launch) for short tables, as long as
-    // every block finds an SM: against runs and a join, us a call, 8 heads of 64
-    // in bf16 4.2 / 7.5 at 300 positions, 6.7 / 7.7 at 1024, 11.0 / 9.7 at 2048;
-    // 4 heads of 64 in fp32 5.4 / 7.4 at 300, 11.1 / 8.8 at 1000.
+    // every block finds an SM: against runs and a join, us a call (captured), 8 heads
+    // of 64 in bf16 4.3 / 7.6 at 300 positions, 7.1 / 7.8 at 1024, 11.7 / 9.8 at 2048;
+    // 4 heads of 64 in fp32 5.3 / 7.4 at 300, 11.1 / 8.9 at 1000.
     pl.parts = a.w_out != nullptr || p.cap > 1024 || p.cap * a.Dh * es > 128 * 1024 || seqs > sms;
     const int workers = stream_blocks(a.Dh * (int)es) * NWARP;
     p.runs = workers / (p.units < workers ? p.units : workers);
@@ -1161,12 +1183,11 @@ int run_ring(const Plan& pl, cudaStream_t st) {
   return launch_stream<T, DH, GT, NWARP, false>(pl.p, stream_blocks(DH * (int)sizeof(T)), st);
 }
 
-template <typename T, int A, int B>
+template <typename T, int GT>
 int run_dh(const Plan& pl, cudaStream_t st) {
-  const bool wide = pl.p.gt == B;
-  if (pl.p.a.Dh == 32) return wide ? run_ring<T, 32, B>(pl, st) : run_ring<T, 32, A>(pl, st);
-  if (pl.p.a.Dh == 64) return wide ? run_ring<T, 64, B>(pl, st) : run_ring<T, 64, A>(pl, st);
-  return wide ? run_ring<T, 128, B>(pl, st) : run_ring<T, 128, A>(pl, st);
+  if (pl.p.a.Dh == 32) return run_ring<T, 32, GT>(pl, st);
+  if (pl.p.a.Dh == 64) return run_ring<T, 64, GT>(pl, st);
+  return run_ring<T, 128, GT>(pl, st);
 }
 
 template <typename T, int VEC, int NV>
@@ -1201,7 +1222,12 @@ int paged_attention(const ck_paged_attention_args& a, void* ws, size_t ws_bytes,
   p.scores = a.w_out != nullptr ? reinterpret_cast<float*>(w + pl.off_s) : nullptr;
   const bool bf = a.dtype == CK_BF16;
   if (pl.ring) {
-    rc = bf ? run_dh<__nv_bfloat16, 8, 16>(pl, st) : run_dh<float, 1, 4>(pl, st);
+    if (bf)
+      rc = p.gt == 4   ? run_dh<__nv_bfloat16, 4>(pl, st)
+           : p.gt == 8 ? run_dh<__nv_bfloat16, 8>(pl, st)
+                       : run_dh<__nv_bfloat16, 16>(pl, st);
+    else
+      rc = p.gt == 1 ? run_dh<float, 1>(pl, st) : run_dh<float, 4>(pl, st);
   } else if (bf) {
     if (pl.vec == 4)
       rc = pl.nv == 1 ? launch_simt<__nv_bfloat16, 4, 1>(p, st) : launch_simt<__nv_bfloat16, 4, 2>(p, st);
